@@ -47,7 +47,7 @@ typedef enum s2r_grammar_kind {
   S2R_GRAMMAR_TABLE = 1  /* synthetic [states, vocab] table grammar */
 } s2r_grammar_kind;
 
-typedef enum s2r_dtype { S2R_F32 = 0, S2R_BF16 = 1 } s2r_dtype;
+typedef enum s2r_dtype { S2R_F32 = 0, S2R_BF16 = 1, S2R_F16 = 2 /* s2r_sample and s2r_shared_attention only */ } s2r_dtype;
 
 /* Decoder shape and engine sizes.
  * Replaces DecoderConfig (decoder.py:12-21) plus the BatchDecoder constructor
@@ -292,6 +292,57 @@ int32_t s2r_free_pages(s2r_ctx* ctx);
  * engine.py:316-317,349-350, inside its engine). */
 int32_t s2r_masked_argmax_noalloc(const float* logits, const float* bias, const uint8_t* allowed, int32_t rows,
                                   int32_t vocab, int64_t* out, void* stream);
+
+#define S2R_SAMPLE_MAX_ROWS 65536
+#define S2R_SAMPLE_MAX_VOCAB 524288
+
+/* Arguments of s2r_sample.  Device memory throughout; strides in elements. */
+typedef struct s2r_sample_args {
+  const void* logits;     /* [rows, vocab], each row contiguous */
+  int64_t logits_stride;  /* between rows (0: every row the same logits) */
+  int32_t logits_dtype;   /* s2r_dtype */
+  int32_t rows;           /* 1 .. S2R_SAMPLE_MAX_ROWS */
+  int32_t vocab;          /* 1 .. S2R_SAMPLE_MAX_VOCAB */
+  const float* bias;      /* [vocab] added in float32, or NULL */
+  const uint8_t* allowed; /* [rows, vocab] non-zero = allowed, or NULL (all) */
+  int64_t allowed_stride; /* between rows (0: one mask for all) */
+  const float* uniforms;  /* [rows] in [0, 1) */
+  /* per row [rows], or NULL for the value given below */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all; /* >= 0; 0: the largest allowed logit, as s2r_masked_argmax_noalloc */
+  int32_t top_k_all;     /* >= 0; 0: no limit */
+  float top_p_all;       /* 0 .. 1; 1: no limit */
+  float min_p_all;       /* 0 .. 1; 0: no limit */
+  int64_t* tokens;       /* [rows] */
+  float* logprobs;       /* [rows] or NULL */
+} s2r_sample_args;
+
+/* Draw one token per row from the allowed tokens, with given uniforms.  With
+ * x = float32(logit) + bias, M its largest allowed value and w = exp((x - M) /
+ * temperature), tokens ordered by value (descending) and then index: top_k
+ * keeps the first k, top_p the shortest prefix holding a share p of what is
+ * left (at least one token), min_p of those the ones with w >= min_p (the best
+ * always stays).  tokens[r] is the lowest index whose running sum of kept
+ * weights exceeds uniforms[r] times their total, logprobs[r] its
+ * log-probability among the allowed tokens before temperature and filters
+ * (x - M - log sum exp(x - M)).  The weights are summed in 64-bit fixed point,
+ * so the draw does not depend on how the work was split.
+ *
+ * A row with nothing allowed, or whose best allowed value is -inf, gives token
+ * 0 and -inf; a NaN among the allowed values gives the lowest such index and
+ * NaN; a best value of +inf its lowest index and 0; temperature 0 the lowest
+ * index of the best value.  Per-row parameters out of range: a temperature
+ * that is negative or NaN counts as 0, top_k < 0 as 0, top_p above 1 or NaN as
+ * 1 and below 0 as 0, min_p below 0 or NaN as 0 and above 1 as 1.  Uniforms
+ * below 0 or NaN count as 0, those of 1 or more draw the last kept token.
+ *
+ * One launch, no scratch memory, asynchronous on `stream` of the current
+ * device; calls may overlap and be captured (offsets are 64-bit).  No
+ * counterpart in the reference, which decodes greedily (engine.py:349-350). */
+int32_t s2r_sample(const s2r_sample_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libs2r.so"
 
 S2R_OK, S2R_EINVAL, S2R_ECUDA, S2R_ENOMEM, S2R_ESTATE, S2R_ENOTSUP, S2R_EDEVICE = range(7)
-S2R_F32, S2R_BF16 = 0, 1
+S2R_F32, S2R_BF16, S2R_F16 = 0, 1, 2
 S2R_NO_TARGET = (1 << 63) - 1
 S2R_FLAG_NO_PDL, S2R_FLAG_NO_GRAPH = 1, 2
 S2R_FLAG_NO_TENSOR_CORE = 32
@@ -79,6 +79,30 @@ class Rescore(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("logits_stride", C.c_int64),
+        ("logits_dtype", C.c_int32),
+        ("rows", C.c_int32),
+        ("vocab", C.c_int32),
+        ("bias", C.c_void_p),
+        ("allowed", C.c_void_p),
+        ("allowed_stride", C.c_int64),
+        ("uniforms", C.c_void_p),
+        ("temperature", C.c_void_p),
+        ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p),
+        ("temperature_all", C.c_float),
+        ("top_k_all", C.c_int32),
+        ("top_p_all", C.c_float),
+        ("min_p_all", C.c_float),
+        ("tokens", C.c_void_p),
+        ("logprobs", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/s2r.h declares.
 SIGNATURES = {
     "s2r_abi_version": (C.c_int32, []),
@@ -108,6 +132,7 @@ SIGNATURES = {
                                    C.POINTER(C.c_int32), C.c_int32, C.POINTER(C.c_int32)]),
     "s2r_masked_argmax_noalloc": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
                                               C.c_void_p]),
+    "s2r_sample": (C.c_int32, [C.POINTER(SampleArgs), C.c_void_p]),
 }
 
 _lib = None
