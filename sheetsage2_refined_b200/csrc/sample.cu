@@ -12,17 +12,21 @@
 //   logprob x_t - M - log sum_allowed exp(x - M): the token's log-probability
 //           before temperature and filters, to rank readings by.
 //
-// Every filter keeps a prefix of one order, so what is kept is "value above a
+// Every filter keeps a prefix of one order, so what is kept is "values above a
 // threshold, and the first few of the threshold's ties".  The threshold is
-// found by an adaptive radix search over the order-preserving 32-bit images
-// of the values: 2048 bins over the range still open, up to 3 rounds, with
-// counts (top-k) or weights (top-p) summed per bin.
+// found in two exchanges: a histogram of counts (top-k) or weights (top-p) over
+// 1024 bins linear in M - x, which a decoder's logits fill evenly, then the
+// tokens of the bin in which the sum crosses its target, gathered and sorted.
+// When that bin holds more than 2048 tokens (masses of equal values) a radix
+// search over the 32-bit images of the values takes over.
 //
 // Weights are fixed-point integers, rint(exp(.) * 2^(61 - bits(vocab))), with
 // the exponential in 64 bits: which token is drawn depends on which side of a
 // border a running sum falls, integer sums do not depend on the order in
 // which threads add, and the rounding (2^-46 of the largest weight at 32,576
-// tokens) is far below what a 32-bit sum could resolve.
+// tokens) is far below what a 32-bit sum could resolve.  Tokens whose weight
+// rounds to 0 cannot be drawn and are left out from the start.  With top-k the
+// counts come first, so that only the k survivors need the exponential.
 //
 // A row is one thread-block cluster of C CTAs, each holding a contiguous
 // share of the vocabulary as images in shared memory; sums cross the cluster
@@ -50,11 +54,16 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048;
 constexpr int kSampleBinBits = 11;
 constexpr int kSampleMaxSplits = 16;
+constexpr int kSampleLinear = 1024;  // bins of the first histogram
+constexpr int kSampleListMax = 2048;  // tokens of its crossing bin that are gathered and sorted
 constexpr uint32_t kImgNegInf = 0x007fffffu;  // image of -inf: tokens at or below it are never drawn
 constexpr uint32_t kImgPosInf = 0xff800000u;
 
 struct SampleShared {
-  u64 hist[2][kSampleBins];  // by parity of the search round, so one cluster barrier per round suffices
+  u64 hist[2][kSampleBins];  // by parity of the exchange, so one cluster barrier each suffices; also the lists
+  u64 sorted[kSampleListMax];
+  double pow2[64];           // 2^(j / 64)
+  unsigned listed;
   u64 part[kSampleWarps];    // per-warp values of a block reduction
   u64 cta[2][2];             // this CTA's values of an exchange, by parity
   u64 scan[kSampleWarps];
@@ -87,8 +96,9 @@ struct RowSampler {
   int w0, w1;           // this warp's part of the share
   int turn = 0;         // exchanges done (parity of the buffers)
   float best;
-  double inv_t;
-  double scale;
+  float cut;     // tokens with best - x >= cut weigh nothing
+  double inv_t;  // 1 / (T ln 2)
+  int scale_bits;
 
   __device__ void barrier() {
     if (C > 1)
@@ -151,11 +161,22 @@ struct RowSampler {
     return s;
   }
 
-  // rint(exp((x - best) / T) * scale)
+  // rint(exp((x - best) / T) * 2^scale_bits): y = (x - best) / (T ln 2) = k / 64 + f, 2^y =
+  // 2^(k >> 6) * pow2[k & 63] * 2^f with |f| <= 1/128 (the table-driven exponential of Tang, 1989),
+  // 2^f by its series: the first term left out is (ln2 / 128)^6 / 720 = 4e-17.
   __device__ u64 weight(uint32_t u) {
-    if (u <= kImgNegInf) return 0;
-    const double d = ((double)image_value(u) - (double)best) * inv_t;
-    return __double2ull_rn(exp(d) * scale);
+    const double y = ((double)image_value(u) - (double)best) * inv_t;  // (T's factor holds 1 / ln 2)
+    if (!(y > -62.0 - 1.0)) return 0;
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low word
+    const double shifted = fma(y, 64.0, magic);
+    const int k = __double2loint(shifted);
+    const double f = fma(shifted - magic, -0.015625, y);
+    double q = fma(f, 0x1.5d87fe78a6730p-10, 0x1.3b2ab6fba4e77p-7);
+    q = fma(f, q, 0x1.c6b08d704a0bfp-5);
+    q = fma(f, q, 0x1.ebfbdff82c58ep-3);
+    q = fma(f, q, 0x1.62e42fefa39efp-1);
+    const double m = sh.pow2[k & 63] * fma(f, q, 1.0);
+    return __double2ull_rn(m * __hiloint2double(((k >> 6) + scale_bits + 1023) << 20, 0));
   }
 };
 
@@ -166,10 +187,15 @@ struct Kept {
   __device__ bool has(uint32_t u, int i) const { return u > lo || (u == lo && i <= last); }
 };
 
-// Shrinks `kept` to the shortest prefix of the order whose sum of value(image) reaches
-// `target` (1 <= target <= the sum over `kept`).  COUNT: value = 1, else the weight.
+// The shortest prefix of `kept` whose sum of value(token) reaches `target` (1 <= target <= the sum
+// over `kept`), by radix rounds over the images.  COUNT: value = 1, else the weight.
+// Out of line and by value: rare, and the common path's state stays in registers.
+struct RadixResult {
+  Kept kept;
+  int turn;
+};
 template <bool COUNT>
-__device__ void shrink(RowSampler& row, Kept& kept, u64 target) {
+__device__ __noinline__ RadixResult shrink_radix(RowSampler row, Kept kept, u64 target) {
   SampleShared& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t lo = kept.lo + (kept.last < 0 ? 1u : 0u), hi = value_image(row.best);  // open range, both inclusive
@@ -239,7 +265,7 @@ __device__ void shrink(RowSampler& row, Kept& kept, u64 target) {
         kept.lo = lo - 1;
         kept.last = -1;
       }
-      return;
+      return RadixResult{kept, row.turn};
     }
   }
   // one value is left: its ties are taken in index order
@@ -250,7 +276,7 @@ __device__ void shrink(RowSampler& row, Kept& kept, u64 target) {
       kept.lo = lo - 1;
       kept.last = -1;
     }
-    return;
+    return RadixResult{kept, row.turn};
   }
   u64 mine = 0;
   for (int i = row.w0 + lane; i < row.w1; i += 32) mine += row.img[i] == lo && kept.has(lo, row.first + i);
@@ -286,6 +312,162 @@ __device__ void shrink(RowSampler& row, Kept& kept, u64 target) {
   for (int r = 0; r < row.C; ++r) last += row.peer(all, r)[0];
   kept.lo = lo;
   kept.last = (int)last - 1;
+  return RadixResult{kept, row.turn};
+}
+
+// The same through the histogram that fill_histogram left in sh.hist[(turn - 1) & 1], one barrier
+// after it was filled: `per_unit` bins per unit of best - x.  `total`, if given, receives the sum over
+// `kept` and `share` of it is the target.
+template <bool COUNT>
+__device__ void shrink(RowSampler& row, Kept& kept, float per_unit, u64 target, const float* share) {
+  SampleShared& sh = row.sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64* hist = sh.hist[(row.turn - 1) & 1];
+  constexpr int kPer = kSampleLinear / kSampleThreads;  // bin 0 holds the largest values
+  const int b0 = (int)threadIdx.x * kPer;
+  u64 v[kPer], sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) v[j] = 0;
+  if (COUNT) {
+    for (int r = 0; r < row.C; ++r) {
+      const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint32_t*>(row.peer(hist, r)) + b0);
+      v[0] += x.x;
+      v[1] += x.y;
+    }
+  } else {
+    for (int r = 0; r < row.C; ++r) {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(row.peer(hist, r) + b0);
+      v[0] += x.x;
+      v[1] += x.y;
+    }
+  }
+  static_assert(kPer == 2, "two bins a thread");
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) sum += v[j];
+  u64 incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) sh.scan[warp] = incl;
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+  u64 run = incl - sum, all = 0;
+  for (int w = 0; w < kSampleWarps; ++w) {
+    if (w < warp) run += sh.scan[w];
+    all += sh.scan[w];
+  }
+  if (share) {  // a share of the whole sum
+    const double goal = ceil((double)*share * (double)all);
+    target = goal < 1.0 ? 1ull : (u64)goal;
+  }
+  if (target >= all && COUNT) return;  // nothing to leave out
+  target = target > all ? all : target;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (run < target && run + v[j] >= target) {
+      sh.found[0] = (u64)(b0 + j);
+      sh.part[0] = run;
+    }
+    run += v[j];
+  }
+  __syncthreads();
+  const int bin = (int)sh.found[0];
+  const u64 above = sh.part[0];
+  // ---- the tokens of the crossing bin
+  u64* list = sh.hist[row.turn & 1];
+  for (int i = row.w0 + lane; i < row.w1; i += 32) {
+    const uint32_t u = row.img[i];
+    if (u <= kImgNegInf) continue;
+    const float d = row.best - image_value(u);
+    if (d < row.cut && min(kSampleLinear - 1, (int)(d * per_unit)) == bin && kept.has(u, row.first + i)) {
+      const unsigned at = atomicAdd(&sh.listed, 1u);
+      if (at < (unsigned)kSampleListMax) list[at] = ((u64)u << 32) | (uint32_t)~(uint32_t)(row.first + i);
+    }
+  }
+  __syncthreads();
+  const u64* counts = row.exchange(sh.listed, 0);
+  unsigned n = 0;
+  for (int r = 0; r < row.C; ++r) n += (unsigned)row.peer(counts, r)[0];
+  if (n > (unsigned)kSampleListMax) {
+    const RadixResult res = shrink_radix<COUNT>(row, kept, target);
+    kept = res.kept;
+    row.turn = res.turn;
+    return;
+  }
+  int padded = 32;
+  while (padded < (int)n) padded *= 2;
+  unsigned from = 0;
+  for (int r = 0; r < row.C; ++r) {
+    const unsigned c = (unsigned)row.peer(counts, r)[0];
+    const u64* theirs = row.peer(list, r);
+    for (unsigned i = threadIdx.x; i < c; i += kSampleThreads) sh.sorted[from + i] = theirs[i];
+    from += c;
+  }
+  for (unsigned i = n + threadIdx.x; i < (unsigned)padded; i += kSampleThreads) sh.sorted[i] = 0;
+  __syncthreads();
+  for (int size = 2; size <= padded; size *= 2)  // bitonic, descending
+    for (int step = size / 2; step > 0; step /= 2) {
+      for (int i = threadIdx.x; i < padded / 2; i += kSampleThreads) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const u64 x = sh.sorted[lo], y = sh.sorted[hi];
+        if ((x < y) == ((lo & size) == 0)) {
+          sh.sorted[lo] = y;
+          sh.sorted[hi] = x;
+        }
+      }
+      __syncthreads();
+    }
+  // ---- the entry at which the running sum reaches the target (warp 0)
+  if (warp == 0) {
+    u64 before = above;
+    for (int i0 = 0; i0 < (int)n; i0 += 32) {
+      const u64 key = i0 + lane < (int)n ? sh.sorted[i0 + lane] : 0ull;
+      u64 s = key ? (COUNT ? 1ull : row.weight((uint32_t)(key >> 32))) : 0ull;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + s >= target);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) sh.found[0] = key;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, s, 31);
+    }
+  }
+  __syncthreads();
+  kept.lo = (uint32_t)(sh.found[0] >> 32);
+  kept.last = (int)~(uint32_t)sh.found[0];
+}
+
+// Bins of best - x over the row's kept tokens, of counts or weights, behind one cluster barrier.
+template <bool COUNT>
+__device__ void fill_histogram(RowSampler& row, const Kept& kept, float per_unit) {
+  u64* hist = row.sh.hist[row.turn & 1];
+  ++row.turn;
+  __syncthreads();
+  constexpr int kWords = kSampleLinear * (COUNT ? 1 : 2);
+  for (int b = threadIdx.x; b < kWords; b += kSampleThreads) reinterpret_cast<uint32_t*>(hist)[b] = 0;
+  __syncthreads();
+  for (int i = row.w0 + (int)(threadIdx.x & 31); i < row.w1; i += 32) {
+    const uint32_t u = row.img[i];
+    if (u <= kImgNegInf) continue;
+    const float d = row.best - image_value(u);
+    if (!(d < row.cut) || !kept.has(u, row.first + i)) continue;
+    uint32_t* bin = reinterpret_cast<uint32_t*>(hist) + min(kSampleLinear - 1, (int)(d * per_unit)) * (COUNT ? 1 : 2);
+    if (COUNT) {
+      atomicAdd(bin, 1u);
+    } else {  // 64-bit sum from 32-bit atomics: exactly the add that wraps the low word carries
+      const u64 w = row.weight(u);
+      const uint32_t low = (uint32_t)w, old = atomicAdd(bin, low);
+      const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
+      if (high) atomicAdd(bin + 1, high);
+    }
+  }
+  row.barrier();
 }
 
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
@@ -297,12 +479,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   const int first = min(a.vocab, rank * a.chunk), n = min(a.vocab - first, a.chunk);
   const int per_warp = ((a.chunk + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;
   const int w0 = min(n, warp * per_warp), w1 = min(n, w0 + per_warp);
+  if (threadIdx.x < 64) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
   pdl_wait();
 
   // ---- images of the allowed tokens; the largest
   const size_t at = (size_t)r * a.logits_stride + first;
   const uint8_t* allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride + first : nullptr;
-  uint32_t top = 0;
+  uint32_t top = 0, bottom = 0xffffffffu;  // bottom: the lowest drawable value
 #pragma unroll 4
   for (int i = w0 + lane; i < w1; i += 32) {
     float x = load_logit(a.logits, a.dtype, at + i);
@@ -310,31 +493,41 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
     const uint32_t u = (!allowed || allowed[i]) ? value_image(x) : 0u;
     img[i] = u;
     top = u > top ? u : top;
+    if (u > kImgNegInf) bottom = u < bottom ? u : bottom;
   }
   RowSampler row{sh, img, first, n, C, rank, w0, w1};
   {
-    const u64* all = row.exchange(row.block_max(top), 0);
-    for (int p = 0; p < C; ++p) top = max(top, (uint32_t)row.peer(all, p)[0]);
+    top = __reduce_max_sync(0xffffffffu, top);
+    bottom = __reduce_min_sync(0xffffffffu, bottom);
+    if (lane == 0) sh.part[warp] = ((u64)top << 32) | bottom;
+    __syncthreads();
+    for (int w = 0; w < kSampleWarps; ++w) {
+      top = max(top, (uint32_t)(sh.part[w] >> 32));
+      bottom = min(bottom, (uint32_t)sh.part[w]);
+    }
+    const u64* all = row.exchange(((u64)top << 32) | bottom, 0);
+    for (int p = 0; p < C; ++p) {
+      const u64 x = row.peer(all, p)[0];
+      top = max(top, (uint32_t)(x >> 32));
+      bottom = min(bottom, (uint32_t)x);
+    }
   }
   const float t = a.temperature ? a.temperature[r] : a.temperature_all;
   const bool finite = top > kImgNegInf && top < kImgPosInf;
   const float best = finite ? image_value(top) : 0.f;
   row.best = best;
-  row.inv_t = 1.0 / (double)t;
-  row.scale = a.scale;
+  row.inv_t = 1.4426950408889634 / (double)t;
+  row.scale_bits = a.scale_bits;
+  row.cut = a.cut * t;
   const bool greedy = !finite || !(t > 0.f);
 
-  // ---- sum of exp(x - best) for the log-probability, and of the weights (or the greedy index)
+  // ---- sum of exp(x - best) for the log-probability, and the greedy index
   float z = 0.f;
-  u64 sum = 0;
   int lowest = INT_MAX;
   for (int i = w0 + lane; i < w1; i += 32) {
     const uint32_t u = img[i];
     if (greedy && u == top) lowest = min(lowest, i);
-    if (finite && u > kImgNegInf) {
-      z += expf(image_value(u) - best);
-      if (!greedy) sum += row.weight(u);
-    }
+    if (finite && u > kImgNegInf) z += __expf(image_value(u) - best);
   }
   z = warp_sum(z);
   // the float sums cross the block and the cluster in a fixed order
@@ -343,31 +536,26 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   __syncthreads();
   z = 0.f;
   for (int w = 0; w < kSampleWarps; ++w) z += __uint_as_float((uint32_t)sh.part[w]);
-  u64 total = row.block_sum(sum), before = 0;
-  const u64 block_low = greedy ? ~row.block_max(~(u64)(lowest == INT_MAX ? 0xffffffffu : (uint32_t)(first + lowest))) : 0;
-  {
-    const u64* all = row.exchange(greedy ? block_low : total, __float_as_uint(z));
-    total = 0;
+  if (greedy) {
+    const u64 low = ~row.block_max(~(u64)(lowest == INT_MAX ? 0xffffffffu : (uint32_t)(first + lowest)));
+    const u64* all = row.exchange(low, __float_as_uint(z));
     z = 0.f;
-    u64 low = 0xffffffffu;
+    u64 lowest_all = 0xffffffffu;
     for (int p = 0; p < C; ++p) {
       const u64* x = row.peer(all, p);
-      if (greedy) low = x[0] < low ? x[0] : low;
-      else total += x[0];
+      lowest_all = x[0] < lowest_all ? x[0] : lowest_all;
       z += __uint_as_float((uint32_t)x[1]);
     }
-    if (greedy) {
-      if (rank == 0 && threadIdx.x == 0) {
-        a.tokens[r] = top > kImgNegInf ? (int64_t)low : 0;
-        if (a.logprobs)
-          a.logprobs[r] = finite ? -logf(z)
-                          : top <= kImgNegInf ? -INFINITY
-                          : top == kImgPosInf ? 0.f
-                                              : __uint_as_float(0x7fc00000u);
-      }
-      row.barrier();  // peers have read this CTA's values
-      return;
+    if (rank == 0 && threadIdx.x == 0) {
+      a.tokens[r] = top > kImgNegInf ? (int64_t)lowest_all : 0;
+      if (a.logprobs)
+        a.logprobs[r] = finite ? -logf(z)
+                        : top <= kImgNegInf ? -INFINITY
+                        : top == kImgPosInf ? 0.f
+                                            : __uint_as_float(0x7fc00000u);
     }
+    row.barrier();  // peers have read this CTA's values
+    return;
   }
 
   // ---- the filters
@@ -375,34 +563,26 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   const int k = a.top_k ? a.top_k[r] : a.top_k_all;
   const float p = a.top_p ? a.top_p[r] : a.top_p_all;
   const float m = a.min_p ? a.min_p[r] : a.min_p_all;
+  float per_unit = fminf((float)kSampleLinear / fminf(row.cut, best - image_value(bottom)), 3e38f);
   if (k > 0 && k < a.vocab) {
-    u64 live = 0;
-    for (int i = w0 + lane; i < w1; i += 32) live += img[i] > kImgNegInf;
-    live = row.cluster_sum(row.block_sum(live), nullptr);
-    if ((u64)k < live) {
-      shrink<true>(row, kept, (u64)k);
-      sum = 0;
-      for (int i = w0 + lane; i < w1; i += 32)
-        if (kept.has(img[i], first + i)) sum += row.weight(img[i]);
-      total = row.cluster_sum(row.block_sum(sum), nullptr);
-    }
+    fill_histogram<true>(row, kept, per_unit);
+    shrink<true>(row, kept, per_unit, (u64)k, nullptr);
+    if (kept.lo > kImgNegInf) per_unit = fminf((float)kSampleLinear / (best - image_value(kept.lo)), 3e38f);
   }
   if (p < 1.f) {
-    const double goal = ceil((double)p * (double)total);
-    u64 target = goal < 1.0 ? 1ull : (u64)goal;
-    target = target > total ? total : target;
-    shrink<false>(row, kept, target);
+    fill_histogram<false>(row, kept, per_unit);
+    shrink<false>(row, kept, per_unit, 0, &p);
   }
-  const double floor_w = m > 0.f ? (double)fminf(m, 1.f) : 0.0;
+  const u64 floor_w = m > 0.f ? (u64)ceil((double)fminf(m, 1.f) * (double)(1ull << a.scale_bits)) : 0ull;
   auto kept_weight = [&](int i) -> u64 {
     const uint32_t u = img[i];
     if (!kept.has(u, first + i) || u <= kImgNegInf) return 0;
-    const double e = exp(((double)image_value(u) - (double)best) * row.inv_t);
-    return e >= floor_w ? __double2ull_rn(e * row.scale) : 0ull;
+    const u64 w = row.weight(u);
+    return w >= floor_w ? w : 0ull;
   };
 
   // ---- the token: running sums in index order
-  sum = 0;
+  u64 sum = 0, before = 0;
   for (int i = w0 + lane; i < w1; i += 32) sum += kept_weight(i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -410,7 +590,17 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   const u64 block = row.block_sum(lane == 0 ? mine : 0ull);
   u64 run = 0;
   for (int w = 0; w < warp; ++w) run += sh.part[w];
-  total = row.cluster_sum(block, &before);
+  u64 total = 0;
+  {
+    const u64* all = row.exchange(block, __float_as_uint(z));
+    z = 0.f;
+    for (int q = 0; q < C; ++q) {
+      const u64* x = row.peer(all, q);
+      if (q < rank) before += x[0];
+      total += x[0];
+      z += __uint_as_float((uint32_t)x[1]);
+    }
+  }
   run += before;
   const float uniform = a.uniforms[r];
   u64 target = uniform > 0.f ? (u64)((double)uniform * (double)total) : 0ull;
@@ -461,7 +651,8 @@ int launch_sample(SampleArgs a, cudaStream_t stream, const char** why) {
   a.chunk = (a.vocab + a.splits - 1) / a.splits;
   int bits = 0;
   while ((1ll << bits) <= a.vocab) ++bits;
-  a.scale = (double)(1ull << (61 - bits));
+  a.scale_bits = 61 - bits;
+  a.cut = (float)(a.scale_bits + 2) * 0.69315f;  // exp(-cut) * 2^scale_bits < 1/2
   const size_t smem = sizeof(SampleShared) + (size_t)a.chunk * sizeof(uint32_t);
   *why = "launch failed";
   if (cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
