@@ -36,8 +36,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <climits>
+#include <atomic>
 #include <cstdio>
+#include <mutex>
 
 #include "../../include/s2r.h"
 #include "common.cuh"
@@ -51,23 +52,25 @@ typedef unsigned long long u64;
 
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 2048;
-constexpr int kSampleBinBits = 11;
+constexpr int kSampleBins = 1024;  // of either histogram
+constexpr int kSampleBinBits = 10;
 constexpr int kSampleMaxSplits = 16;
-constexpr int kSampleLinear = 1024;  // bins of the first histogram
-constexpr int kSampleListMax = 2048;  // tokens of its crossing bin that are gathered and sorted
+constexpr int kSampleListMax = 1024;   // tokens of the crossing bin that are gathered and sorted
+constexpr int kSampleFinishMax = 256;  // kept tokens that one CTA finishes alone
 constexpr uint32_t kImgNegInf = 0x007fffffu;  // image of -inf: tokens at or below it are never drawn
 constexpr uint32_t kImgPosInf = 0xff800000u;
 
-struct SampleShared {
-  u64 hist[2][kSampleBins];  // by parity of the exchange, so one cluster barrier each suffices; also the lists
-  u64 sorted[kSampleListMax];
-  double pow2[64];           // 2^(j / 64)
-  unsigned listed;
-  u64 part[kSampleWarps];    // per-warp values of a block reduction
-  u64 cta[2][2];             // this CTA's values of an exchange, by parity
+struct alignas(16) SampleShared {  // (the images behind it are stored four at a time)
+  u64 hist[2][kSampleBins];             // by parity of the exchange, so one cluster barrier each suffices
+  u64 cross[kSampleListMax];            // this CTA's tokens of the crossing bin
+  u64 survive[kSampleFinishMax];        // ... and of it and the bins above
+  u64 sorted[kSampleListMax];           // the cluster's, in order
+  u64 inbox[2][kSampleMaxSplits][2];    // what the peers sent, by parity of the exchange
+  u64 part[kSampleWarps];               // per-warp values of a block reduction
   u64 scan[kSampleWarps];
+  double pow2[64];                      // 2^(j / 64)
   u64 found[2];
+  unsigned crossing, surviving;
 };
 
 // Order-preserving image of a float (select.cuh): -0 as +0, every NaN on top.
@@ -81,18 +84,79 @@ __device__ __forceinline__ float image_value(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-__device__ __forceinline__ float load_logit(const void* p, int dtype, size_t i) {
-  if (dtype == S2R_F32) return static_cast<const float*>(p)[i];
-  if (dtype == S2R_BF16) return __bfloat162float(static_cast<const bf16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+// This warp's images [w0, w1) of the allowed tokens (0: masked) into shared memory, and the largest
+// and the lowest drawable of each lane.  VEC: the row's logits, mask and bias allow four tokens a load.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_images(const T* __restrict__ logits, const float* __restrict__ bias,
+                                            const uint8_t* __restrict__ allowed, uint32_t* img, int w0, int w1,
+                                            uint32_t& top, uint32_t& bottom) {
+  constexpr int kEach = VEC ? 4 : 1;
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int i = w0 + lane * kEach; i < w1; i += 32 * kEach) {
+    float x[kEach];
+    bool ok[kEach];
+    if constexpr (VEC) {
+      alignas(16) T raw[4];
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(logits + i));
+      else
+        *reinterpret_cast<uint2*>(raw) = __ldg(reinterpret_cast<const uint2*>(logits + i));
+      const uint32_t m = allowed ? __ldg(reinterpret_cast<const uint32_t*>(allowed + i)) : 0xffffffffu;
+      const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = bias ? __fadd_rn(to_float(raw[j]), bb[j]) : to_float(raw[j]);
+        ok[j] = ((m >> (8 * j)) & 0xffu) != 0;
+      }
+    } else {
+      x[0] = to_float(logits[i]);
+      if (bias) x[0] = __fadd_rn(x[0], bias[i]);
+      ok[0] = !allowed || allowed[i];
+    }
+    uint32_t u[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      u[j] = ok[j] ? value_image(x[j]) : 0u;
+      top = u[j] > top ? u[j] : top;
+      if (u[j] > kImgNegInf) bottom = u[j] < bottom ? u[j] : bottom;
+    }
+    if constexpr (VEC)
+      *reinterpret_cast<uint4*>(img + i) = make_uint4(u[0], u[1], u[2], u[3]);
+    else
+      img[i] = u[0];
+  }
 }
 
-// One row's search state; every thread of the cluster holds the same values.
+template <typename T>
+__device__ __forceinline__ void load_images(const SampleArgs& a, int r, int first, uint32_t* img, int w0, int w1,
+                                            uint32_t& top, uint32_t& bottom) {
+  const T* logits = static_cast<const T*>(a.logits) + (size_t)r * a.logits_stride + first;
+  const uint8_t* allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride + first : nullptr;
+  const float* bias = a.bias ? a.bias + first : nullptr;
+  // w0 and first are multiples of 4; only a row's last tokens can be fewer
+  const bool vec = reinterpret_cast<uintptr_t>(logits) % (4 * sizeof(T)) == 0 &&
+                   reinterpret_cast<uintptr_t>(allowed) % 4 == 0 && reinterpret_cast<uintptr_t>(bias) % 16 == 0;
+  int from = w0;
+  if (vec) {
+    from = w0 + (w1 - w0) / 4 * 4;
+    load_images<T, true>(logits, bias, allowed, img, w0, from, top, bottom);
+  }
+  load_images<T, false>(logits, bias, allowed, img, from, w1, top, bottom);
+}
+
+// One row's search state; every thread of the cluster (of C CTAs) holds the same values.
+template <int C>
 struct RowSampler {
   SampleShared& sh;
   const uint32_t* img;  // this CTA's images
-  int first, n;         // its share of the vocabulary
-  int C, rank;
+  int first;            // its share of the vocabulary
+  int rank;
   int w0, w1;           // this warp's part of the share
   int turn = 0;         // exchanges done (parity of the buffers)
   float best;
@@ -123,42 +187,18 @@ struct RowSampler {
     for (int w = 0; w < kSampleWarps; ++w) s += sh.part[w];
     return s;
   }
-  __device__ u64 block_max(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const u64 x = __shfl_xor_sync(0xffffffffu, v, o);
-      v = x > v ? x : v;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    u64 s = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) s = sh.part[w] > s ? sh.part[w] : s;
-    return s;
-  }
-  // Publish a block-uniform pair to the cluster; afterwards peer(sh.cta[t & 1], r) holds rank r's.
-  __device__ const u64* exchange(u64 a, u64 b) {
-    u64* mine = sh.cta[turn & 1];
+  // Send a block-uniform pair to every CTA of the cluster; behind the barrier inbox[r] holds rank
+  // r's.  Senders write into the peers' memory, so what follows reads only this CTA's own.
+  __device__ const u64 (*exchange(u64 a, u64 b))[2] {
+    u64(*box)[2] = sh.inbox[turn & 1];
     ++turn;
-    if (threadIdx.x == 0) {
-      mine[0] = a;
-      mine[1] = b;
+    if (threadIdx.x < C) {
+      u64* dst = peer(box[rank], (int)threadIdx.x);
+      dst[0] = a;
+      dst[1] = b;
     }
     barrier();
-    return mine;
-  }
-  // Sums over the cluster and over the ranks below this one.
-  __device__ u64 cluster_sum(u64 block_value, u64* before) {
-    const u64* mine = exchange(block_value, 0);
-    u64 s = 0, lo = 0;
-    for (int r = 0; r < C; ++r) {
-      const u64 x = peer(mine, r)[0];
-      if (r < rank) lo += x;
-      s += x;
-    }
-    if (before) *before = lo;
-    return s;
+    return box;
   }
 
   // rint(exp((x - best) / T) * 2^scale_bits): y = (x - best) / (T ln 2) = k / 64 + f, 2^y =
@@ -194,8 +234,8 @@ struct RadixResult {
   Kept kept;
   int turn;
 };
-template <bool COUNT>
-__device__ __noinline__ RadixResult shrink_radix(RowSampler row, Kept kept, u64 target) {
+template <bool COUNT, int C>
+__device__ __noinline__ RadixResult shrink_radix(RowSampler<C> row, Kept kept, u64 target) {
   SampleShared& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t lo = kept.lo + (kept.last < 0 ? 1u : 0u), hi = value_image(row.best);  // open range, both inclusive
@@ -221,7 +261,8 @@ __device__ __noinline__ RadixResult shrink_radix(RowSampler row, Kept kept, u64 
     u64 v[kPer], sum = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) v[j] = 0;
-    for (int r = 0; r < row.C; ++r) {
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
       const u64* h = row.peer(hist, r);
 #pragma unroll
       for (int j = 0; j < kPer; ++j) v[j] += h[b1 - j];
@@ -284,10 +325,9 @@ __device__ __noinline__ RadixResult shrink_radix(RowSampler row, Kept kept, u64 
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   const u64 block = row.block_sum(lane == 0 ? mine : 0ull);  // leaves the warps' counts in sh.part
   u64 before = 0;
-  u64 in_block = 0;
-  for (int w = 0; w < warp; ++w) in_block += sh.part[w];
-  row.cluster_sum(block, &before);
-  before += in_block;
+  for (int w = 0; w < warp; ++w) before += sh.part[w];
+  const u64(*blocks)[2] = row.exchange(block, 0);
+  for (int r = 0; r < row.rank; ++r) before += blocks[r][0];
   __syncthreads();
   if (threadIdx.x == 0) sh.found[1] = 0;
   __syncthreads();
@@ -307,123 +347,197 @@ __device__ __noinline__ RadixResult shrink_radix(RowSampler row, Kept kept, u64 
     }
   }
   __syncthreads();
-  const u64* all = row.exchange(sh.found[1], 0);
+  const u64(*all)[2] = row.exchange(sh.found[1], 0);
   u64 last = 0;
-  for (int r = 0; r < row.C; ++r) last += row.peer(all, r)[0];
+#pragma unroll
+  for (int r = 0; r < C; ++r) last += all[r][0];
   kept.lo = lo;
   kept.last = (int)last - 1;
   return RadixResult{kept, row.turn};
 }
 
-// The same through the histogram that fill_histogram left in sh.hist[(turn - 1) & 1], one barrier
-// after it was filled: `per_unit` bins per unit of best - x.  `total`, if given, receives the sum over
-// `kept` and `share` of it is the target.
-template <bool COUNT>
-__device__ void shrink(RowSampler& row, Kept& kept, float per_unit, u64 target, const float* share) {
-  SampleShared& sh = row.sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const u64* hist = sh.hist[(row.turn - 1) & 1];
-  constexpr int kPer = kSampleLinear / kSampleThreads;  // bin 0 holds the largest values
-  const int b0 = (int)threadIdx.x * kPer;
-  u64 v[kPer], sum = 0;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) v[j] = 0;
-  if (COUNT) {
-    for (int r = 0; r < row.C; ++r) {
-      const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint32_t*>(row.peer(hist, r)) + b0);
-      v[0] += x.x;
-      v[1] += x.y;
-    }
-  } else {
-    for (int r = 0; r < row.C; ++r) {
-      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(row.peer(hist, r) + b0);
-      v[0] += x.x;
-      v[1] += x.y;
-    }
-  }
-  static_assert(kPer == 2, "two bins a thread");
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) sum += v[j];
-  u64 incl = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
-  }
-  if (lane == 31) sh.scan[warp] = incl;
-  if (threadIdx.x == 0) sh.listed = 0;
-  __syncthreads();
-  u64 run = incl - sum, all = 0;
-  for (int w = 0; w < kSampleWarps; ++w) {
-    if (w < warp) run += sh.scan[w];
-    all += sh.scan[w];
-  }
-  if (share) {  // a share of the whole sum
-    const double goal = ceil((double)*share * (double)all);
-    target = goal < 1.0 ? 1ull : (u64)goal;
-  }
-  if (target >= all && COUNT) return;  // nothing to leave out
-  target = target > all ? all : target;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (run < target && run + v[j] >= target) {
-      sh.found[0] = (u64)(b0 + j);
-      sh.part[0] = run;
-    }
-    run += v[j];
-  }
-  __syncthreads();
-  const int bin = (int)sh.found[0];
-  const u64 above = sh.part[0];
-  // ---- the tokens of the crossing bin
-  u64* list = sh.hist[row.turn & 1];
-  for (int i = row.w0 + lane; i < row.w1; i += 32) {
-    const uint32_t u = row.img[i];
-    if (u <= kImgNegInf) continue;
-    const float d = row.best - image_value(u);
-    if (d < row.cut && min(kSampleLinear - 1, (int)(d * per_unit)) == bin && kept.has(u, row.first + i)) {
-      const unsigned at = atomicAdd(&sh.listed, 1u);
-      if (at < (unsigned)kSampleListMax) list[at] = ((u64)u << 32) | (uint32_t)~(uint32_t)(row.first + i);
-    }
-  }
-  __syncthreads();
-  const u64* counts = row.exchange(sh.listed, 0);
-  unsigned n = 0;
-  for (int r = 0; r < row.C; ++r) n += (unsigned)row.peer(counts, r)[0];
-  if (n > (unsigned)kSampleListMax) {
-    const RadixResult res = shrink_radix<COUNT>(row, kept, target);
-    kept = res.kept;
-    row.turn = res.turn;
-    return;
-  }
-  int padded = 32;
-  while (padded < (int)n) padded *= 2;
-  unsigned from = 0;
-  for (int r = 0; r < row.C; ++r) {
-    const unsigned c = (unsigned)row.peer(counts, r)[0];
-    const u64* theirs = row.peer(list, r);
-    for (unsigned i = threadIdx.x; i < c; i += kSampleThreads) sh.sorted[from + i] = theirs[i];
-    from += c;
-  }
-  for (unsigned i = n + threadIdx.x; i < (unsigned)padded; i += kSampleThreads) sh.sorted[i] = 0;
-  __syncthreads();
-  for (int size = 2; size <= padded; size *= 2)  // bitonic, descending
+// Sort sh.sorted[0, padded) (a power of two), largest first.
+__device__ __forceinline__ void sort_descending(u64* v, int padded) {
+  for (int size = 2; size <= padded; size *= 2)  // bitonic
     for (int step = size / 2; step > 0; step /= 2) {
       for (int i = threadIdx.x; i < padded / 2; i += kSampleThreads) {
         const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const u64 x = sh.sorted[lo], y = sh.sorted[hi];
+        const u64 x = v[lo], y = v[hi];
         if ((x < y) == ((lo & size) == 0)) {
-          sh.sorted[lo] = y;
-          sh.sorted[hi] = x;
+          v[lo] = y;
+          v[hi] = x;
         }
       }
+      // pairs within 32 entries belong to one warp from step 16 down
+      if (step > 32)
+        __syncthreads();
+      else
+        __syncwarp();
+      if (step == 1 || step == 64) __syncthreads();
+    }
+}
+
+// The cluster's lists one after the other into sh.sorted, filled up with zeros to a power of two.
+template <int C>
+__device__ __forceinline__ int gather(RowSampler<C>& row, const u64* list, const unsigned (&count)[C], unsigned n) {
+  int padded = 32;
+  while (padded < (int)n) padded *= 2;
+  unsigned from = 0;
+#pragma unroll
+  for (int r = 0; r < C; ++r) {
+    const u64* theirs = row.peer(list, r);
+    for (unsigned i = threadIdx.x; i < count[r]; i += kSampleThreads) row.sh.sorted[from + i] = theirs[i];
+    from += count[r];
+  }
+  for (unsigned i = n + threadIdx.x; i < (unsigned)padded; i += kSampleThreads) row.sh.sorted[i] = 0;
+  __syncthreads();
+  return padded;
+}
+
+// Inclusive sums over the block's threads.
+__device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  if (lane == 31) sh.scan[warp] = v;
+  __syncthreads();
+  u64 sum = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) {
+    if (w < warp) v += sh.scan[w];
+    sum += sh.scan[w];
+  }
+  *all = sum;
+  return v;
+}
+
+__device__ __forceinline__ u64 share_of(float share, u64 all) {  // the least sum that holds a share
+  const double goal = ceil((double)share * (double)all);
+  return goal < 1.0 ? 1ull : goal >= (double)all ? all : (u64)goal;
+}
+
+struct DrawArgs {  // what is left of a row once its survivors are gathered
+  int k;
+  float p, uniform;
+  u64 floor_w;
+};
+
+enum Shrunk { kShrunkAll, kShrunk, kShrunkDone };
+
+// Cuts `kept` to its first k tokens (COUNT) or to the shortest prefix that holds a share p of its
+// weight, from the histogram that fill_histogram left in sh.hist[(turn - 1) & 1] behind a barrier
+// (`per_unit` bins per unit of best - x).  Where at most kSampleFinishMax tokens lie in the crossing
+// bin and above, rank 0 applies all filters to them, draws the token and leaves it in sh.found:
+// its key and kShrunkDone.  `z_sum`: in this CTA's sum of exponentials, out the row's.
+template <bool COUNT, int C>
+__device__ Shrunk shrink(RowSampler<C>& row, Kept& kept, float per_unit, const DrawArgs& d, float& z_sum) {
+  SampleShared& sh = row.sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64* hist = sh.hist[(row.turn - 1) & 1];
+  constexpr int kPer = kSampleBins / kSampleThreads;  // bin 0 holds the largest values
+  static_assert(kPer == 2, "two bins a thread");
+  const int b0 = (int)threadIdx.x * kPer;
+  u64 v0 = 0, v1 = 0;
+#pragma unroll
+  for (int r = 0; r < C; ++r) {
+    if (COUNT) {
+      const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint32_t*>(row.peer(hist, r)) + b0);
+      v0 += x.x;
+      v1 += x.y;
+    } else {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(row.peer(hist, r) + b0);
+      v0 += x.x;
+      v1 += x.y;
+    }
+  }
+  if (threadIdx.x == 0) sh.crossing = sh.surviving = 0;
+  u64 all = 0;
+  const u64 incl = block_scan(sh, v0 + v1, &all);
+  u64 target = COUNT ? (u64)d.k : share_of(d.p, all);
+  if (COUNT && target >= all) return kShrunkAll;  // nothing to leave out
+  const u64 run = incl - v0 - v1;
+  if (run < target && incl >= target) {
+    const bool second = run + v0 < target;
+    sh.found[0] = (u64)(b0 + second);
+    sh.found[1] = second ? run + v0 : run;
+  }
+  __syncthreads();
+  const int bin = (int)sh.found[0];
+  const u64 above = sh.found[1];
+  // ---- the tokens of the crossing bin, and with those above it
+  for (int i = row.w0 + lane; i < row.w1; i += 32) {
+    const uint32_t u = row.img[i];
+    if (u <= kImgNegInf) continue;
+    const float gap = row.best - image_value(u);
+    const int b = min(kSampleBins - 1, (int)(gap * per_unit));
+    if (gap < row.cut && b <= bin && kept.has(u, row.first + i)) {
+      const u64 key = ((u64)u << 32) | (uint32_t)~(uint32_t)(row.first + i);
+      const unsigned s = atomicAdd(&sh.surviving, 1u);
+      if (s < (unsigned)kSampleFinishMax) sh.survive[s] = key;
+      if (b == bin) {
+        const unsigned at = atomicAdd(&sh.crossing, 1u);
+        if (at < (unsigned)kSampleListMax) sh.cross[at] = key;
+      }
+    }
+  }
+  __syncthreads();
+  const u64(*box)[2] = row.exchange(((u64)sh.surviving << 32) | sh.crossing, __float_as_uint(z_sum));
+  unsigned n_survive = 0, n_cross = 0, survive[C], cross[C];
+  float z = 0.f;
+#pragma unroll
+  for (int r = 0; r < C; ++r) {
+    survive[r] = (unsigned)(box[r][0] >> 32);
+    cross[r] = (unsigned)box[r][0];
+    n_survive += survive[r];
+    n_cross += cross[r];
+    z += __uint_as_float((uint32_t)box[r][1]);
+  }
+  z_sum = z;
+  if (n_survive <= (unsigned)kSampleFinishMax) {
+    if (row.rank != 0) return kShrunkDone;
+    const int padded = gather(row, sh.survive, survive, n_survive);
+    sort_descending(sh.sorted, padded);
+    const int i = (int)threadIdx.x;
+    const u64 key = i < (int)n_survive ? sh.sorted[i] : 0ull;
+    u64 w = key && (!COUNT || i < d.k) ? row.weight((uint32_t)(key >> 32)) : 0ull;
+    if (!COUNT || d.p < 1.f) {
+      u64 sum = 0;
+      const u64 to = block_scan(sh, w, &sum);
+      if (to - w >= (COUNT ? share_of(d.p, sum) : target)) w = 0;
       __syncthreads();
     }
-  // ---- the entry at which the running sum reaches the target (warp 0)
-  if (warp == 0) {
+    if (w < d.floor_w) w = 0;
+    u64 total = 0;
+    block_scan(sh, w, &total);
+    // running sums in index order: the entry whose own weight crosses the target
+    if (i < kSampleFinishMax) sh.cross[i] = w;
+    __syncthreads();
+    u64 goal = d.uniform > 0.f ? (u64)((double)d.uniform * (double)total) : 0ull;
+    goal = goal >= total ? total - 1 : goal;
+    if (w) {
+      u64 to = 0;
+      for (int j = 0; j < (int)n_survive; ++j)
+        if ((uint32_t)sh.sorted[j] >= (uint32_t)key) to += sh.cross[j];  // the low word holds ~index
+      if (to > goal && to - w <= goal) sh.found[0] = key;
+    }
+    __syncthreads();
+    return kShrunkDone;
+  }
+  if (n_cross > (unsigned)kSampleListMax) {
+    const RadixResult res = shrink_radix<COUNT, C>(row, kept, target);
+    kept = res.kept;
+    row.turn = res.turn;
+    return kShrunk;
+  }
+  const int padded = gather(row, sh.cross, cross, n_cross);
+  sort_descending(sh.sorted, padded);
+  if (warp == 0) {  // the entry at which the running sum reaches the target
     u64 before = above;
-    for (int i0 = 0; i0 < (int)n; i0 += 32) {
-      const u64 key = i0 + lane < (int)n ? sh.sorted[i0 + lane] : 0ull;
+    for (int i0 = 0; i0 < (int)n_cross; i0 += 32) {
+      const u64 key = i0 + lane < (int)n_cross ? sh.sorted[i0 + lane] : 0ull;
       u64 s = key ? (COUNT ? 1ull : row.weight((uint32_t)(key >> 32))) : 0ull;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -441,23 +555,26 @@ __device__ void shrink(RowSampler& row, Kept& kept, float per_unit, u64 target, 
   __syncthreads();
   kept.lo = (uint32_t)(sh.found[0] >> 32);
   kept.last = (int)~(uint32_t)sh.found[0];
+  return kShrunk;
 }
 
 // Bins of best - x over the row's kept tokens, of counts or weights, behind one cluster barrier.
-template <bool COUNT>
-__device__ void fill_histogram(RowSampler& row, const Kept& kept, float per_unit) {
+// SUM: on the way, this thread's part of sum exp(x - best) over the allowed tokens.
+template <bool COUNT, bool SUM, int C>
+__device__ float fill_histogram(RowSampler<C>& row, const Kept& kept, float per_unit) {
   u64* hist = row.sh.hist[row.turn & 1];
-  ++row.turn;
-  __syncthreads();
-  constexpr int kWords = kSampleLinear * (COUNT ? 1 : 2);
+  constexpr int kWords = kSampleBins * (COUNT ? 1 : 2);
   for (int b = threadIdx.x; b < kWords; b += kSampleThreads) reinterpret_cast<uint32_t*>(hist)[b] = 0;
   __syncthreads();
+  float z = 0.f;
+#pragma unroll 2
   for (int i = row.w0 + (int)(threadIdx.x & 31); i < row.w1; i += 32) {
     const uint32_t u = row.img[i];
     if (u <= kImgNegInf) continue;
-    const float d = row.best - image_value(u);
-    if (!(d < row.cut) || !kept.has(u, row.first + i)) continue;
-    uint32_t* bin = reinterpret_cast<uint32_t*>(hist) + min(kSampleLinear - 1, (int)(d * per_unit)) * (COUNT ? 1 : 2);
+    const float gap = row.best - image_value(u);
+    if (SUM) z += __expf(-gap);
+    if (!(gap < row.cut) || !kept.has(u, row.first + i)) continue;
+    uint32_t* bin = reinterpret_cast<uint32_t*>(hist) + min(kSampleBins - 1, (int)(gap * per_unit)) * (COUNT ? 1 : 2);
     if (COUNT) {
       atomicAdd(bin, 1u);
     } else {  // 64-bit sum from 32-bit atomics: exactly the add that wraps the low word carries
@@ -467,123 +584,165 @@ __device__ void fill_histogram(RowSampler& row, const Kept& kept, float per_unit
       if (high) atomicAdd(bin + 1, high);
     }
   }
-  row.barrier();
+  return z;
 }
 
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+// This CTA's sum of the threads' parts, in a fixed order.
+__device__ __forceinline__ float block_sum_f32(SampleShared& sh, float z) {
+  z = warp_sum(z);
+  if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = __float_as_uint(z);
+  __syncthreads();
+  z = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSampleWarps; ++w) z += __uint_as_float((uint32_t)sh.part[w]);
+  return z;
+}
+
+template <int C>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char sample_smem[];
   SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_smem);
   uint32_t* img = reinterpret_cast<uint32_t*>(sample_smem + sizeof(SampleShared));
-  const int C = a.splits, rank = blockIdx.x % C, r = blockIdx.x / C;
+  const int rank = (int)(blockIdx.x % C), r = (int)(blockIdx.x / C);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = min(a.vocab, rank * a.chunk), n = min(a.vocab - first, a.chunk);
-  const int per_warp = ((a.chunk + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;
+  const int per_warp = a.chunk / kSampleWarps;
   const int w0 = min(n, warp * per_warp), w1 = min(n, w0 + per_warp);
   if (threadIdx.x < 64) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
   pdl_wait();
 
-  // ---- images of the allowed tokens; the largest
-  const size_t at = (size_t)r * a.logits_stride + first;
-  const uint8_t* allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride + first : nullptr;
-  uint32_t top = 0, bottom = 0xffffffffu;  // bottom: the lowest drawable value
-#pragma unroll 4
-  for (int i = w0 + lane; i < w1; i += 32) {
-    float x = load_logit(a.logits, a.dtype, at + i);
-    if (a.bias) x = __fadd_rn(x, a.bias[first + i]);
-    const uint32_t u = (!allowed || allowed[i]) ? value_image(x) : 0u;
-    img[i] = u;
-    top = u > top ? u : top;
-    if (u > kImgNegInf) bottom = u < bottom ? u : bottom;
-  }
-  RowSampler row{sh, img, first, n, C, rank, w0, w1};
+  // ---- images of the allowed tokens; the largest and the lowest drawable value
+  uint32_t top = 0, bottom = 0xffffffffu;
+  if (a.dtype == S2R_F32)
+    load_images<float>(a, r, first, img, w0, w1, top, bottom);
+  else if (a.dtype == S2R_BF16)
+    load_images<bf16>(a, r, first, img, w0, w1, top, bottom);
+  else
+    load_images<__half>(a, r, first, img, w0, w1, top, bottom);
+  const float t = a.temperature ? a.temperature[r] : a.temperature_all;
+  DrawArgs d;
+  d.k = a.top_k ? a.top_k[r] : a.top_k_all;
+  d.p = a.top_p ? a.top_p[r] : a.top_p_all;
+  d.uniform = a.uniforms[r];
+  const float m = a.min_p ? a.min_p[r] : a.min_p_all;
+  RowSampler<C> row{sh, img, first, rank, w0, w1};
   {
     top = __reduce_max_sync(0xffffffffu, top);
     bottom = __reduce_min_sync(0xffffffffu, bottom);
     if (lane == 0) sh.part[warp] = ((u64)top << 32) | bottom;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < kSampleWarps; ++w) {
       top = max(top, (uint32_t)(sh.part[w] >> 32));
       bottom = min(bottom, (uint32_t)sh.part[w]);
     }
-    const u64* all = row.exchange(((u64)top << 32) | bottom, 0);
+    const u64(*box)[2] = row.exchange(((u64)top << 32) | bottom, 0);
+#pragma unroll
     for (int p = 0; p < C; ++p) {
-      const u64 x = row.peer(all, p)[0];
-      top = max(top, (uint32_t)(x >> 32));
-      bottom = min(bottom, (uint32_t)x);
+      top = max(top, (uint32_t)(box[p][0] >> 32));
+      bottom = min(bottom, (uint32_t)box[p][0]);
     }
   }
-  const float t = a.temperature ? a.temperature[r] : a.temperature_all;
   const bool finite = top > kImgNegInf && top < kImgPosInf;
-  const float best = finite ? image_value(top) : 0.f;
-  row.best = best;
+  row.best = finite ? image_value(top) : 0.f;
   row.inv_t = 1.4426950408889634 / (double)t;
   row.scale_bits = a.scale_bits;
   row.cut = a.cut * t;
   const bool greedy = !finite || !(t > 0.f);
-
-  // ---- sum of exp(x - best) for the log-probability, and the greedy index
+  d.floor_w = m > 0.f ? (u64)ceil((double)fminf(m, 1.f) * (double)(1ull << a.scale_bits)) : 0ull;
   float z = 0.f;
-  int lowest = INT_MAX;
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t u = img[i];
-    if (greedy && u == top) lowest = min(lowest, i);
-    if (finite && u > kImgNegInf) z += __expf(image_value(u) - best);
-  }
-  z = warp_sum(z);
-  // the float sums cross the block and the cluster in a fixed order
-  __syncthreads();
-  if (lane == 0) sh.part[warp] = __float_as_uint(z);
-  __syncthreads();
-  z = 0.f;
-  for (int w = 0; w < kSampleWarps; ++w) z += __uint_as_float((uint32_t)sh.part[w]);
+
   if (greedy) {
-    const u64 low = ~row.block_max(~(u64)(lowest == INT_MAX ? 0xffffffffu : (uint32_t)(first + lowest)));
-    const u64* all = row.exchange(low, __float_as_uint(z));
+    uint32_t lowest = 0xffffffffu;
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const uint32_t u = img[i];
+      if (u == top) lowest = min(lowest, (uint32_t)(first + i));
+      if (finite && u > kImgNegInf) z += __expf(image_value(u) - row.best);
+    }
+    __syncthreads();
+    z = block_sum_f32(sh, z);
+    lowest = __reduce_min_sync(0xffffffffu, lowest);
+    if (lane == 0) sh.scan[warp] = lowest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSampleWarps; ++w) lowest = min(lowest, (uint32_t)sh.scan[w]);
+    const u64(*box)[2] = row.exchange(lowest, __float_as_uint(z));
     z = 0.f;
-    u64 lowest_all = 0xffffffffu;
+#pragma unroll
     for (int p = 0; p < C; ++p) {
-      const u64* x = row.peer(all, p);
-      lowest_all = x[0] < lowest_all ? x[0] : lowest_all;
-      z += __uint_as_float((uint32_t)x[1]);
+      lowest = min(lowest, (uint32_t)box[p][0]);
+      z += __uint_as_float((uint32_t)box[p][1]);
     }
     if (rank == 0 && threadIdx.x == 0) {
-      a.tokens[r] = top > kImgNegInf ? (int64_t)lowest_all : 0;
+      a.tokens[r] = top > kImgNegInf ? (int64_t)lowest : 0;
       if (a.logprobs)
         a.logprobs[r] = finite ? -logf(z)
                         : top <= kImgNegInf ? -INFINITY
                         : top == kImgPosInf ? 0.f
                                             : __uint_as_float(0x7fc00000u);
     }
-    row.barrier();  // peers have read this CTA's values
+    return;  // (nothing reads a peer's memory: what was sent landed before the barrier)
+  }
+
+  // ---- the filters; the sum of exp(x - best) on the way of the first pass
+  Kept kept;
+  const float span = row.best - image_value(bottom);
+  float per_unit = fminf((float)kSampleBins / fminf(row.cut, span), 3e38f);
+  const bool by_count = d.k > 0 && d.k < a.vocab, by_share = d.p < 1.f;
+  Shrunk done = kShrunkAll;
+  bool summed = false;  // z is the row's sum
+  if (by_count) {
+    z = fill_histogram<true, true>(row, kept, per_unit);
+    z = block_sum_f32(sh, z);
+    ++row.turn;
+    row.barrier();
+    done = shrink<true>(row, kept, per_unit, d, z);
+    summed = done != kShrunkAll;
+    if (done == kShrunk) {
+      const float left = row.best - image_value(kept.lo);
+      per_unit = fminf((float)kSampleBins / left, 3e38f);
+    }
+  }
+  if (by_share && done != kShrunkDone) {
+    if (by_count) {
+      __syncthreads();
+      fill_histogram<false, false>(row, kept, per_unit);
+    } else {
+      z = fill_histogram<false, true>(row, kept, per_unit);
+      z = block_sum_f32(sh, z);
+    }
+    ++row.turn;
+    row.barrier();
+    float sum = summed ? 0.f : z;
+    done = shrink<false>(row, kept, per_unit, d, sum);
+    if (!summed) z = sum;
+    summed = true;
+  }
+  if (done == kShrunkDone) {
+    if (rank == 0 && threadIdx.x == 0) {
+      const u64 key = sh.found[0];
+      a.tokens[r] = (int64_t)~(uint32_t)key;
+      if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
+    }
+    row.barrier();  // rank 0 has read the peers' lists
     return;
   }
 
-  // ---- the filters
-  Kept kept;
-  const int k = a.top_k ? a.top_k[r] : a.top_k_all;
-  const float p = a.top_p ? a.top_p[r] : a.top_p_all;
-  const float m = a.min_p ? a.min_p[r] : a.min_p_all;
-  float per_unit = fminf((float)kSampleLinear / fminf(row.cut, best - image_value(bottom)), 3e38f);
-  if (k > 0 && k < a.vocab) {
-    fill_histogram<true>(row, kept, per_unit);
-    shrink<true>(row, kept, per_unit, (u64)k, nullptr);
-    if (kept.lo > kImgNegInf) per_unit = fminf((float)kSampleLinear / (best - image_value(kept.lo)), 3e38f);
-  }
-  if (p < 1.f) {
-    fill_histogram<false>(row, kept, per_unit);
-    shrink<false>(row, kept, per_unit, 0, &p);
-  }
-  const u64 floor_w = m > 0.f ? (u64)ceil((double)fminf(m, 1.f) * (double)(1ull << a.scale_bits)) : 0ull;
-  auto kept_weight = [&](int i) -> u64 {
-    const uint32_t u = img[i];
-    if (!kept.has(u, first + i) || u <= kImgNegInf) return 0;
-    const u64 w = row.weight(u);
-    return w >= floor_w ? w : 0ull;
-  };
-
   // ---- the token: running sums in index order
+  auto kept_weight = [&](int i, uint32_t u) -> u64 {
+    if (u <= kImgNegInf || !kept.has(u, first + i)) return 0;
+    const u64 w = row.weight(u);
+    return w >= d.floor_w ? w : 0ull;
+  };
   u64 sum = 0, before = 0;
-  for (int i = w0 + lane; i < w1; i += 32) sum += kept_weight(i);
+  const bool add_z = !by_count && !by_share;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t u = img[i];
+    if (add_z && u > kImgNegInf) z += __expf(image_value(u) - row.best);
+    sum += kept_weight(i, u);
+  }
+  __syncthreads();
+  if (add_z) z = block_sum_f32(sh, z);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const u64 mine = sum;
@@ -592,23 +751,24 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   for (int w = 0; w < warp; ++w) run += sh.part[w];
   u64 total = 0;
   {
-    const u64* all = row.exchange(block, __float_as_uint(z));
-    z = 0.f;
+    const u64(*box)[2] = row.exchange(block, __float_as_uint(z));
+    float sum_z = 0.f;
+#pragma unroll
     for (int q = 0; q < C; ++q) {
-      const u64* x = row.peer(all, q);
-      if (q < rank) before += x[0];
-      total += x[0];
-      z += __uint_as_float((uint32_t)x[1]);
+      if (q < rank) before += box[q][0];
+      total += box[q][0];
+      sum_z += __uint_as_float((uint32_t)box[q][1]);
     }
+    if (!summed) z = sum_z;
   }
   run += before;
-  const float uniform = a.uniforms[r];
-  u64 target = uniform > 0.f ? (u64)((double)uniform * (double)total) : 0ull;
+  u64 target = d.uniform > 0.f ? (u64)((double)d.uniform * (double)total) : 0ull;
   target = target >= total ? total - 1 : target;
   if (run <= target && target < run + mine) {
     for (int i0 = w0; i0 < w1; i0 += 32) {
       const int i = i0 + lane;
-      u64 s = i < w1 ? kept_weight(i) : 0ull;
+      const uint32_t u = i < w1 ? img[i] : 0u;
+      u64 s = kept_weight(i, u);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const u64 x = __shfl_up_sync(0xffffffffu, s, o);
@@ -618,60 +778,101 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
       if (hit) {
         if (lane == __ffs(hit) - 1) {
           a.tokens[r] = first + i;
-          if (a.logprobs) a.logprobs[r] = (image_value(img[i]) - best) - logf(z);
+          if (a.logprobs) a.logprobs[r] = (image_value(u) - row.best) - logf(z);
         }
         break;
       }
       run += __shfl_sync(0xffffffffu, s, 31);
     }
   }
-  row.barrier();  // peers have read this CTA's values
 }
+
+static_assert(sizeof(SampleShared) % 16 == 0, "images start 16-byte aligned");
 
 constexpr int kSampleMaxChunk = 40960;  // tokens of one CTA: 160 KB of images
 
-}  // namespace
+typedef void (*SampleFn)(const SampleArgs);
+
+SampleFn sample_fn(int splits) {
+  switch (splits) {
+    case 1: return sample_kernel<1>;
+    case 2: return sample_kernel<2>;
+    case 4: return sample_kernel<4>;
+    case 8: return sample_kernel<8>;
+    default: return sample_kernel<16>;
+  }
+}
+
+int sample_chunk(int vocab, int splits) {  // a multiple of 32 tokens a warp
+  const int per = (vocab + splits - 1) / splits;
+  return (per + kSampleWarps * 32 - 1) / (kSampleWarps * 32) * (kSampleWarps * 32);
+}
 
 // CTAs per row: enough that a CTA's share fits its shared memory, then more while the rows leave
-// SMs idle and a share is worth splitting.
-static int sample_splits(int rows, int vocab, int sms) {
+// SMs idle (two CTAs fit one) and a share is worth splitting.
+int sample_splits(int rows, int vocab, int sms) {
   int c = 1;
-  while (c < kSampleMaxSplits && (vocab + c - 1) / c > kSampleMaxChunk) c *= 2;
-  while (c < 8 && (long long)rows * c * 2 <= sms && vocab / (2 * c) >= 2048) c *= 2;
+  while (c < kSampleMaxSplits && sample_chunk(vocab, c) > kSampleMaxChunk) c *= 2;
+  while (c < 8 && (long long)rows * c * 2 <= 2 * sms && vocab / (2 * c) >= 2048) c *= 2;
   return c;
 }
 
+// Per device, once: SMs, and every instantiation allowed its shared memory and cluster size.
+struct SampleDevice {
+  int sms = 0;
+  cudaError_t error = cudaSuccess;
+};
+
+const SampleDevice& sample_device(int device) {
+  static std::mutex mu;
+  static SampleDevice devices[64];
+  static std::atomic<bool> ready[64];
+  SampleDevice& dev = devices[device];
+  if (ready[device].load(std::memory_order_acquire)) return dev;
+  std::lock_guard<std::mutex> lock(mu);
+  if (ready[device].load(std::memory_order_relaxed)) return dev;
+  dev.error = cudaDeviceGetAttribute(&dev.sms, cudaDevAttrMultiProcessorCount, device);
+  for (int c = 1; c <= kSampleMaxSplits && dev.error == cudaSuccess; c *= 2) {
+    const int smem = (int)(sizeof(SampleShared) + kSampleMaxChunk * sizeof(uint32_t));
+    dev.error = cudaFuncSetAttribute(sample_fn(c), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (dev.error == cudaSuccess && c > 8)
+      dev.error = cudaFuncSetAttribute(sample_fn(c), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (dev.error == cudaSuccess)
+      dev.error = cudaFuncSetAttribute(sample_fn(c), cudaFuncAttributePreferredSharedMemoryCarveout,
+                                       (int)cudaSharedmemCarveoutMaxShared);
+  }
+  if (dev.error == cudaSuccess) ready[device].store(true, std::memory_order_release);
+  return dev;
+}
+
+}  // namespace
+
 int launch_sample(SampleArgs a, cudaStream_t stream, const char** why) {
-  int device = 0, sms = 0;
+  int device = 0;
   *why = "no usable current device";
-  if (cudaGetDevice(&device) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return S2R_ECUDA;
-  a.splits = sample_splits(a.rows, a.vocab, sms);
-  a.chunk = (a.vocab + a.splits - 1) / a.splits;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return S2R_ECUDA;
+  const SampleDevice& dev = sample_device(device);
+  if (dev.error != cudaSuccess) return S2R_ECUDA;
+  const int splits = sample_splits(a.rows, a.vocab, dev.sms);
+  a.chunk = sample_chunk(a.vocab, splits);
   int bits = 0;
   while ((1ll << bits) <= a.vocab) ++bits;
   a.scale_bits = 61 - bits;
   a.cut = (float)(a.scale_bits + 2) * 0.69315f;  // exp(-cut) * 2^scale_bits < 1/2
-  const size_t smem = sizeof(SampleShared) + (size_t)a.chunk * sizeof(uint32_t);
   *why = "launch failed";
-  if (cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      (a.splits > 8 &&
-       cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
-    return S2R_ECUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.rows * a.splits);
+  cfg.gridDim = dim3((unsigned)a.rows * splits);
   cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.chunk * sizeof(uint32_t);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = a.splits;
+  attr.val.clusterDim.x = splits;
   attr.val.clusterDim.y = 1;
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = a.splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, sample_kernel, a) == cudaSuccess ? S2R_OK : S2R_ECUDA;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, sample_fn(splits), a) == cudaSuccess ? S2R_OK : S2R_ECUDA;
 }
 
 }  // namespace s2r

@@ -27,9 +27,9 @@ struct SampleArgs {
   int64_t* tokens;  // [rows]
   float* logprobs;  // [rows] or null
   // set by launch_sample
-  int splits, chunk;  // CTAs per row, tokens per CTA
-  int scale_bits;     // fixed-point scale of the weights: 2^scale_bits
-  float cut;          // tokens this many temperatures below the best weigh nothing
+  int chunk;       // tokens per CTA
+  int scale_bits;  // fixed-point scale of the weights: 2^scale_bits
+  float cut;       // tokens this many temperatures below the best weigh nothing
 };
 
 // Queue the kernel on `stream` of the current device; an s2r_status, and on failure why.

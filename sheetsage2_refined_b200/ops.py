@@ -22,43 +22,40 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.S2R_F32, torch.bfloat16: _lib.S2R_BF16, torch.float16: _lib.S2R_F16}
+_MASKS = (torch.uint8, torch.bool)
 
 
-def _on_device(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+def _bad(name: str, t, dtype, shape, device) -> ValueError:
+    """The error for an argument that is not a ``dtype`` tensor of ``shape`` on ``device`` with contiguous rows."""
+
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
+        return ValueError(f"{name} must be a CUDA tensor")
     if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    return t
+        return ValueError(f"{name} is on {t.device}, expected {device}")
+    return ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)} with contiguous rows, "
+                      f"not {t.dtype} {list(t.shape)} with strides {t.stride()}")
+
+
+def _vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> int:
+    """Address of a contiguous ``[n]`` tensor."""
+
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != (n,) or not (
+            n == 1 or t.stride(0) == 1):
+        raise _bad(name, t, dtype, (n,), device)
+    return t.data_ptr()
 
 
 def _call(fn, args, device: torch.device) -> None:
     """Run a C entry point with the tensors' device current and its current stream."""
 
-    stream = C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(C.byref(args), stream))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        code = fn(C.byref(args), torch.cuda.current_stream(index).cuda_stream)
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(C.byref(args), stream))
-
-
-def _vector(name: str, t: torch.Tensor, rows: int, dtype: torch.dtype, device: torch.device) -> int:
-    _on_device(name, t, device)
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or (rows > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {rows} values")
-    return t.data_ptr()
-
-
-def _matrix(name: str, t: torch.Tensor, rows: int, cols: int, device: torch.device) -> tuple[int, int]:
-    """Address and row stride (elements) of a [rows, cols] tensor whose rows are contiguous."""
-
-    _on_device(name, t, device)
-    if t.dim() == 1:
-        t = t.unsqueeze(0).expand(rows, -1)
-    if t.dim() != 2 or tuple(t.shape) != (rows, cols) or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be [{rows}, {cols}] with contiguous rows")
-    return t.data_ptr(), t.stride(0) if rows > 1 else 0
+        with torch.cuda.device(index):
+            code = fn(C.byref(args), torch.cuda.current_stream(index).cuda_stream)
+    if code:
+        _lib.check(code)
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -83,33 +80,37 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
         raise ValueError("logits must be a [rows, vocab] CUDA tensor")
     if logits.dtype not in _DTYPES:
         raise ValueError(f"logits of {logits.dtype}: float32, bfloat16 or float16 expected")
-    lib = _lib.load()
     device = logits.device
     rows, vocab = logits.shape
     if rows < 1 or vocab < 1:
         raise ValueError("logits must have at least one row and one token")
-    a = _lib.SampleArgs(logits_dtype=_DTYPES[logits.dtype], rows=rows, vocab=vocab)
-    a.logits, a.logits_stride = _matrix("logits", logits, rows, vocab, device)
-    a.uniforms = _vector("uniforms", uniforms, rows, torch.float32, device)
-    if bias is not None:
-        a.bias = _vector("bias", bias, vocab, torch.float32, device)
+    row_stride, stride = logits.stride()
+    if vocab > 1 and stride != 1:
+        raise _bad("logits", logits, logits.dtype, (rows, vocab), device)
+    mask = mask_stride = None
     if allowed is not None:
-        if not isinstance(allowed, torch.Tensor) or allowed.dtype not in (torch.uint8, torch.bool):
-            raise ValueError("allowed must be a uint8 or bool tensor")
-        a.allowed, a.allowed_stride = _matrix("allowed", allowed, rows, vocab, device)
-    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(value, torch.Tensor):
-            setattr(a, name, _vector(name, value, rows, dtype, device))
-        elif dtype == torch.int32:
-            a.top_k_all = max(-1, min(int(value), 2**31 - 1))
-        else:
-            setattr(a, name + "_all", value)
+        if not isinstance(allowed, torch.Tensor) or allowed.dtype not in _MASKS or allowed.device != device or (
+                allowed.shape not in ((rows, vocab), (vocab,))) or (vocab > 1 and allowed.stride(-1) != 1):
+            raise _bad("allowed", allowed, "uint8 or bool", (rows, vocab), device)
+        mask, mask_stride = allowed.data_ptr(), allowed.stride(0) if allowed.dim() == 2 else 0
     if out is None:
         out = torch.empty(rows, dtype=torch.int64, device=device)
     if logprobs is None:
         logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-    a.tokens = _vector("out", out, rows, torch.int64, device)
-    a.logprobs = _vector("logprobs", logprobs, rows, torch.float32, device)
-    _call(lib.s2r_sample, a, device)
+    each, values = [], []
+    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if isinstance(value, torch.Tensor):
+            each.append(_vector(name, value, rows, dtype, device))
+            values.append(0)
+        else:
+            each.append(None)
+            values.append(value if name != "top_k" else max(-1, min(int(value), 2**31 - 1)))
+    lib = _lib.load()
+    _call(lib.s2r_sample, _lib.SampleArgs(
+        logits.data_ptr(), row_stride if rows > 1 else 0, _DTYPES[logits.dtype], rows, vocab,
+        None if bias is None else _vector("bias", bias, vocab, torch.float32, device), mask, mask_stride or 0,
+        _vector("uniforms", uniforms, rows, torch.float32, device), *each, *values,
+        _vector("out", out, rows, torch.int64, device), _vector("logprobs", logprobs, rows, torch.float32, device)),
+        device)
     return out, logprobs
