@@ -47,7 +47,7 @@ typedef enum s2r_grammar_kind {
   S2R_GRAMMAR_TABLE = 1  /* synthetic [states, vocab] table grammar */
 } s2r_grammar_kind;
 
-typedef enum s2r_dtype { S2R_F32 = 0, S2R_BF16 = 1, S2R_F16 = 2 /* s2r_sample and s2r_shared_attention only */ } s2r_dtype;
+typedef enum s2r_dtype { S2R_F32 = 0, S2R_BF16 = 1, S2R_F16 = 2 /* s2r_sample, s2r_shared_attention */ } s2r_dtype;
 
 /* Decoder shape and engine sizes.
  * Replaces DecoderConfig (decoder.py:12-21) plus the BatchDecoder constructor
@@ -343,6 +343,61 @@ typedef struct s2r_sample_args {
  * device; calls may overlap and be captured (offsets are 64-bit).  No
  * counterpart in the reference, which decodes greedily (engine.py:349-350). */
 int32_t s2r_sample(const s2r_sample_args* args, void* stream);
+
+/* Arguments of s2r_shared_attention.  Device memory throughout; strides in
+ * elements, head_dim contiguous. */
+typedef struct s2r_shared_attention_args {
+  int32_t dtype;    /* S2R_BF16 or S2R_F16, of q, every K/V and out */
+  int32_t rows;     /* 1 .. 65535: one query token each */
+  int32_t heads;    /* query heads, a multiple of kv_heads, at most 4096 */
+  int32_t kv_heads;
+  int32_t head_dim; /* 64 or 128 */
+  float scale;      /* on the scores; head_dim ** -0.5 for the usual attention */
+  const void* q;    /* [rows, heads, head_dim] */
+  int64_t q_row_stride, q_head_stride;
+  /* keys and values that every row sees; 16-byte aligned, strides multiples of 8 */
+  const void* shared_k; /* [shared_tokens, kv_heads, head_dim] */
+  const void* shared_v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int32_t shared_tokens;     /* >= 0 */
+  const int32_t* shared_len; /* NULL, or one value: only the first *shared_len shared tokens are seen
+                                (clamped to 0 .. shared_tokens; read on the device, so a captured call follows it) */
+  /* each row's own keys and values, in pages of S2R_PAGE_TOKENS tokens (all NULL: none) */
+  const void* own_k; /* [own_pages][kv_heads][S2R_PAGE_TOKENS][head_dim], contiguous, 16-byte aligned */
+  const void* own_v;
+  int32_t own_pages;
+  int32_t pages_per_row;
+  const int32_t* page_table; /* [rows, pages_per_row]; entries past a row's length are not read */
+  int64_t page_table_stride; /* between rows; 0: every row the same pages */
+  const int32_t* own_len;    /* [rows] tokens of each row, 0 .. pages_per_row * S2R_PAGE_TOKENS (below 0 counts as 0) */
+  void* out;                 /* [rows, heads, head_dim] */
+  int64_t out_row_stride, out_head_stride;
+  float* lse;                /* [rows, heads] contiguous, or NULL */
+  void* workspace;           /* s2r_shared_attention_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int32_t* error;            /* NULL, or a word that the kernels set when a row's pages are broken (never cleared) */
+} s2r_shared_attention_args;
+
+/* Attention of `rows` single query tokens over one shared K/V, read once for
+ * all of them (the cross K/V of a window that several readings decode, or the
+ * K/V of a prompt they share), and over each row's own pages: with the keys
+ * [shared 0 .. S) ++ [own 0 .. own_len[r]), out = softmax(scale q.k) v and lse =
+ * log sum exp(scale q.k).  Scores, softmax and sums are float32; out is
+ * rounded once.  A row without any key gives 0 and -inf.  K/V behind a
+ * length (page tails, shared tokens past *shared_len) may hold anything,
+ * NaN included.  A row whose length exceeds its page table, or with a page
+ * index outside [0, own_pages), gives NaN and sets *error to 12 or 11; nothing
+ * outside the pool is read.
+ *
+ * Asynchronous on `stream` of the current device; calls may overlap and be
+ * captured if each has a workspace of its own, which need not be cleared.  In the
+ * reference every slot attends over its own copy of the window's cross K/V
+ * (engine.py:296-312). */
+int32_t s2r_shared_attention(const s2r_shared_attention_args* args, void* stream);
+
+/* The workspace bytes of that call (of its sizes only; pointers are checked but
+ * workspace, which is not read) on the current device. */
+int32_t s2r_shared_attention_workspace(const s2r_shared_attention_args* args, int64_t* bytes);
 
 #ifdef __cplusplus
 }

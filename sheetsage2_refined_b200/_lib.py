@@ -15,6 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libs2r.so"
 S2R_OK, S2R_EINVAL, S2R_ECUDA, S2R_ENOMEM, S2R_ESTATE, S2R_ENOTSUP, S2R_EDEVICE = range(7)
 S2R_F32, S2R_BF16, S2R_F16 = 0, 1, 2
 S2R_NO_TARGET = (1 << 63) - 1
+S2R_PAGE_TOKENS = 64
 S2R_FLAG_NO_PDL, S2R_FLAG_NO_GRAPH = 1, 2
 S2R_FLAG_NO_TENSOR_CORE = 32
 DTYPE_CODES = {0: "<f4", 1: "<V2", 2: "<i8", 3: "|u1", 4: "<f8", 5: "<i4"}
@@ -103,6 +104,42 @@ class SampleArgs(C.Structure):
     ]
 
 
+class SharedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("rows", C.c_int32),
+        ("heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("scale", C.c_float),
+        ("q", C.c_void_p),
+        ("q_row_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("shared_k", C.c_void_p),
+        ("shared_v", C.c_void_p),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("shared_tokens", C.c_int32),
+        ("shared_len", C.c_void_p),
+        ("own_k", C.c_void_p),
+        ("own_v", C.c_void_p),
+        ("own_pages", C.c_int32),
+        ("pages_per_row", C.c_int32),
+        ("page_table", C.c_void_p),
+        ("page_table_stride", C.c_int64),
+        ("own_len", C.c_void_p),
+        ("out", C.c_void_p),
+        ("out_row_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("lse", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("error", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/s2r.h declares.
 SIGNATURES = {
     "s2r_abi_version": (C.c_int32, []),
@@ -133,6 +170,8 @@ SIGNATURES = {
     "s2r_masked_argmax_noalloc": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
                                               C.c_void_p]),
     "s2r_sample": (C.c_int32, [C.POINTER(SampleArgs), C.c_void_p]),
+    "s2r_shared_attention": (C.c_int32, [C.POINTER(SharedAttentionArgs), C.c_void_p]),
+    "s2r_shared_attention_workspace": (C.c_int32, [C.POINTER(SharedAttentionArgs), C.POINTER(C.c_int64)]),
 }
 
 _lib = None

@@ -6,7 +6,10 @@ it, in the engine's own kernels (``libs2r.so``):
 
 * ``sample`` draws a token per row with temperature, top-k, top-p and min-p
   under the grammar mask and the mode bias, from uniforms the caller gives,
-  and returns its log-probability, to rank readings by (``s2r_sample``).
+  and returns its log-probability, to rank readings by (``s2r_sample``);
+* ``shared_attention`` lets many rows attend over one K/V that is read once for
+  all of them (a window's cross K/V, a common prompt's K/V) and over each row's
+  own pages (``s2r_shared_attention``).
 
 Every call is asynchronous on the current stream of its tensors' device, which
 need not be the current device.  Arguments are checked on the host and raise
@@ -114,3 +117,85 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
         _vector("out", out, rows, torch.int64, device), _vector("logprobs", logprobs, rows, torch.float32, device)),
         device)
     return out, logprobs
+
+
+def shared_attention(q: torch.Tensor, shared_k: torch.Tensor, shared_v: torch.Tensor, *,
+                     own_k: torch.Tensor | None = None, own_v: torch.Tensor | None = None,
+                     page_table: torch.Tensor | None = None, own_len: torch.Tensor | None = None,
+                     scale: float | None = None, shared_len: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                     error: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of single query tokens over one shared K/V and each row's own pages.
+
+    ``q`` ``[rows, heads, dim]``; ``shared_k`` / ``shared_v`` ``[tokens,
+    kv_heads, dim]`` (any strides that are multiples of 8 elements: a
+    ``[kv_heads, tokens, dim]`` buffer is passed transposed), bfloat16 or
+    float16, ``dim`` 64 or 128, ``heads`` a multiple of ``kv_heads``.  Row r
+    sees every shared token (the first ``shared_len`` of them, an int32 tensor
+    of one value, if given) and then the first ``own_len[r]`` tokens of the
+    pages ``page_table[r]`` names in the pools ``own_k`` / ``own_v``
+    ``[pages, kv_heads, 64, dim]`` (contiguous); ``page_table`` ``[rows,
+    pages]`` and ``own_len`` ``[rows]`` are int32.  ``scale`` defaults to
+    ``dim ** -0.5``.
+
+    Returns ``(out, lse)``: ``out`` like ``q``, ``lse`` ``[rows, heads]``
+    float32, the log of the sum of exponentials of the scaled scores.  A row
+    without keys gives 0 and ``-inf``; a row whose pages are broken gives NaN
+    and sets ``error`` (an int32 tensor of one value) if given.
+    """
+
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3:
+        raise ValueError("q must be a [rows, heads, dim] CUDA tensor")
+    dtype, device = q.dtype, q.device
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q of {dtype}: bfloat16 or float16 expected")
+    rows, heads, dim = q.shape
+    for name, t in (("shared_k", shared_k), ("shared_v", shared_v)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.dim() != 3 or (
+                t.shape != shared_k.shape or t.shape[2] != dim or t.stride(2) != 1):
+            raise _bad(name, t, dtype, ("tokens", "kv_heads", dim), device)
+    if q.stride(2) != 1:
+        raise _bad("q", q, dtype, (rows, heads, dim), device)
+    tokens, kv_heads, _ = shared_k.shape
+    own_args = (None, None, 0, 0, None, 0, None)
+    if own_k is not None or own_v is not None or page_table is not None or own_len is not None:
+        if own_k is None or own_v is None or page_table is None or own_len is None:
+            raise ValueError("own_k, own_v, page_table and own_len go together")
+        shape = (own_k.shape[0] if isinstance(own_k, torch.Tensor) and own_k.dim() else 0, kv_heads,
+                 _lib.S2R_PAGE_TOKENS, dim)
+        for name, t in (("own_k", own_k), ("own_v", own_v)):
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape or (
+                    not t.is_contiguous()):
+                raise _bad(name, t, dtype, shape, device)
+        if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or (
+                page_table.device != device or page_table.dim() != 2 or page_table.shape[0] != rows or (
+                    page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+            raise _bad("page_table", page_table, torch.int32, (rows, "pages"), device)
+        own_args = (own_k.data_ptr(), own_v.data_ptr(), shape[0], page_table.shape[1], page_table.data_ptr(),
+                    page_table.stride(0) if rows > 1 else 0, _vector("own_len", own_len, rows, torch.int32, device))
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+    elif not isinstance(out, torch.Tensor) or out.dtype != dtype or out.device != device or (
+            out.shape != q.shape or out.stride(2) != 1):
+        raise _bad("out", out, dtype, (rows, heads, dim), device)
+    if lse is None:
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=device)
+    elif not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 or lse.device != device or (
+            lse.shape != (rows, heads) or not lse.is_contiguous()):
+        raise _bad("lse", lse, torch.float32, (rows, heads), device)
+    k_token, k_head, _ = shared_k.stride()
+    v_token, v_head, _ = shared_v.stride()
+    args = _lib.SharedAttentionArgs(
+        _DTYPES[dtype], rows, heads, kv_heads, dim, dim**-0.5 if scale is None else scale,
+        q.data_ptr(), q.stride(0), q.stride(1), shared_k.data_ptr(), shared_v.data_ptr(), k_token, k_head, v_token,
+        v_head, tokens, None if shared_len is None else _vector("shared_len", shared_len, 1, torch.int32, device),
+        *own_args, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), None, 0,
+        None if error is None else _vector("error", error, 1, torch.int32, device))
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        need = C.c_int64()
+        _lib.check(lib.s2r_shared_attention_workspace(C.byref(args), C.byref(need)))
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
+        _call(lib.s2r_shared_attention, args, device)
+    return out, lse

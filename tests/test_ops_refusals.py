@@ -38,3 +38,50 @@ def test_sample_refuses_null_arguments():
 def test_sample_wrapper_refuses_host_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         ops.sample(torch.zeros(2, 8), torch.zeros(2))
+
+
+def attention_args(**kw):
+    a = _lib.SharedAttentionArgs(
+        dtype=_lib.S2R_BF16, rows=2, heads=4, kv_heads=2, head_dim=64, scale=0.125, q=16, q_row_stride=256,
+        q_head_stride=64, shared_k=16, shared_v=16, k_token_stride=128, k_head_stride=64, v_token_stride=128,
+        v_head_stride=64, shared_tokens=100, out=16, out_row_stride=256, out_head_stride=64)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+OWN = dict(own_k=16, own_v=16, own_pages=4, pages_per_row=2, page_table=16, page_table_stride=2, own_len=16)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(dtype=_lib.S2R_F32), b"bfloat16"), (dict(rows=0), b"rows"), (dict(rows=65536), b"65535"),
+    (dict(heads=5), b"multiple"), (dict(heads=0), b"heads"), (dict(kv_heads=0), b"kv_heads"),
+    (dict(heads=8192), b"4096"), (dict(shared_tokens=-1), b"shared_tokens"), (dict(shared_tokens=2**30), b"2^28"),
+    (dict(q=None), b"NULL"), (dict(out=None), b"NULL"), (dict(shared_v=None), b"NULL"), (dict(shared_k=24), b"aligned"),
+    (dict(k_token_stride=132), b"multiples of 8"), (dict(v_head_stride=65), b"multiples of 8"),
+    (dict(k_token_stride=32), b"overlap"), (dict(out_row_stride=32), b"overlap"), (dict(out_head_stride=8), b"overlap"),
+    (dict(q_row_stride=-1), b"strides"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"),
+    (dict(scale=float("inf")), b"scale"), (dict(own_k=16), b"go together"), (dict(own_len=16), b"go together"),
+    (dict(OWN, own_pages=0), b"own_pages"), (dict(OWN, pages_per_row=0), b"pages_per_row"),
+    (dict(OWN, page_table_stride=1), b"page table"), (dict(OWN, own_v=40), b"aligned"),
+])
+def test_shared_attention_entry_point_refuses(change, word):
+    lib = _lib.load()
+    assert lib.s2r_shared_attention(C.byref(attention_args(**change)), None) == _lib.S2R_EINVAL
+    assert word in lib.s2r_last_error()
+    n = C.c_int64(-1)
+    assert lib.s2r_shared_attention_workspace(C.byref(attention_args(**change)), C.byref(n)) == _lib.S2R_EINVAL
+    assert n.value == -1
+
+
+def test_shared_attention_refuses_other_head_dims_and_null_arguments():
+    lib = _lib.load()
+    assert lib.s2r_shared_attention(C.byref(attention_args(head_dim=80)), None) == _lib.S2R_ENOTSUP
+    assert lib.s2r_shared_attention(None, None) == _lib.S2R_EINVAL
+    assert lib.s2r_shared_attention_workspace(C.byref(attention_args()), None) == _lib.S2R_EINVAL
+
+
+def test_shared_attention_wrapper_refuses_host_tensors():
+    t = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.shared_attention(t, t, t)
