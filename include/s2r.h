@@ -348,7 +348,7 @@ int32_t s2r_sample(const s2r_sample_args* args, void* stream);
  * elements, head_dim contiguous. */
 typedef struct s2r_shared_attention_args {
   int32_t dtype;    /* S2R_BF16 or S2R_F16, of q, every K/V and out */
-  int32_t rows;     /* 1 .. 65535: one query token each */
+  int32_t rows;     /* 1 .. 65535: one query token each; rows * heads at most 2^24 */
   int32_t heads;    /* query heads, a multiple of kv_heads, at most 4096 */
   int32_t kv_heads;
   int32_t head_dim; /* 64 or 128 */
@@ -387,7 +387,8 @@ typedef struct s2r_shared_attention_args {
  * length (page tails, shared tokens past *shared_len) may hold anything,
  * NaN included.  A row whose length exceeds its page table, or with a page
  * index outside [0, own_pages), gives NaN and sets *error to 12 or 11; nothing
- * outside the pool is read.
+ * outside the pool is read.  (*error 13: a wait inside a kernel timed out and
+ * its rows are NaN; this means a defect of the library.)
  *
  * Asynchronous on `stream` of the current device; calls may overlap and be
  * captured if each has a workspace of its own, which need not be cleared.  In the

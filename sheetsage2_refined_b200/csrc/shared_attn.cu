@@ -11,18 +11,25 @@
 // The keys of a (row, head) are cut into parts; every part gives (m, l, o)
 // with o = sum exp(s - m) v in float32, and the parts are joined in a fixed
 // order: M = max m, out = sum_p o_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), with
-// m in units of log2.
+// m in units of log2.  Shared parts come from shared_tile_kernel (tensor
+// cores), own parts from row_attn_kernel (CUDA cores: every key is read for
+// heads / kv_heads queries only, so memory bounds it), which runs beside it.
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include "../../include/s2r.h"
 #include "common.cuh"
+#include "mbarrier.cuh"
 #include "shared_attn.cuh"
+#include "tensor_core.cuh"
 
 namespace s2r {
 namespace {
@@ -53,7 +60,7 @@ constexpr int kOwnUnroll = 4;  // key rows a lane group keeps in flight
 // One part of one row's keys for GC query heads of one kv head.  A key row is
 // read by D / 8 lanes, 16 bytes each; every such lane group keeps its own
 // online softmax over the keys it sees.
-template <typename T, int D, int GC, bool PAGED>
+template <typename T, int D, int GC>
 __global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_constant__ SharedAttnArgs a, float* part_o,
                                                                float2* part_ml, int first_part) {
   constexpr int kLanes = D / 8, kGroups = 32 / kLanes;  // lanes of a key row, key rows of a warp
@@ -67,17 +74,12 @@ __global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_cons
   __shared__ float2 sml[kOwnWarps][GC];
 
   bool broken = false;
-  int n;
-  if (PAGED) {
-    n = a.own_len[r];
-    if (n > a.pages_per_row * kPageTokens) {
-      broken = true;
-      if (threadIdx.x == 0 && a.error) atomicExch(a.error, kErrOwnLength);
-    }
-    n = broken || n < 0 ? 0 : n;
-  } else {
-    n = a.shared_len ? min(max(*a.shared_len, 0), a.shared_tokens) : a.shared_tokens;
+  int n = a.own_len[r];
+  if (n > a.pages_per_row * kPageTokens) {
+    broken = true;
+    if (threadIdx.x == 0 && a.error) atomicExch(a.error, kErrOwnLength);
   }
+  n = broken || n < 0 ? 0 : n;
   const int pages = (n + kPageTokens - 1) / kPageTokens, per = (pages + splits - 1) / splits;
   const int p0 = min(pages, part * per), p1 = min(pages, p0 + per);
 
@@ -93,24 +95,15 @@ __global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_cons
     l[i] = 0.f;
   }
   for (int p = p0 + warp; p < p1; p += kOwnWarps) {
-    const T *k, *v;
-    int64_t k_step = D, v_step = D;
-    if (PAGED) {
-      const int page = a.page_table[r * a.page_stride + p];
-      if (page < 0 || page >= a.own_pages) {
-        broken = true;
-        if (lane == 0 && a.error) atomicExch(a.error, kErrOwnPage);
-        continue;
-      }
-      const size_t base = ((size_t)page * a.kv_heads + g) * (kPageTokens * D);
-      k = static_cast<const T*>(a.own_k) + base;
-      v = static_cast<const T*>(a.own_v) + base;
-    } else {
-      k_step = a.k_token;
-      v_step = a.v_token;
-      k = static_cast<const T*>(a.shared_k) + g * a.k_head + (int64_t)p * kPageTokens * k_step;
-      v = static_cast<const T*>(a.shared_v) + g * a.v_head + (int64_t)p * kPageTokens * v_step;
+    const int page = a.page_table[r * a.page_stride + p];
+    if (page < 0 || page >= a.own_pages) {
+      broken = true;
+      if (lane == 0 && a.error) atomicExch(a.error, kErrOwnPage);
+      continue;
     }
+    const size_t base = ((size_t)page * a.kv_heads + g) * (kPageTokens * D);
+    const T* k = static_cast<const T*>(a.own_k) + base;
+    const T* v = static_cast<const T*>(a.own_v) + base;
     const int live = min(kPageTokens, n - p * kPageTokens);
 #pragma unroll 1
     for (int t0 = 0; t0 < live; t0 += kGroups * kOwnUnroll) {
@@ -119,8 +112,8 @@ __global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_cons
       for (int u = 0; u < kOwnUnroll; ++u) {
         const int t = t0 + u * kGroups + sub;
         if (t < live) {
-          load8(k + t * k_step + at, kx[u]);
-          load8(v + t * v_step + at, vx[u]);
+          load8(k + t * D + at, kx[u]);
+          load8(v + t * D + at, vx[u]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) kx[u][e] = vx[u][e] = 0.f;
@@ -191,12 +184,27 @@ __global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_cons
     part_o[dst * D + e] = acc;
     if (e == 0) part_ml[dst] = make_float2(top, sum);
   }
+  pdl_launch_dependents();
+  pdl_wait();  // this kernel runs beside the shared part; the join waits for both
+}
+
+// out and lse of one (row, head) from its joined sums, `n` channels from `d`.
+template <typename T, int N>
+__device__ __forceinline__ void store_out(const SharedAttnArgs& a, int r, int h, int d, const float (&o)[N], float sum,
+                                          float top, bool first) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key at all: 0
+  T* dst = static_cast<T*>(a.out) + r * a.out_row + h * a.out_head + d;
+#pragma unroll
+  for (int e = 0; e < N; ++e) dst[e] = T(o[e] * inv);
+  if (a.lse && first) a.lse[(size_t)r * a.heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Joins the parts of every (row, head): a warp each.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SharedAttnArgs a, const float* part_o,
                                                    const float2* part_ml, int parts) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), pairs = (int64_t)a.rows * a.heads;
   if (pair >= pairs) return;
@@ -208,55 +216,535 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
   for (int e = 0; e < kEach; ++e) acc[e] = 0.f;
   for (int p = 0; p < parts; ++p) {
     const float2 ml = part_ml[p * pairs + pair];
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-    sum += ml.x == -INFINITY ? ml.y : ml.y * f;
+    if (ml.x == -INFINITY) {  // an empty part (its o is not written): l is 0, or NaN where something broke
+      sum += ml.y;
+      continue;
+    }
+    const float f = exp2f(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
     const float* src = part_o + (size_t)(p * pairs + pair) * D + lane * kEach;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) acc[e] = fmaf(src[e], f, acc[e]);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key at all: 0
-  const int r = (int)(pair / a.heads), h = (int)(pair % a.heads);
-  T* dst = static_cast<T*>(a.out) + r * a.out_row + h * a.out_head + lane * kEach;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) dst[e] = T(acc[e] * inv);
-  if (a.lse && lane == 0) a.lse[pair] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  store_out<T>(a, (int)(pair / a.heads), (int)(pair % a.heads), lane * kEach, acc, sum, top, lane == 0);
 }
 
-template <typename T, int D, int GC>
-cudaError_t launch_rows(const SharedAttnArgs& a, cudaStream_t s) {
-  const int group = a.heads / a.kv_heads, chunks = (group + GC - 1) / GC, parts = a.shared_splits + a.own_splits;
-  const size_t pairs = (size_t)a.rows * a.heads;
-  float2* ml = static_cast<float2*>(a.workspace);
-  float* o = reinterpret_cast<float*>(ml + (parts * pairs + 1) / 2 * 2);
-  if (a.shared_splits)
-    row_attn_kernel<T, D, GC, false><<<dim3(a.shared_splits, a.kv_heads * chunks, a.rows), kOwnThreads, 0, s>>>(a, o, ml, 0);
-  if (a.own_splits)
-    row_attn_kernel<T, D, GC, true><<<dim3(a.own_splits, a.kv_heads * chunks, a.rows), kOwnThreads, 0, s>>>(
-        a, o, ml, a.shared_splits);
-  join_kernel<T, D><<<(unsigned)((pairs + 3) / 4), 128, 0, s>>>(a, o, ml, parts);
-  return cudaGetLastError();
+// ---- the shared part on tensor cores
+//
+// The queries of one kv head, (row, group member) pairs in order, are tiles of
+// 128: the MMA's M, one tensor-memory lane and one softmax thread each.  A CTA
+// walks its part of the keys in tiles of 128, with two streams in flight, each
+// with a score tile S, an output accumulator O and a warpgroup of its own:
+//
+//   one query tile (PAIR = false): the streams take the even and the odd key
+//     tiles and are joined at the end;
+//   two query tiles (PAIR = true): stream s is query tile s, both walk every
+//     key tile, which is then read once for 256 queries.
+//
+//   S = Q K^T      tcgen05.mma M128 N128 K=dim, float32 in tensor memory
+//   p = 2^(c s - m) c = scale log2(e); m trails the running maximum by at most
+//                  2^8, so that O is rescaled only when the maximum moves far
+//                  (Milakov and Gimelshein's online softmax, with slack)
+//   O += P V       P packed to 16 bits in tensor memory: the A operand; V as
+//                  it lies in memory (token rows): the B operand with the
+//                  channel axis contiguous
+//
+// Rounding: P is rounded to the tensors' 16-bit type for the product, as in
+// every 16-bit attention (half a step of each weight); l sums the unrounded
+// float32 values; O is float32 throughout.
+//
+// Warp 0 loads K and V tiles by TMA into a ring, warp 1 issues the MMAs (S0 S1 |
+// PV0 S0' | PV1 S1' | ...), warps 4-7 and 8-11 are the softmax warpgroups.
+// Tensor memory holds S twice and O twice; at dim 64 there is room for P beside
+// them, and the softmax waits for the product before it overwrites P.  At dim
+// 128 P lies in S's columns: the next S of the stream follows the product that
+// reads P, and MMAs of one accumulator shape (both 128 x 128) execute in order.
+// Every mbarrier wait is
+// bounded; on a timeout the CTA marks its rows NaN, drains its copies and MMAs
+// (bounded), frees its tensor memory and returns.
+constexpr int kTileThreads = 384;
+constexpr int kTileRows = 128;  // queries of a tile
+constexpr int kTileKeys = 128;  // keys of a tile
+constexpr int kTileBox = kTileKeys * 64 * 2;  // bytes of a 64-channel box of a tile
+constexpr int kTileCols = 512;  // tensor memory: S at 0 and 128, O at 256 and 256 + D, P: tile_p_at
+constexpr float kMaxSlack = 8.f;
+
+template <int D, bool PAIR>
+struct TileSmem {
+  static constexpr int kSlot = kTileKeys * D * 2;  // a K or V tile
+  static constexpr int kQueries = (PAIR ? 2 : 1) * kTileRows * D * 2;
+  static constexpr int kSlots = D == 64 ? 8 : 5;
+  static constexpr int kBytes = kQueries + kSlots * kSlot + 1024;  // + alignment slack
+  static_assert(kBytes + 1024 <= 227 * 1024, "fits an SM");
+  static_assert(kTileRows * (D + 4) * 4 <= kSlots * kSlot, "a stream's partial fits the ring");
+};
+
+template <int D>
+__device__ __forceinline__ uint32_t tile_p_at(int s) {  // columns of stream s's P (64)
+  return D == 64 ? 384 + s * 64 : s * kTileKeys;
+}
+
+struct TileArgs {
+  SharedAttnArgs a;
+  float* part_o;    // null: the part is the whole answer
+  float2* part_ml;
+  bool token_last;  // the tensor maps' axes are (channel, head, token) instead of (channel, token, head)
+  bool q_vector;    // q can be read 16 bytes at a time
+};
+
+template <typename T, int D, bool PAIR>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    shared_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ TileArgs t) {
+  using Smem = TileSmem<D, PAIR>;
+  constexpr int kSlots = Smem::kSlots, kBoxes = D / 64;
+  const SharedAttnArgs& a = t.a;
+  extern __shared__ __align__(1024) unsigned char tile_smem[];
+  unsigned char* base =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tile_smem) + 1023) & ~uintptr_t(1023));
+  unsigned char* sq = base;                    // query tiles: [tile][box][128 rows][128 bytes]
+  unsigned char* ring = base + Smem::kQueries;  // slot i: the i-th of K0 V0 K1 V1 ...
+  __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], s_full[2], p_full[2], pv_done[2], done;
+  __shared__ uint32_t tmem_base;
+  __shared__ int aborted;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = blockIdx.x, parts = gridDim.x, g = blockIdx.z;
+  const int group = a.heads / a.kv_heads, queries = a.rows * group;
+  const int tile0 = blockIdx.y * (PAIR ? 2 : 1);  // first query tile
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);  // one arrival per warp of the stream
+      mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(&done, 1);
+    aborted = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(kTileCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();  // the queries come from the kernel before
+  const int tokens = a.shared_len ? min(max(*a.shared_len, 0), a.shared_tokens) : a.shared_tokens;
+  const int tiles = (tokens + kTileKeys - 1) / kTileKeys, per = (tiles + parts - 1) / parts;
+  const int t0 = min(tiles, part * per), nt = min(tiles, t0 + per) - t0;
+
+  // ---- the queries, in the 128-byte-swizzled rows the MMA reads
+  for (int i = threadIdx.x; i < (PAIR ? 2 : 1) * kTileRows * (D / 8); i += kTileThreads) {
+    const int row = i / (D / 8), c = i % (D / 8), x = tile0 * kTileRows + row;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (x < queries) {
+      const T* src = static_cast<const T*>(a.q) + x / group * a.q_row + (g * group + x % group) * a.q_head + c * 8;
+      if (t.q_vector) {
+        v = *reinterpret_cast<const uint4*>(src);
+      } else {
+        const unsigned short* e = reinterpret_cast<const unsigned short*>(src);
+        v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                       e[6] | (uint32_t)e[7] << 16);
+      }
+    }
+    unsigned char* tile = sq + row / kTileRows * (kTileRows * D * 2) + c / 8 * kTileBox;
+    *reinterpret_cast<uint4*>(tile + sw128_off(row % kTileRows, c % 8)) = v;
+  }
+  fence_async_smem();
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  // Dependents may start only now: one that needs tensor memory must not take it ahead of this CTA.
+  pdl_launch_dependents();
+  const uint32_t tmem = tmem_base;
+  auto fail = [&]() {
+    if (a.error) atomicExch(a.error, kErrSharedWait);
+    *(volatile int*)&aborted = 1;
+  };
+  auto stopped = [&]() { return *(volatile int*)&aborted != 0; };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- producer
+      int issued = 0;
+      for (int i = 0; i < 2 * nt; ++i) {
+        const int slot = i % kSlots;
+        if (i >= kSlots && (!mbar_wait(&empty[slot], (i / kSlots - 1) & 1) || stopped())) {
+          fail();
+          break;
+        }
+        mbar_expect_tx(&full[slot], Smem::kSlot);
+        const CUtensorMap* map = i & 1 ? &map_v : &map_k;
+        const int token = (t0 + i / 2) * kTileKeys;
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b)
+          tma_load_3d(ring + slot * Smem::kSlot + b * kTileBox, map, b * 64, t.token_last ? g : token,
+                      t.token_last ? token : g, &full[slot]);
+        issued = i + 1;
+      }
+      // every copy has landed before the ring is reused or the CTA exits (bounded)
+      for (int i = max(0, issued - kSlots); i < issued; ++i) mbar_wait(&full[i % kSlots], (i / kSlots) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---- MMA issuer
+      constexpr uint32_t kFormat = std::is_same<T, bf16>::value ? 1u : 0u;
+      constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, kTileKeys, false);
+      constexpr uint32_t kIdescO = umma_idesc(kFormat, kTileRows, D, true);
+      bool ok = true;
+      auto issue_s = [&](int s, int k) {  // S_s = Q K_k^T
+        const int i = 2 * k, slot = i % kSlots;
+        if (!ok) return;
+        if (!mbar_wait(&full[slot], (i / kSlots) & 1) || stopped()) {
+          ok = false;
+          return;
+        }
+        tmem_fence_after();
+        const uint64_t da = umma_desc_sw128(sq + (PAIR ? s * (kTileRows * D * 2) : 0));
+        const uint64_t db = umma_desc_sw128(ring + slot * Smem::kSlot);
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) {  // 16 channels: 32 bytes of a row, a box every 64
+          const uint64_t at = (uint64_t)((e / 4) * (kTileBox >> 4) + (e % 4) * 2);
+          umma_f16(tmem + s * kTileKeys, da + at, db + at, kIdescS, e > 0);
+        }
+        umma_commit(&s_full[s]);
+        if (!PAIR || s == 1) umma_commit(&empty[slot]);
+      };
+      auto issue_pv = [&](int s, int k, int nth) {  // O_s += P_s V_k, the stream's nth product
+        const int i = 2 * k + 1, slot = i % kSlots;
+        if (!ok) return;
+        if (!mbar_wait(&p_full[s], nth & 1) || !mbar_wait(&full[slot], (i / kSlots) & 1) || stopped()) {
+          ok = false;
+          return;
+        }
+        tmem_fence_after();
+        const uint64_t db = umma_desc_mn_sw128(ring + slot * Smem::kSlot, kTileBox);
+#pragma unroll
+        for (int e = 0; e < kTileKeys / 16; ++e)  // 16 keys: 8 columns of packed P, 16 rows of V
+          umma_f16_ta(tmem + 256 + s * D, tmem + tile_p_at<D>(s) + e * 8, db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO,
+                      nth > 0 || e > 0);
+        umma_commit(&pv_done[s]);
+        if (!PAIR || s == 1) umma_commit(&empty[slot]);
+      };
+      if (PAIR) {
+        if (nt > 0) {
+          issue_s(0, 0);
+          issue_s(1, 0);
+        }
+        for (int k = 0; k < nt; ++k)
+          for (int s = 0; s < 2; ++s) {
+            issue_pv(s, k, k);
+            if (k + 1 < nt) issue_s(s, k + 1);
+          }
+      } else {
+        for (int k = 0; k < min(nt, 2); ++k) issue_s(k, k);
+        for (int k = 0; k < nt; ++k) {
+          issue_pv(k & 1, k, k >> 1);
+          if (k + 2 < nt) issue_s(k & 1, k + 2);
+        }
+      }
+      if (!ok) fail();
+      umma_commit(&done);  // arrives once every MMA issued has completed
+    }
+  }
+
+  // ---- softmax: thread = query (tensor-memory lane) of stream s
+  const int s = (warp >> 2) - 1;  // -1: not a softmax warp
+  const int row = (warp & 3) * 32 + lane;
+  const int x = (tile0 + (PAIR && s > 0 ? s : 0)) * kTileRows + row;  // query of the kv head
+  float m = -INFINITY, l = 0.f;
+  const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+  const int first = PAIR ? 0 : max(s, 0), step = PAIR ? 1 : 2;
+  const int mine = nt > first ? (nt - first + step - 1) / step : 0;  // tiles of the stream
+  bool ok = true;
+  if (s >= 0) {
+    const float c = a.scale * kLog2e;
+    const uint32_t s_at = tmem + lanes + s * kTileKeys, o_at = tmem + lanes + 256 + s * D;
+    const bool live_warp = x - lane < queries;  // some query of the warp exists
+    for (int j = 0; j < mine; ++j) {
+      const int k = first + j * step;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], j & 1) && !stopped())) {
+        ok = false;
+        break;
+      }
+      const int live = tokens - (t0 + k) * kTileKeys;  // keys of the tile, if fewer than 128
+      if (live < kTileKeys) {
+        // V rows behind the last token may hold anything: zero for the product (P is 0 there)
+        const int i = 2 * k + 1, slot = i % kSlots;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kSlots) & 1) && !stopped())) {
+          ok = false;
+          break;
+        }
+        for (int e = live * 8 + row; e < kTileKeys * 8; e += kTileRows)
+#pragma unroll
+          for (int b = 0; b < kBoxes; ++b)
+            *reinterpret_cast<uint4*>(ring + slot * Smem::kSlot + b * kTileBox + e * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
+      tmem_fence_after();
+      if (live_warp) {
+        uint32_t v[kTileKeys];
+#pragma unroll
+        for (int e = 0; e < kTileKeys; e += 32) tmem_ld32(s_at + e, *reinterpret_cast<uint32_t(*)[32]>(v + e));
+        tmem_wait_ld();
+        if (live < kTileKeys) {
+#pragma unroll
+          for (int e = 0; e < kTileKeys; ++e)
+            if (e >= live) v[e] = 0xff800000u;
+        }
+        float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < kTileKeys; e += 2) {
+          top = fmaxf(top, __uint_as_float(v[e]));
+          top2 = fmaxf(top2, __uint_as_float(v[e + 1]));
+        }
+        top = fmaxf(top, top2) * c;
+        const bool move = top > m + kMaxSlack || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, move)) {
+          const float to = move ? top : m, keep = m == -INFINITY ? 1.f : exp2f(m - to);
+          l *= keep;
+          m = to;
+          if (j > 0) {  // O holds earlier tiles: rescale it once the last product has landed
+            if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[s], (j - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            tmem_fence_after();
+#pragma unroll 1
+            for (int e = 0; e < D; e += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_at + e, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * keep);
+              tmem_st32(o_at + e, o);
+            }
+          }
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+        float sum = 0.f, sum2 = 0.f;
+        if (D == 64 && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[s], (j - 1) & 1))) {
+          ok = false;  // the product that reads P
+          break;
+        }
+        if (D == 64) tmem_fence_after();
+#pragma unroll
+        for (int e = 0; e < kTileKeys; e += 64) {
+          uint32_t p[32];
+#pragma unroll
+          for (int q = 0; q < 32; ++q) {
+            const float p0 = exp2_approx(fmaf(__uint_as_float(v[e + 2 * q]), c, -shift));
+            const float p1 = exp2_approx(fmaf(__uint_as_float(v[e + 2 * q + 1]), c, -shift));
+            sum += p0;
+            sum2 += p1;
+            p[q] = pack_pair(T(), p0, p1);
+          }
+          tmem_st32(tmem + lanes + tile_p_at<D>(s) + e / 2, p);
+        }
+        l += sum + sum2;
+        tmem_wait_st();
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[s]);
+    }
+    if (!ok && lane == 0) fail();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (!mbar_wait(&done, 0)) fail();  // every MMA has completed
+  }
+  __syncthreads();
+  tmem_fence_after();
+
+  // ---- the part's sums
+  const bool good = !stopped();
+  float o[D];
+  if (s >= 0) {
+    if (mine > 0 && good) {
+#pragma unroll
+      for (int e = 0; e < D; e += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem + lanes + 256 + s * D + e, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 32; ++q) o[e + q] = __uint_as_float(v[q]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < D; ++e) o[e] = 0.f;
+    }
+    if (!good) l = __uint_as_float(0x7fc00000u);
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTileCols) : "memory");
+  if (!PAIR) {  // stream 1's sums join stream 0's
+    float* so = reinterpret_cast<float*>(ring) + row * (D + 4);
+    if (s == 1) {
+#pragma unroll
+      for (int e = 0; e < D; e += 4) *reinterpret_cast<float4*>(so + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      so[D] = m;
+      so[D + 1] = l;
+    }
+    __syncthreads();
+    if (s == 0) {
+      const float om = so[D], ol = so[D + 1], top = fmaxf(m, om);
+      const float f0 = m == -INFINITY ? 0.f : exp2f(m - top), f1 = om == -INFINITY ? 0.f : exp2f(om - top);
+      l = (m == -INFINITY ? l : l * f0) + (om == -INFINITY ? ol : ol * f1);
+      if (f1 != 0.f) {
+#pragma unroll
+        for (int e = 0; e < D; ++e) o[e] = fmaf(so[e], f1, o[e] * f0);
+      }
+      m = top;
+    }
+    if (s != 0) return;
+  }
+  if (s < 0 || x >= queries) return;
+  const int r = x / group, h = g * group + x % group;
+  if (t.part_o == nullptr) {
+    store_out<T>(a, r, h, 0, o, l, m, true);
+    return;
+  }
+  const size_t dst = ((size_t)part * a.rows + r) * a.heads + h;
+  t.part_ml[dst] = make_float2(m, l);
+  if (m != -INFINITY) {
+    float4* po = reinterpret_cast<float4*>(t.part_o + dst * D);
+#pragma unroll
+    for (int e = 0; e < D; e += 4) po[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+  }
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool pdl, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// Shared K or V as a 3-D tensor of boxes of 64 channels x 128 tokens x 1 head; tokens past the last
+// read as zeros.  The axis with the smaller stride comes first.
+bool encode_shared(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int64_t token, int64_t head, bool token_last) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = map_encoder();
+  if (!enc) return false;
+  const cuuint64_t tokens = (cuuint64_t)a.shared_tokens, heads = (cuuint64_t)a.kv_heads;
+  const cuuint64_t row = (cuuint64_t)token * 2, one = (cuuint64_t)(a.kv_heads == 1 ? token : head) * 2;
+  cuuint64_t dims[3] = {(cuuint64_t)a.dim, token_last ? heads : tokens, token_last ? tokens : heads};
+  cuuint64_t strides[2] = {token_last ? one : row, token_last ? row : one};
+  cuuint32_t box[3] = {64, token_last ? 1u : (cuuint32_t)kTileKeys, token_last ? (cuuint32_t)kTileKeys : 1u};
+  cuuint32_t each[3] = {1, 1, 1};
+  const CUtensorMapDataType type =
+      a.dtype == S2R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, type, 3, const_cast<void*>(p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int query_tiles(const SharedAttnArgs& a) { return (a.rows * (a.heads / a.kv_heads) + kTileRows - 1) / kTileRows; }
+
+template <typename T, int D, bool PAIR>
+cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml, cudaStream_t s, bool pdl) {
+  CUtensorMap map_k, map_v;
+  TileArgs t{};
+  t.a = a;
+  t.part_o = part_o;
+  t.part_ml = part_ml;
+  t.token_last = a.kv_heads > 1 && a.k_head < a.k_token && a.v_head < a.v_token;
+  t.q_vector = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_row % 8 == 0 && a.q_head % 8 == 0;
+  if (!encode_shared(&map_k, a, a.shared_k, a.k_token, a.k_head, t.token_last) ||
+      !encode_shared(&map_v, a, a.shared_v, a.v_token, a.v_head, t.token_last))
+    return cudaErrorInvalidValue;
+  auto* kernel = shared_tile_kernel<T, D, PAIR>;
+  constexpr int smem = TileSmem<D, PAIR>::kBytes;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int tiles = PAIR ? (query_tiles(a) + 1) / 2 : query_tiles(a);
+  return launch(kernel, dim3(a.shared_splits, tiles, a.kv_heads), kTileThreads, smem, s, pdl, map_k, map_v, t);
 }
 
 template <typename T, int D>
-cudaError_t launch_group(const SharedAttnArgs& a, cudaStream_t s) {
+cudaError_t launch_rows(const SharedAttnArgs& a, float* o, float2* ml, cudaStream_t s, bool pdl) {
   const int group = a.heads / a.kv_heads;
-  if (group == 1) return launch_rows<T, D, 1>(a, s);
-  if (group == 2) return launch_rows<T, D, 2>(a, s);
-  return launch_rows<T, D, 4>(a, s);
+  auto grid = [&](int gc) { return dim3(a.own_splits, a.kv_heads * ((group + gc - 1) / gc), a.rows); };
+  if (group == 1) return launch(row_attn_kernel<T, D, 1>, grid(1), kOwnThreads, 0, s, pdl, a, o, ml, a.shared_splits);
+  if (group == 2) return launch(row_attn_kernel<T, D, 2>, grid(2), kOwnThreads, 0, s, pdl, a, o, ml, a.shared_splits);
+  return launch(row_attn_kernel<T, D, 4>, grid(4), kOwnThreads, 0, s, pdl, a, o, ml, a.shared_splits);
+}
+
+template <typename T, int D>
+cudaError_t launch_all(const SharedAttnArgs& a, cudaStream_t s) {
+  const int parts = a.shared_splits + a.own_splits;
+  const size_t pairs = (size_t)a.rows * a.heads;
+  const bool join = parts != 1 || a.own_splits;
+  float2* ml = static_cast<float2*>(a.workspace);
+  float* o = reinterpret_cast<float*>(ml + (parts * pairs + 1) / 2 * 2);
+  cudaError_t e = cudaSuccess;
+  if (a.shared_splits)
+    e = a.pair ? launch_tiles<T, D, true>(a, join ? o : nullptr, ml, s, a.pdl)
+               : launch_tiles<T, D, false>(a, join ? o : nullptr, ml, s, a.pdl);
+  // beside the shared part, which reads nothing the own part writes
+  if (e == cudaSuccess && a.own_splits) e = launch_rows<T, D>(a, o, ml, s, a.shared_splits > 0);
+  if (e == cudaSuccess && join)
+    e = launch(join_kernel<T, D>, dim3((unsigned)((pairs + 3) / 4)), 128, 0, s, parts > 0, a, o, ml, parts);
+  return e;
 }
 
 }  // namespace
 
 size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
-  auto splits = [&](int tokens) {
-    const int pages = (tokens + kPageTokens - 1) / kPageTokens;
+  const size_t pairs = (size_t)a.rows * a.heads;
+  a.shared_splits = a.own_splits = 0;
+  if (a.shared_tokens > 0) {
+    const int tiles = query_tiles(a), keys = (a.shared_tokens + kTileKeys - 1) / kTileKeys;
+    a.pair = tiles > 1;
+    // the split with the fewest key tiles one after the other: waves of CTAs (one an SM) times the
+    // tiles of each plus about 3 tiles' time to start and end it
+    const long long ctas = (long long)(a.pair ? (tiles + 1) / 2 : tiles) * a.kv_heads;
+    long long best = -1;
+    for (int sp = 1; sp <= keys && sp <= kMaxSharedSplits; ++sp) {
+      const int per = (keys + sp - 1) / sp;
+      if ((keys + per - 1) / per != sp) continue;  // the same tiles in fewer parts
+      const long long cost = (ctas * sp + sms - 1) / sms * (per + 3);
+      if (best < 0 || cost < best) {
+        best = cost;
+        a.shared_splits = sp;
+      }
+    }
+  }
+  if (a.own_k) {
     int sp = 1;
-    while (sp < 16 && (long long)a.rows * a.kv_heads * sp < 4ll * sms && pages / (sp * 2) >= 2) sp *= 2;
-    return tokens > 0 ? sp : 0;
-  };
-  a.shared_splits = splits(a.shared_tokens);
-  a.own_splits = a.own_k ? splits(a.pages_per_row * kPageTokens) : 0;
-  const size_t pairs = (size_t)a.rows * a.heads, parts = a.shared_splits + a.own_splits;
+    while (sp < 16 && (long long)a.rows * a.kv_heads * sp < 4ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
+    a.own_splits = sp;
+  }
+  const size_t parts = a.shared_splits + a.own_splits;
+  if (parts == 0 || (parts == 1 && !a.own_splits)) return 0;
   return (parts * pairs + 1) / 2 * 16 + parts * pairs * a.dim * sizeof(float);
 }
 
@@ -264,9 +752,9 @@ int launch_shared_attn(const SharedAttnArgs& a, cudaStream_t s, const char** why
   *why = "launch failed";
   cudaError_t e;
   if (a.dtype == S2R_BF16)
-    e = a.dim == 64 ? launch_group<bf16, 64>(a, s) : launch_group<bf16, 128>(a, s);
+    e = a.dim == 64 ? launch_all<bf16, 64>(a, s) : launch_all<bf16, 128>(a, s);
   else
-    e = a.dim == 64 ? launch_group<__half, 64>(a, s) : launch_group<__half, 128>(a, s);
+    e = a.dim == 64 ? launch_all<__half, 64>(a, s) : launch_all<__half, 128>(a, s);
   return e == cudaSuccess ? S2R_OK : S2R_ECUDA;
 }
 
@@ -292,6 +780,7 @@ int prepare(const s2r_shared_attention_args* in, s2r::SharedAttnArgs& a, size_t*
   if (in->rows < 1 || in->heads < 1 || in->kv_heads < 1 || in->shared_tokens < 0)
     return bad("rows, heads and kv_heads must be >= 1, shared_tokens >= 0");
   if (in->rows > 65535) return bad("at most 65535 rows a call");
+  if ((int64_t)in->rows * in->heads > (1 << 24)) return bad("at most 2^24 rows x heads a call");
   if (in->heads % in->kv_heads || in->heads > 4096) return bad("heads must be a multiple of kv_heads, at most 4096");
   if (in->shared_tokens > (1 << 28)) return bad("at most 2^28 shared tokens");
   if (!in->q || !in->out) return bad("q or out is NULL");
@@ -319,6 +808,8 @@ int prepare(const s2r_shared_attention_args* in, s2r::SharedAttnArgs& a, size_t*
       return bad("shared_k and shared_v must be 16-byte aligned with strides that are multiples of 8 elements");
     if (in->shared_tokens > 1 && (in->k_token_stride < in->head_dim || in->v_token_stride < in->head_dim))
       return bad("shared tokens overlap (token stride below head_dim)");
+    if (in->kv_heads > 1 && (in->k_head_stride < in->head_dim || in->v_head_stride < in->head_dim))
+      return bad("shared heads overlap (head stride below head_dim)");
   }
   const bool own = in->own_k || in->own_v || in->page_table || in->own_len;
   if (own) {

@@ -10,6 +10,8 @@ namespace s2r {
 
 constexpr int kErrOwnPage = 11;    // a page of a row's own K/V outside the pool
 constexpr int kErrOwnLength = 12;  // a row longer than its page table
+constexpr int kErrSharedWait = 13;  // a wait of the shared part timed out
+constexpr int kMaxSharedSplits = 64;
 
 struct SharedAttnArgs {
   int dtype;  // s2r_dtype: bf16 or f16
@@ -34,6 +36,8 @@ struct SharedAttnArgs {
   int* error;  // null, or set to kErrOwn* when a row's pages are broken
   // set by plan_shared_attn
   int shared_splits, own_splits;  // parts of a (row, head)'s keys
+  bool pair;                      // two query tiles a CTA
+  bool pdl;                       // the first launch may start while the kernel before it drains (it waits itself)
 };
 
 // Choose the splits for `sms` SMs and return the workspace bytes the launch needs.
