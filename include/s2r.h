@@ -365,7 +365,7 @@ typedef struct s2r_shared_attention_args {
   /* each row's own keys and values, in pages of S2R_PAGE_TOKENS tokens (all NULL: none) */
   const void* own_k; /* [own_pages][kv_heads][S2R_PAGE_TOKENS][head_dim], contiguous, 16-byte aligned */
   const void* own_v;
-  int32_t own_pages;
+  int32_t own_pages; /* own_pages * kv_heads below 2^25 */
   int32_t pages_per_row;
   const int32_t* page_table; /* [rows, pages_per_row]; entries past a row's length are not read */
   int64_t page_table_stride; /* between rows; 0: every row the same pages */

@@ -12,8 +12,7 @@
 // with o = sum exp(s - m) v in float32, and the parts are joined in a fixed
 // order: M = max m, out = sum_p o_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), with
 // m in units of log2.  Shared parts come from shared_tile_kernel (tensor
-// cores), own parts from row_attn_kernel (CUDA cores: every key is read for
-// heads / kv_heads queries only, so memory bounds it), which runs beside it.
+// cores), own parts from own_attn_kernel, which runs beside it.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -36,43 +35,71 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float2 pair_to_float(bf16, uint32_t v) { return make_float2(bf_lo(v), bf_hi(v)); }
-__device__ __forceinline__ float2 pair_to_float(__half, uint32_t v) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-// The 8 elements at p (16-byte aligned) as floats.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 v = ld_stream(p);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = pair_to_float(T(), w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
-}
-
-constexpr int kOwnThreads = 128;
+// ---- the rows' own parts
+//
+// A CTA takes one part of one (row, kv head): two warps, which take its
+// 16 KB chunks of K and V (64 tokens at dim 64, 32 at dim 128; a page is a
+// contiguous 64 x dim block per head) in turn, each through a ring of two
+// chunks of its own that one lane fills by TMA with the 128-byte swizzle.  No
+// barrier beyond the warp: memory bounds this part (a key is read for
+// heads / kv_heads queries), so what counts is bytes in flight, 192 KB an SM.
+// The products are mma.sync m16n8k16, rows = the group's queries (8, or 16 with
+// WIDE): a 128-row tcgen05 tile would hold at most 16 live rows and its round
+// trip through tensor memory would sit in the chain of every chunk.
+constexpr int kOwnThreads = 64;
 constexpr int kOwnWarps = kOwnThreads / 32;
-constexpr int kOwnUnroll = 4;  // key rows a lane group keeps in flight
+constexpr int kOwnStages = 2;
+constexpr int kOwnStage = 16384;  // bytes of a chunk, K then V
+constexpr int kOwnSmem = kOwnWarps * kOwnStages * kOwnStage + 1024;  // + alignment slack
 
-// One part of one row's keys for GC query heads of one kv head.  A key row is
-// read by D / 8 lanes, 16 bytes each; every such lane group keeps its own
-// online softmax over the keys it sees.
-template <typename T, int D, int GC>
-__global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_constant__ SharedAttnArgs a, float* part_o,
-                                                               float2* part_ml, int first_part) {
-  constexpr int kLanes = D / 8, kGroups = 32 / kLanes;  // lanes of a key row, key rows of a warp
-  const int part = blockIdx.x, splits = gridDim.x;
-  const int group = a.heads / a.kv_heads, chunks = (group + GC - 1) / GC;
-  const int g = blockIdx.y / chunks, h0 = g * group + (blockIdx.y % chunks) * GC;
-  const int heads = min(GC, (g + 1) * group - h0);
-  const int r = blockIdx.z;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / kLanes, at = (lane % kLanes) * 8;
-  __shared__ float so[kOwnWarps][GC][D];
-  __shared__ float2 sml[kOwnWarps][GC];
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(bf16, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
+template <typename T, int D, bool WIDE>
+__global__ void __launch_bounds__(kOwnThreads)
+    own_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ SharedAttnArgs a, float* part_o, float2* part_ml, int first_part) {
+  constexpr int kTokens = kOwnStage / (4 * D);  // of a chunk: 64 or 32
+  constexpr int kBoxes = D / 64, kBox = kTokens * 128;
+  constexpr int kHalves = WIDE ? 2 : 1;  // live halves of the MMA's 16 rows
+  constexpr int kQueries = 8 * kHalves;
+  extern __shared__ __align__(1024) unsigned char own_smem[];
+  __shared__ __align__(8) uint64_t full[kOwnWarps][kOwnStages];
+  __shared__ float2 sml[kQueries];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned char* base =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(own_smem) + 1023) & ~uintptr_t(1023));
+  unsigned char* ring = base + warp * kOwnStages * kOwnStage;
+  const int part = blockIdx.x, splits = gridDim.x, r = blockIdx.z;
+  const int group = a.heads / a.kv_heads, sets = (group + kQueries - 1) / kQueries;
+  const int g = blockIdx.y / sets, h0 = g * group + (blockIdx.y % sets) * kQueries;
+  const int heads = min(kQueries, (g + 1) * group - h0);
+
+  if (lane == 0) {
+    for (int i = 0; i < kOwnStages; ++i) mbar_init(&full[warp][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
   bool broken = false;
   int n = a.own_len[r];
   if (n > a.pages_per_row * kPageTokens) {
@@ -80,109 +107,190 @@ __global__ void __launch_bounds__(kOwnThreads) row_attn_kernel(const __grid_cons
     if (threadIdx.x == 0 && a.error) atomicExch(a.error, kErrOwnLength);
   }
   n = broken || n < 0 ? 0 : n;
-  const int pages = (n + kPageTokens - 1) / kPageTokens, per = (pages + splits - 1) / splits;
-  const int p0 = min(pages, part * per), p1 = min(pages, p0 + per);
+  const int chunks = (n + kTokens - 1) / kTokens, per = (chunks + splits - 1) / splits;
+  const int c0 = min(chunks, part * per) + warp, c1 = min(chunks, (part + 1) * per);
+  const int mine = c1 > c0 ? (c1 - c0 + kOwnWarps - 1) / kOwnWarps : 0;  // chunks of this warp
 
-  float q[GC][8], o[GC][8], m[GC], l[GC];
-#pragma unroll
-  for (int i = 0; i < GC; ++i) {
-    const T* src = static_cast<const T*>(a.q) + r * a.q_row + (h0 + min(i, heads - 1)) * a.q_head + at;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[i][e] = (float)src[e] * (a.scale * kLog2e);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[i][e] = 0.f;
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-  }
-  for (int p = p0 + warp; p < p1; p += kOwnWarps) {
-    const int page = a.page_table[r * a.page_stride + p];
+  // Page numbers of 32 chunks at a time, one a lane.
+  const int32_t* table = a.page_table + r * a.page_stride;
+  int pages = 0, pages_from = -32;
+  auto load_chunk = [&](int i) -> bool {  // the warp's i-th chunk into its stage
+    if (i >= pages_from + 32) {
+      pages_from = i;
+      const int c = c0 + (i + lane) * kOwnWarps;
+      pages = c < c1 ? table[c * kTokens / kPageTokens] : 0;
+    }
+    const int page = __shfl_sync(0xffffffffu, pages, i - pages_from);
     if (page < 0 || page >= a.own_pages) {
-      broken = true;
       if (lane == 0 && a.error) atomicExch(a.error, kErrOwnPage);
-      continue;
+      return false;
     }
-    const size_t base = ((size_t)page * a.kv_heads + g) * (kPageTokens * D);
-    const T* k = static_cast<const T*>(a.own_k) + base;
-    const T* v = static_cast<const T*>(a.own_v) + base;
-    const int live = min(kPageTokens, n - p * kPageTokens);
-#pragma unroll 1
-    for (int t0 = 0; t0 < live; t0 += kGroups * kOwnUnroll) {
-      float kx[kOwnUnroll][8], vx[kOwnUnroll][8];
+    if (lane == 0) {
+      unsigned char* stage = ring + (i % kOwnStages) * kOwnStage;
+      uint64_t* bar = &full[warp][i % kOwnStages];
+      const int token = (page * a.kv_heads + g) * kPageTokens + (c0 + i * kOwnWarps) * kTokens % kPageTokens;
+      mbar_expect_tx(bar, kOwnStage);
 #pragma unroll
-      for (int u = 0; u < kOwnUnroll; ++u) {
-        const int t = t0 + u * kGroups + sub;
-        if (t < live) {
-          load8(k + t * D + at, kx[u]);
-          load8(v + t * D + at, vx[u]);
-        } else {
+      for (int b = 0; b < kBoxes; ++b) tma_load_2d(stage + b * kBox, &map_k, b * 64, token, bar);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) kx[u][e] = vx[u][e] = 0.f;
-        }
+      for (int b = 0; b < kBoxes; ++b) tma_load_2d(stage + kOwnStage / 2 + b * kBox, &map_v, b * 64, token, bar);
+    }
+    return true;
+  };
+  int loaded = 0;  // chunks requested
+  while (loaded < min(mine, kOwnStages) && !broken) {
+    broken = !load_chunk(loaded);
+    loaded += !broken;
+  }
+
+  // ---- the queries: A operand of rows lane / 4 (and 8 more), 16 channels a step
+  uint32_t qa[D / 16][4];
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const int row = lane / 4 + (f & 1) * 8, at = e * 16 + (f >> 1) * 8 + (lane & 3) * 2;
+      qa[e][f] = 0;
+      if ((f & 1) < kHalves && row < heads) {
+        const unsigned short* src =
+            reinterpret_cast<const unsigned short*>(static_cast<const T*>(a.q) + r * a.q_row + (h0 + row) * a.q_head + at);
+        qa[e][f] = src[0] | (uint32_t)src[1] << 16;
       }
+    }
+  const float c = a.scale * kLog2e;
+  float o[D / 8][4], m[kHalves], l[kHalves];
 #pragma unroll
-      for (int i = 0; i < GC; ++i) {
-        float s[kOwnUnroll], top = m[i];
+  for (int e = 0; e < D / 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
 #pragma unroll
-        for (int u = 0; u < kOwnUnroll; ++u) {
-          s[u] = 0.f;
+  for (int f = 0; f < kHalves; ++f) m[f] = -INFINITY, l[f] = 0.f;
+
+  bool timeout = false;
+  for (int i = 0; i < loaded; ++i) {
+    const uint32_t k_at = smem_u32(ring + (i % kOwnStages) * kOwnStage), v_at = k_at + kOwnStage / 2;
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1))) {
+      timeout = true;
+      break;
+    }
+    const int live = n - (c0 + i * kOwnWarps) * kTokens;  // tokens of the chunk, if fewer
+    if (live < kTokens) {  // V rows behind the last token may hold anything: zero for the product
+      for (int x = live * 8 + lane; x < kTokens * 8; x += 32)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[u] = fmaf(q[i][e], kx[u][e], s[u]);
+        for (int b = 0; b < kBoxes; ++b)
+          *reinterpret_cast<uint4*>(ring + (i % kOwnStages) * kOwnStage + kOwnStage / 2 + b * kBox + x * 16) =
+              make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
+    // S = Q K^T, 8 keys a tile
+    float s[kTokens / 8][4];
 #pragma unroll
-          for (int x = kLanes / 2; x > 0; x >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], x);
-          if (t0 + u * kGroups + sub >= live) s[u] = -INFINITY;
-          top = fmaxf(top, s[u]);
-        }
-        const float keep = top == -INFINITY ? 1.f : exp2f(m[i] - top);
-        l[i] *= keep;
+    for (int j = 0; j < kTokens / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[i][e] *= keep;
+    for (int e = 0; e < D / 16; ++e)
 #pragma unroll
-        for (int u = 0; u < kOwnUnroll; ++u) {
-          const float w = s[u] == -INFINITY ? 0.f : exp2f(s[u] - top);
-          l[i] += w;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[i][e] = fmaf(w, vx[u][e], o[i][e]);
-        }
-        m[i] = top;
+      for (int j = 0; j < kTokens / 8; j += 2) {
+        const int key = j * 8 + (lane & 7) + (lane >> 4) * 8, piece = e * 2 + ((lane >> 3) & 1);
+        uint32_t b[4];
+        ldmatrix4(b, k_at + (piece / 8) * kBox + sw128_off(key, piece % 8));
+        mma16816(T(), s[j], qa[e], b[0], b[1]);
+        mma16816(T(), s[j + 1], qa[e], b[2], b[3]);
       }
+    if (live < kTokens) {
+#pragma unroll
+      for (int j = 0; j < kTokens / 8; ++j)
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+          if (j * 8 + (lane & 3) * 2 + (f & 1) >= live) s[j][f] = -INFINITY;
+    }
+    // online softmax of each row (4 lanes hold it)
+    uint32_t pa[kTokens / 16][4];
+#pragma unroll
+    for (int f = 0; f < kHalves; ++f) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kTokens / 8; ++j) top = fmaxf(top, fmaxf(s[j][2 * f], s[j][2 * f + 1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(top * c, m[f]);
+      if (__any_sync(0xffffffffu, top > m[f])) {
+        const float keep = m[f] == -INFINITY ? 1.f : exp2f(m[f] - top);
+        l[f] *= keep;
+#pragma unroll
+        for (int e = 0; e < D / 8; ++e) o[e][2 * f] *= keep, o[e][2 * f + 1] *= keep;
+        m[f] = top;
+      }
+      const float shift = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int j = 0; j < kTokens / 8; ++j) {
+        const float p0 = exp2_approx(fmaf(s[j][2 * f], c, -shift)), p1 = exp2_approx(fmaf(s[j][2 * f + 1], c, -shift));
+        l[f] += p0 + p1;  // (this lane's keys; the row's lanes are added at the end)
+        pa[j / 2][(j & 1) * 2 + f] = pack_pair(T(), p0, p1);
+      }
+    }
+    if (!WIDE) {
+#pragma unroll
+      for (int j = 0; j < kTokens / 16; ++j) pa[j][1] = pa[j][3] = 0;
+    }
+    // O += P V, 8 channels a tile
+#pragma unroll
+    for (int j = 0; j < kTokens / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < D / 8; e += 2) {
+        const int key = j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, piece = e + (lane >> 4);
+        uint32_t b[4];
+        ldmatrix4_trans(b, v_at + (piece / 8) * kBox + sw128_off(key, piece % 8));
+        mma16816(T(), o[e], pa[j], b[0], b[1]);
+        mma16816(T(), o[e + 1], pa[j], b[2], b[3]);
+      }
+    __syncwarp();  // every lane has read the stage
+    if (loaded < mine && !broken) {
+      broken = !load_chunk(loaded);
+      loaded += !broken;
     }
   }
-  // ---- join the lane groups, then the warps
+  if (timeout) {  // the copies in flight land before the CTA may exit (bounded)
+    for (int i = max(0, loaded - kOwnStages); i < loaded; ++i) mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1);
+    if (lane == 0 && a.error) atomicExch(a.error, kErrSharedWait);
+    broken = true;
+  }
 #pragma unroll
-  for (int i = 0; i < GC; ++i) {
+  for (int f = 0; f < kHalves; ++f) {
+    l[f] += __shfl_xor_sync(0xffffffffu, l[f], 1);
+    l[f] += __shfl_xor_sync(0xffffffffu, l[f], 2);
+    if (broken) l[f] = __uint_as_float(0x7fc00000u);  // a row with broken pages comes out as NaN
+  }
+  // ---- warp 1's sums join warp 0's
+  __syncthreads();  // both warps are done with their stages
+  float* so = reinterpret_cast<float*>(base);  // [kQueries][D + 8]
 #pragma unroll
-    for (int x = kLanes; x < 32; x <<= 1) {
-      const float om = __shfl_xor_sync(0xffffffffu, m[i], x), ol = __shfl_xor_sync(0xffffffffu, l[i], x);
-      const float top = fmaxf(m[i], om);
-      const float mine = m[i] == -INFINITY ? 0.f : exp2f(m[i] - top), other = om == -INFINITY ? 0.f : exp2f(om - top);
-      l[i] = l[i] * mine + ol * other;
+  for (int f = 0; f < kHalves; ++f) {
+    const int row = lane / 4 + 8 * f;
+    if (warp == 1) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[i][e] = o[i][e] * mine + __shfl_xor_sync(0xffffffffu, o[i][e], x) * other;
-      m[i] = top;
+      for (int e = 0; e < D / 8; ++e)
+        *reinterpret_cast<float2*>(so + row * (D + 8) + e * 8 + (lane & 3) * 2) = make_float2(o[e][2 * f], o[e][2 * f + 1]);
+      if ((lane & 3) == 0) sml[row] = make_float2(m[f], l[f]);
     }
-    if (broken) l[i] = __uint_as_float(0x7fc00000u);  // a row with broken pages comes out as NaN
-    if (sub == 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) so[warp][i][at + e] = o[i][e];
-    }
-    if (lane == 0) sml[warp][i] = make_float2(m[i], l[i]);
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < heads * D; x += kOwnThreads) {
-    const int i = x / D, e = x % D;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
+  if (warp == 0) {
 #pragma unroll
-    for (int w = 0; w < kOwnWarps; ++w) top = fmaxf(top, sml[w][i].x);
+    for (int f = 0; f < kHalves; ++f) {
+      const int row = lane / 4 + 8 * f;
+      if (row >= heads) continue;
+      const float2 ml = sml[row];
+      const float top = fmaxf(m[f], ml.x);
+      const float f0 = m[f] == -INFINITY ? 0.f : exp2f(m[f] - top), f1 = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      const float sum = (m[f] == -INFINITY ? l[f] : l[f] * f0) + (ml.x == -INFINITY ? ml.y : ml.y * f1);
+      const size_t dst = ((size_t)(first_part + part) * a.rows + r) * a.heads + h0 + row;
+      if ((lane & 3) == 0) part_ml[dst] = make_float2(top, sum);
+      if (top == -INFINITY) continue;
 #pragma unroll
-    for (int w = 0; w < kOwnWarps; ++w) {
-      const float2 ml = sml[w][i];
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-      sum += ml.x == -INFINITY ? ml.y : ml.y * f;  // (l of an empty part is 0, or NaN where pages are broken)
-      acc = fmaf(so[w][i][e], f, acc);
+      for (int e = 0; e < D / 8; ++e) {
+        const float2 x = *reinterpret_cast<const float2*>(so + row * (D + 8) + e * 8 + (lane & 3) * 2);
+        *reinterpret_cast<float2*>(part_o + dst * D + e * 8 + (lane & 3) * 2) =
+            make_float2(fmaf(x.x, f1, o[e][2 * f] * f0), fmaf(x.y, f1, o[e][2 * f + 1] * f0));
+      }
     }
-    const size_t dst = ((size_t)(first_part + part) * a.rows + r) * a.heads + h0 + i;
-    part_o[dst * D + e] = acc;
-    if (e == 0) part_ml[dst] = make_float2(top, sum);
   }
   pdl_launch_dependents();
   pdl_wait();  // this kernel runs beside the shared part; the join waits for both
@@ -667,6 +775,21 @@ bool encode_shared(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A pool of own K or V as rows of `dim` channels, read in boxes of 64 channels x one chunk's tokens.
+bool encode_pool(CUtensorMap* map, const SharedAttnArgs& a, const void* p) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)a.dim, (cuuint64_t)a.own_pages * a.kv_heads * kPageTokens};
+  cuuint64_t strides[1] = {(cuuint64_t)a.dim * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)(kOwnStage / (4 * a.dim))};
+  cuuint32_t each[2] = {1, 1};
+  const CUtensorMapDataType type =
+      a.dtype == S2R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, type, 2, const_cast<void*>(p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int query_tiles(const SharedAttnArgs& a) { return (a.rows * (a.heads / a.kv_heads) + kTileRows - 1) / kTileRows; }
 
 template <typename T, int D, bool PAIR>
@@ -689,13 +812,16 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml
   return launch(kernel, dim3(a.shared_splits, tiles, a.kv_heads), kTileThreads, smem, s, pdl, map_k, map_v, t);
 }
 
-template <typename T, int D>
-cudaError_t launch_rows(const SharedAttnArgs& a, float* o, float2* ml, cudaStream_t s, bool pdl) {
-  const int group = a.heads / a.kv_heads;
-  auto grid = [&](int gc) { return dim3(a.own_splits, a.kv_heads * ((group + gc - 1) / gc), a.rows); };
-  if (group == 1) return launch(row_attn_kernel<T, D, 1>, grid(1), kOwnThreads, 0, s, pdl, a, o, ml, a.shared_splits);
-  if (group == 2) return launch(row_attn_kernel<T, D, 2>, grid(2), kOwnThreads, 0, s, pdl, a, o, ml, a.shared_splits);
-  return launch(row_attn_kernel<T, D, 4>, grid(4), kOwnThreads, 0, s, pdl, a, o, ml, a.shared_splits);
+template <typename T, int D, bool WIDE>
+cudaError_t launch_own(const SharedAttnArgs& a, float* o, float2* ml, cudaStream_t s, bool pdl) {
+  CUtensorMap map_k, map_v;
+  if (!encode_pool(&map_k, a, a.own_k) || !encode_pool(&map_v, a, a.own_v)) return cudaErrorInvalidValue;
+  auto* kernel = own_attn_kernel<T, D, WIDE>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOwnSmem);
+  if (e != cudaSuccess) return e;
+  const int group = a.heads / a.kv_heads, queries = WIDE ? 16 : 8;
+  const dim3 grid(a.own_splits, a.kv_heads * ((group + queries - 1) / queries), a.rows);
+  return launch(kernel, grid, kOwnThreads, kOwnSmem, s, pdl, map_k, map_v, a, o, ml, a.shared_splits);
 }
 
 template <typename T, int D>
@@ -710,7 +836,9 @@ cudaError_t launch_all(const SharedAttnArgs& a, cudaStream_t s) {
     e = a.pair ? launch_tiles<T, D, true>(a, join ? o : nullptr, ml, s, a.pdl)
                : launch_tiles<T, D, false>(a, join ? o : nullptr, ml, s, a.pdl);
   // beside the shared part, which reads nothing the own part writes
-  if (e == cudaSuccess && a.own_splits) e = launch_rows<T, D>(a, o, ml, s, a.shared_splits > 0);
+  if (e == cudaSuccess && a.own_splits)
+    e = a.heads / a.kv_heads > 8 ? launch_own<T, D, true>(a, o, ml, s, a.shared_splits > 0)
+                                 : launch_own<T, D, false>(a, o, ml, s, a.shared_splits > 0);
   if (e == cudaSuccess && join)
     e = launch(join_kernel<T, D>, dim3((unsigned)((pairs + 3) / 4)), 128, 0, s, parts > 0, a, o, ml, parts);
   return e;
@@ -739,8 +867,9 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     }
   }
   if (a.own_k) {
+    // three CTAs fit an SM; twice that evens out rows of different lengths
     int sp = 1;
-    while (sp < 16 && (long long)a.rows * a.kv_heads * sp < 4ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
+    while (sp < 32 && (long long)a.rows * a.kv_heads * sp < 6ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
     a.own_splits = sp;
   }
   const size_t parts = a.shared_splits + a.own_splits;
@@ -817,6 +946,7 @@ int prepare(const s2r_shared_attention_args* in, s2r::SharedAttnArgs& a, size_t*
       return bad("own_k, own_v, page_table and own_len go together");
     if (in->own_pages < 1 || in->pages_per_row < 1) return bad("own_pages and pages_per_row must be >= 1");
     if (in->pages_per_row > (1 << 22)) return bad("at most 2^22 pages a row");
+    if ((int64_t)in->own_pages * in->kv_heads >= (1 << 25)) return bad("own_pages x kv_heads must be below 2^25");
     if (in->rows > 1 && in->page_table_stride < in->pages_per_row && in->page_table_stride != 0)
       return bad("page table rows overlap");
     if (reinterpret_cast<uintptr_t>(in->own_k) % 16 || reinterpret_cast<uintptr_t>(in->own_v) % 16)

@@ -63,7 +63,7 @@ OWN = dict(own_k=16, own_v=16, own_pages=4, pages_per_row=2, page_table=16, page
     (dict(rows=65535, heads=512), b"2^24"), (dict(v_head_stride=32), b"overlap"), (dict(q_row_stride=-1), b"strides"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"),
     (dict(scale=float("inf")), b"scale"), (dict(own_k=16), b"go together"), (dict(own_len=16), b"go together"),
     (dict(OWN, own_pages=0), b"own_pages"), (dict(OWN, pages_per_row=0), b"pages_per_row"),
-    (dict(OWN, page_table_stride=1), b"page table"), (dict(OWN, own_v=40), b"aligned"),
+    (dict(OWN, page_table_stride=1), b"page table"), (dict(OWN, own_pages=2**24), b"2^25"), (dict(OWN, own_v=40), b"aligned"),
 ])
 def test_shared_attention_entry_point_refuses(change, word):
     lib = _lib.load()
