@@ -341,15 +341,16 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 //
 // The queries of one kv head, (row, group member) pairs in order, are tiles of
 // 128: the MMA's M, one tensor-memory lane and one softmax thread each.  A CTA
-// walks its part of the keys in tiles of 128, with two streams in flight, each
-// with a score tile S, an output accumulator O and a warpgroup of its own:
+// walks its part of the keys in tiles of KT (128 at dim 64, 64 at dim 128), with
+// two streams in flight, each with a score tile S, a weight tile P, an output
+// accumulator O and a warpgroup of its own:
 //
 //   one query tile (PAIR = false): the streams take the even and the odd key
 //     tiles and are joined at the end;
 //   two query tiles (PAIR = true): stream s is query tile s, both walk every
 //     key tile, which is then read once for 256 queries.
 //
-//   S = Q K^T      tcgen05.mma M128 N128 K=dim, float32 in tensor memory
+//   S = Q K^T      tcgen05.mma M128 N=KT K=dim, float32 in tensor memory
 //   p = 2^(c s - m) c = scale log2(e); m trails the running maximum by at most
 //                  2^8, so that O is rescaled only when the maximum moves far
 //                  (Milakov and Gimelshein's online softmax, with slack)
@@ -361,36 +362,32 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 // every 16-bit attention (half a step of each weight); l sums the unrounded
 // float32 values; O is float32 throughout.
 //
-// Warp 0 loads K and V tiles by TMA into a ring, warp 1 issues the MMAs (S0 S1 |
-// PV0 S0' | PV1 S1' | ...), warps 4-7 and 8-11 are the softmax warpgroups.
-// Tensor memory holds S twice and O twice; at dim 64 there is room for P beside
-// them, and the softmax waits for the product before it overwrites P.  At dim
-// 128 P lies in S's columns: the next S of the stream follows the product that
-// reads P, and MMAs of one accumulator shape (both 128 x 128) execute in order.
-// Every mbarrier wait is
-// bounded; on a timeout the CTA marks its rows NaN, drains its copies and MMAs
-// (bounded), frees its tensor memory and returns.
+// Warp 0 loads K and V tiles by TMA into a ring, warp 1 issues the MMAs, warps
+// 4-7 and 8-11 are the softmax warpgroups.  A softmax thread takes its whole
+// score row into registers and hands S back at once, so that S of the stream's
+// next tile is computed under this tile's exponentials (with S handed back only
+// with P, each stream waited ~1,850 of every ~4,050 cycles for its products).
+// The exponential unit gives 16 results a cycle and SM, which would bound a
+// large call; a part of the exponentials is computed on the FMA units instead.
+// Every mbarrier wait is bounded; on a timeout the CTA marks its rows NaN, drains
+// its copies and MMAs (bounded), frees its tensor memory and returns.
 constexpr int kTileThreads = 384;
 constexpr int kTileRows = 128;  // queries of a tile
-constexpr int kTileKeys = 128;  // keys of a tile
-constexpr int kTileBox = kTileKeys * 64 * 2;  // bytes of a 64-channel box of a tile
-constexpr int kTileCols = 512;  // tensor memory: S at 0 and 128, O at 256 and 256 + D, P: tile_p_at
+constexpr int kTileCols = 512;  // tensor memory columns: S, O and P of both streams
 constexpr float kMaxSlack = 8.f;
+constexpr int kPolyPairs = 2;  // of every 8 pairs of weights, computed on the FMA units
+
+__host__ __device__ constexpr int tile_keys(int dim) { return dim == 64 ? 128 : 64; }
 
 template <int D, bool PAIR>
 struct TileSmem {
-  static constexpr int kSlot = kTileKeys * D * 2;  // a K or V tile
+  static constexpr int kSlot = tile_keys(D) * D * 2;  // a K or V tile: 16 KB
   static constexpr int kQueries = (PAIR ? 2 : 1) * kTileRows * D * 2;
-  static constexpr int kSlots = D == 64 ? 8 : 5;
+  static constexpr int kSlots = 8;
   static constexpr int kBytes = kQueries + kSlots * kSlot + 1024;  // + alignment slack
   static_assert(kBytes + 1024 <= 227 * 1024, "fits an SM");
   static_assert(kTileRows * (D + 4) * 4 <= kSlots * kSlot, "a stream's partial fits the ring");
 };
-
-template <int D>
-__device__ __forceinline__ uint32_t tile_p_at(int s) {  // columns of stream s's P (64)
-  return D == 64 ? 384 + s * 64 : s * kTileKeys;
-}
 
 struct TileArgs {
   SharedAttnArgs a;
@@ -405,14 +402,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     shared_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ TileArgs t) {
   using Smem = TileSmem<D, PAIR>;
-  constexpr int kSlots = Smem::kSlots, kBoxes = D / 64;
+  constexpr int kSlots = Smem::kSlots, kBoxes = D / 64, KT = tile_keys(D), kBox = KT * 128;
+  constexpr int kQueryBox = kTileRows * 128;
+  constexpr uint32_t kAtS = 0, kAtO = 2 * KT, kAtP = kAtO + 2 * D;  // tensor memory columns, stream 0
+  static_assert(kAtP + KT <= kTileCols, "fits the tensor memory");
   const SharedAttnArgs& a = t.a;
   extern __shared__ __align__(1024) unsigned char tile_smem[];
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tile_smem) + 1023) & ~uintptr_t(1023));
   unsigned char* sq = base;                    // query tiles: [tile][box][128 rows][128 bytes]
   unsigned char* ring = base + Smem::kQueries;  // slot i: the i-th of K0 V0 K1 V1 ...
-  __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], s_full[2], p_full[2], pv_done[2], done;
+  __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], s_full[2], s_empty[2], p_full[2], pv_done[2], done;
   __shared__ uint32_t tmem_base;
   __shared__ int aborted;
 
@@ -428,12 +428,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);  // one arrival per warp of the stream
+      mbar_init(&s_empty[s], 4);  // one arrival per warp of the stream
+      mbar_init(&p_full[s], 4);
       mbar_init(&pv_done[s], 1);
     }
     mbar_init(&done, 1);
     aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();  // this thread starts copies on them ahead of the block's barrier
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
@@ -441,27 +443,64 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
+  }
   pdl_wait();  // the queries come from the kernel before
   const int tokens = a.shared_len ? min(max(*a.shared_len, 0), a.shared_tokens) : a.shared_tokens;
-  const int tiles = (tokens + kTileKeys - 1) / kTileKeys, per = (tiles + parts - 1) / parts;
+  const int tiles = (tokens + KT - 1) / KT, per = (tiles + parts - 1) / parts;
   const int t0 = min(tiles, part * per), nt = min(tiles, t0 + per) - t0;
 
-  // ---- the queries, in the 128-byte-swizzled rows the MMA reads
-  for (int i = threadIdx.x; i < (PAIR ? 2 : 1) * kTileRows * (D / 8); i += kTileThreads) {
-    const int row = i / (D / 8), c = i % (D / 8), x = tile0 * kTileRows + row;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (x < queries) {
-      const T* src = static_cast<const T*>(a.q) + x / group * a.q_row + (g * group + x % group) * a.q_head + c * 8;
-      if (t.q_vector) {
-        v = *reinterpret_cast<const uint4*>(src);
-      } else {
-        const unsigned short* e = reinterpret_cast<const unsigned short*>(src);
-        v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
-                       e[6] | (uint32_t)e[7] << 16);
+  auto fail = [&]() {
+    if (a.error) atomicExch(a.error, kErrSharedWait);
+    *(volatile int*)&aborted = 1;
+  };
+  auto stopped = [&]() { return *(volatile int*)&aborted != 0; };
+  auto load_tile = [&](int i) {  // the i-th of K0 V0 K1 V1 ...
+    const int slot = i % kSlots, token = (t0 + i / 2) * KT;
+    const CUtensorMap* map = i & 1 ? &map_v : &map_k;
+    mbar_expect_tx(&full[slot], Smem::kSlot);
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b)
+      tma_load_3d(ring + slot * Smem::kSlot + b * kBox, map, b * 64, t.token_last ? g : token, t.token_last ? token : g,
+                  &full[slot]);
+  };
+  const int ahead = min(2 * nt, kSlots);  // tiles requested before the queries are staged
+  if (threadIdx.x == 0)
+    for (int i = 0; i < ahead; ++i) load_tile(i);
+
+  // ---- the queries, in the 128-byte-swizzled rows the MMA reads (by the softmax warps, four
+  // pieces in flight each)
+  if (warp >= 4) {
+    constexpr int kPieces = (PAIR ? 2 : 1) * kTileRows * (D / 8), kThreads = kTileThreads - 128;
+    static_assert(kPieces % (4 * kThreads) == 0, "whole batches");
+#pragma unroll 1
+    for (int i0 = threadIdx.x - 128; i0 < kPieces; i0 += 4 * kThreads) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kThreads, x = tile0 * kTileRows + i / (D / 8), c = i % (D / 8);
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (x < queries) {
+          const int r = group == 1 ? x : x / group;
+          const T* src = static_cast<const T*>(a.q) + r * a.q_row + (g * group + x - r * group) * a.q_head + c * 8;
+          if (t.q_vector) {
+            v[u] = *reinterpret_cast<const uint4*>(src);
+          } else {
+            const unsigned short* e = reinterpret_cast<const unsigned short*>(src);
+            v[u] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                              e[6] | (uint32_t)e[7] << 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kThreads, row = i / (D / 8), c = i % (D / 8);
+        unsigned char* tile = sq + row / kTileRows * (kTileRows * D * 2) + c / 8 * kQueryBox;
+        *reinterpret_cast<uint4*>(tile + sw128_off(row % kTileRows, c % 8)) = v[u];
       }
     }
-    unsigned char* tile = sq + row / kTileRows * (kTileRows * D * 2) + c / 8 * kTileBox;
-    *reinterpret_cast<uint4*>(tile + sw128_off(row % kTileRows, c % 8)) = v;
   }
   fence_async_smem();
   tmem_fence_before();
@@ -470,29 +509,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // Dependents may start only now: one that needs tensor memory must not take it ahead of this CTA.
   pdl_launch_dependents();
   const uint32_t tmem = tmem_base;
-  auto fail = [&]() {
-    if (a.error) atomicExch(a.error, kErrSharedWait);
-    *(volatile int*)&aborted = 1;
-  };
-  auto stopped = [&]() { return *(volatile int*)&aborted != 0; };
 
+  // The block's registers: 168 a thread at launch; 40 for the issuing warps leave 232 for the softmax
+  // (128 * (40 + 232 + 232) = 384 * 168).
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 0) {
     if (lane == 0) {
       // ---- producer
-      int issued = 0;
-      for (int i = 0; i < 2 * nt; ++i) {
-        const int slot = i % kSlots;
-        if (i >= kSlots && (!mbar_wait(&empty[slot], (i / kSlots - 1) & 1) || stopped())) {
+      int issued = ahead;
+      for (int i = ahead; i < 2 * nt; ++i) {
+        if (!mbar_wait(&empty[i % kSlots], (i / kSlots - 1) & 1) || stopped()) {
           fail();
           break;
         }
-        mbar_expect_tx(&full[slot], Smem::kSlot);
-        const CUtensorMap* map = i & 1 ? &map_v : &map_k;
-        const int token = (t0 + i / 2) * kTileKeys;
-#pragma unroll
-        for (int b = 0; b < kBoxes; ++b)
-          tma_load_3d(ring + slot * Smem::kSlot + b * kTileBox, map, b * 64, t.token_last ? g : token,
-                      t.token_last ? token : g, &full[slot]);
+        load_tile(i);
         issued = i + 1;
       }
       // every copy has landed before the ring is reused or the CTA exits (bounded)
@@ -502,13 +533,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (lane == 0) {
       // ---- MMA issuer
       constexpr uint32_t kFormat = std::is_same<T, bf16>::value ? 1u : 0u;
-      constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, kTileKeys, false);
+      constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, KT, false);
       constexpr uint32_t kIdescO = umma_idesc(kFormat, kTileRows, D, true);
       bool ok = true;
-      auto issue_s = [&](int s, int k) {  // S_s = Q K_k^T
+      auto issue_s = [&](int s, int k, int nth) {  // S_s = Q K_k^T, the stream's nth
         const int i = 2 * k, slot = i % kSlots;
         if (!ok) return;
-        if (!mbar_wait(&full[slot], (i / kSlots) & 1) || stopped()) {
+        if ((nth > 0 && !mbar_wait(&s_empty[s], (nth - 1) & 1)) || !mbar_wait(&full[slot], (i / kSlots) & 1) || stopped()) {
           ok = false;
           return;
         }
@@ -517,8 +548,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint64_t db = umma_desc_sw128(ring + slot * Smem::kSlot);
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) {  // 16 channels: 32 bytes of a row, a box every 64
-          const uint64_t at = (uint64_t)((e / 4) * (kTileBox >> 4) + (e % 4) * 2);
-          umma_f16(tmem + s * kTileKeys, da + at, db + at, kIdescS, e > 0);
+          umma_f16(tmem + kAtS + s * KT, da + (uint64_t)((e / 4) * (kQueryBox >> 4) + (e % 4) * 2),
+                   db + (uint64_t)((e / 4) * (kBox >> 4) + (e % 4) * 2), kIdescS, e > 0);
         }
         umma_commit(&s_full[s]);
         if (!PAIR || s == 1) umma_commit(&empty[slot]);
@@ -531,29 +562,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           return;
         }
         tmem_fence_after();
-        const uint64_t db = umma_desc_mn_sw128(ring + slot * Smem::kSlot, kTileBox);
+        const uint64_t db = umma_desc_mn_sw128(ring + slot * Smem::kSlot, kBox);
 #pragma unroll
-        for (int e = 0; e < kTileKeys / 16; ++e)  // 16 keys: 8 columns of packed P, 16 rows of V
-          umma_f16_ta(tmem + 256 + s * D, tmem + tile_p_at<D>(s) + e * 8, db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO,
+        for (int e = 0; e < KT / 16; ++e)  // 16 keys: 8 columns of packed P, 16 rows of V
+          umma_f16_ta(tmem + kAtO + s * D, tmem + kAtP + s * (KT / 2) + e * 8, db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO,
                       nth > 0 || e > 0);
         umma_commit(&pv_done[s]);
         if (!PAIR || s == 1) umma_commit(&empty[slot]);
       };
+      // S runs one tile of its stream ahead of PV
       if (PAIR) {
-        if (nt > 0) {
-          issue_s(0, 0);
-          issue_s(1, 0);
-        }
+        for (int s = 0; s < 2 && nt > 0; ++s) issue_s(s, 0, 0);
         for (int k = 0; k < nt; ++k)
           for (int s = 0; s < 2; ++s) {
+            if (k + 1 < nt) issue_s(s, k + 1, k + 1);
             issue_pv(s, k, k);
-            if (k + 1 < nt) issue_s(s, k + 1);
           }
       } else {
-        for (int k = 0; k < min(nt, 2); ++k) issue_s(k, k);
+        for (int k = 0; k < min(nt, 2); ++k) issue_s(k, k, 0);
         for (int k = 0; k < nt; ++k) {
+          if (k + 2 < nt) issue_s(k & 1, k + 2, (k >> 1) + 1);
           issue_pv(k & 1, k, k >> 1);
-          if (k + 2 < nt) issue_s(k & 1, k + 2);
         }
       }
       if (!ok) fail();
@@ -561,18 +590,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   }
 
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (!mbar_wait(&done, 0)) fail();  // every MMA has completed
+  }
+  __syncthreads();
+  __syncthreads();  // the softmax warps have read O
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTileCols) : "memory");
+  if (!PAIR) __syncthreads();
+  return;
+  }
+
   // ---- softmax: thread = query (tensor-memory lane) of stream s
-  const int s = (warp >> 2) - 1;  // -1: not a softmax warp
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+  const int s = (warp >> 2) - 1;
   const int row = (warp & 3) * 32 + lane;
-  const int x = (tile0 + (PAIR && s > 0 ? s : 0)) * kTileRows + row;  // query of the kv head
+  const int x = (tile0 + (PAIR ? s : 0)) * kTileRows + row;  // query of the kv head
   float m = -INFINITY, l = 0.f;
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-  const int first = PAIR ? 0 : max(s, 0), step = PAIR ? 1 : 2;
+  const int first = PAIR ? 0 : s, step = PAIR ? 1 : 2;
   const int mine = nt > first ? (nt - first + step - 1) / step : 0;  // tiles of the stream
   bool ok = true;
-  if (s >= 0) {
+  {
     const float c = a.scale * kLog2e;
-    const uint32_t s_at = tmem + lanes + s * kTileKeys, o_at = tmem + lanes + 256 + s * D;
+    const uint32_t s_at = tmem + lanes + kAtS + s * KT, o_at = tmem + lanes + kAtO + s * D;
+    const uint32_t p_at = tmem + lanes + kAtP + s * (KT / 2);
     const bool live_warp = x - lane < queries;  // some query of the warp exists
     for (int j = 0; j < mine; ++j) {
       const int k = first + j * step;
@@ -580,81 +623,93 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ok = false;
         break;
       }
-      const int live = tokens - (t0 + k) * kTileKeys;  // keys of the tile, if fewer than 128
-      if (live < kTileKeys) {
+      tmem_fence_after();
+      uint32_t v[KT];
+      if (live_warp) {
+#pragma unroll
+        for (int e = 0; e < KT; e += 32) tmem_ld32(s_at + e, *reinterpret_cast<uint32_t(*)[32]>(v + e));
+        tmem_wait_ld();
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[s]);
+      const int live = tokens - (t0 + k) * KT;  // keys of the tile, if fewer
+      if (live < KT) {
         // V rows behind the last token may hold anything: zero for the product (P is 0 there)
         const int i = 2 * k + 1, slot = i % kSlots;
         if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kSlots) & 1) && !stopped())) {
           ok = false;
           break;
         }
-        for (int e = live * 8 + row; e < kTileKeys * 8; e += kTileRows)
+        for (int e = live * 8 + row; e < KT * 8; e += kTileRows)
 #pragma unroll
           for (int b = 0; b < kBoxes; ++b)
-            *reinterpret_cast<uint4*>(ring + slot * Smem::kSlot + b * kTileBox + e * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(ring + slot * Smem::kSlot + b * kBox + e * 16) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
+      }
+      float to = m, keep = 1.f;
+      bool move = false;
+      if (live_warp) {
+        if (live < KT) {
+#pragma unroll
+          for (int e = 0; e < KT; ++e)
+            if (e >= live) v[e] = 0xff800000u;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < KT; e += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            top[q] = max3(top[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
+        to = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        move = to > m + kMaxSlack;
+        to = move ? to : m;
+        keep = m == -INFINITY ? 1.f : exp2f(m - to);
+        move = __any_sync(0xffffffffu, move);
+        m = to;
+        l *= keep;
+        // the weights 2^(c s - m), in pairs
+        const float shift = m == -INFINITY ? 0.f : m;
+        const uint64_t c2 = pack2(c, c), shift2 = pack2(-shift, -shift);
+        uint64_t sum2[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < KT; e += 2) {
+          const uint64_t y = fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, shift2);
+          float p0, p1;
+          if (e / 2 % 8 < kPolyPairs) {
+            exp2_poly2(y, p0, p1);
+          } else {
+            unpack2(y, p0, p1);
+            p0 = exp2_approx(p0);
+            p1 = exp2_approx(p1);
+          }
+          sum2[e / 2 & 1] = add2(sum2[e / 2 & 1], pack2(p0, p1));
+          v[e / 2] = pack_pair(T(), p0, p1);
+        }
+        float x0, x1;
+        unpack2(add2(sum2[0], sum2[1]), x0, x1);
+        l += x0 + x1;
+      }
+      // P and O are free once the stream's last product has landed
+      if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[s], (j - 1) & 1))) {
+        ok = false;
+        break;
       }
       tmem_fence_after();
       if (live_warp) {
-        uint32_t v[kTileKeys];
-#pragma unroll
-        for (int e = 0; e < kTileKeys; e += 32) tmem_ld32(s_at + e, *reinterpret_cast<uint32_t(*)[32]>(v + e));
-        tmem_wait_ld();
-        if (live < kTileKeys) {
-#pragma unroll
-          for (int e = 0; e < kTileKeys; ++e)
-            if (e >= live) v[e] = 0xff800000u;
-        }
-        float top = -INFINITY, top2 = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < kTileKeys; e += 2) {
-          top = fmaxf(top, __uint_as_float(v[e]));
-          top2 = fmaxf(top2, __uint_as_float(v[e + 1]));
-        }
-        top = fmaxf(top, top2) * c;
-        const bool move = top > m + kMaxSlack || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, move)) {
-          const float to = move ? top : m, keep = m == -INFINITY ? 1.f : exp2f(m - to);
-          l *= keep;
-          m = to;
-          if (j > 0) {  // O holds earlier tiles: rescale it once the last product has landed
-            if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[s], (j - 1) & 1))) {
-              ok = false;
-              break;
-            }
-            tmem_fence_after();
+        if (move && j > 0) {
 #pragma unroll 1
-            for (int e = 0; e < D; e += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_at + e, o);
-              tmem_wait_ld();
+          for (int e = 0; e < D; e += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_at + e, o);
+            tmem_wait_ld();
 #pragma unroll
-              for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * keep);
-              tmem_st32(o_at + e, o);
-            }
+            for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * keep);
+            tmem_st32(o_at + e, o);
           }
         }
-        const float shift = m == -INFINITY ? 0.f : m;
-        float sum = 0.f, sum2 = 0.f;
-        if (D == 64 && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[s], (j - 1) & 1))) {
-          ok = false;  // the product that reads P
-          break;
-        }
-        if (D == 64) tmem_fence_after();
 #pragma unroll
-        for (int e = 0; e < kTileKeys; e += 64) {
-          uint32_t p[32];
-#pragma unroll
-          for (int q = 0; q < 32; ++q) {
-            const float p0 = exp2_approx(fmaf(__uint_as_float(v[e + 2 * q]), c, -shift));
-            const float p1 = exp2_approx(fmaf(__uint_as_float(v[e + 2 * q + 1]), c, -shift));
-            sum += p0;
-            sum2 += p1;
-            p[q] = pack_pair(T(), p0, p1);
-          }
-          tmem_st32(tmem + lanes + tile_p_at<D>(s) + e / 2, p);
-        }
-        l += sum + sum2;
+        for (int e = 0; e < KT / 2; e += 32) tmem_st32(p_at + e, *reinterpret_cast<const uint32_t(*)[32]>(v + e));
         tmem_wait_st();
       }
       tmem_fence_before();
@@ -664,35 +719,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (!ok && lane == 0) fail();
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    if (!mbar_wait(&done, 0)) fail();  // every MMA has completed
-  }
-  __syncthreads();
+  __syncthreads();  // every MMA has completed
   tmem_fence_after();
 
   // ---- the part's sums
   const bool good = !stopped();
   float o[D];
-  if (s >= 0) {
-    if (mine > 0 && good) {
+  if (mine > 0 && good) {
 #pragma unroll
-      for (int e = 0; e < D; e += 32) {
-        uint32_t v[32];
-        tmem_ld32(tmem + lanes + 256 + s * D + e, v);
-        tmem_wait_ld();
+    for (int e = 0; e < D; e += 32) {
+      uint32_t v[32];
+      tmem_ld32(tmem + lanes + kAtO + s * D + e, v);
+      tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 32; ++q) o[e + q] = __uint_as_float(v[q]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < D; ++e) o[e] = 0.f;
+      for (int q = 0; q < 32; ++q) o[e + q] = __uint_as_float(v[q]);
     }
-    if (!good) l = __uint_as_float(0x7fc00000u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < D; ++e) o[e] = 0.f;
   }
+  if (!good) l = __uint_as_float(0x7fc00000u);
   tmem_fence_before();
   __syncthreads();
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTileCols) : "memory");
   if (!PAIR) {  // stream 1's sums join stream 0's
     float* so = reinterpret_cast<float*>(ring) + row * (D + 4);
     if (s == 1) {
@@ -714,7 +762,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     if (s != 0) return;
   }
-  if (s < 0 || x >= queries) return;
+  if (x >= queries) return;
   const int r = x / group, h = g * group + x % group;
   if (t.part_o == nullptr) {
     store_out<T>(a, r, h, 0, o, l, m, true);
@@ -757,7 +805,7 @@ PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
   return fn;
 }
 
-// Shared K or V as a 3-D tensor of boxes of 64 channels x 128 tokens x 1 head; tokens past the last
+// Shared K or V as a 3-D tensor of boxes of 64 channels x one tile's tokens x 1 head; tokens past the last
 // read as zeros.  The axis with the smaller stride comes first.
 bool encode_shared(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int64_t token, int64_t head, bool token_last) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = map_encoder();
@@ -766,7 +814,8 @@ bool encode_shared(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int
   const cuuint64_t row = (cuuint64_t)token * 2, one = (cuuint64_t)(a.kv_heads == 1 ? token : head) * 2;
   cuuint64_t dims[3] = {(cuuint64_t)a.dim, token_last ? heads : tokens, token_last ? tokens : heads};
   cuuint64_t strides[2] = {token_last ? one : row, token_last ? row : one};
-  cuuint32_t box[3] = {64, token_last ? 1u : (cuuint32_t)kTileKeys, token_last ? (cuuint32_t)kTileKeys : 1u};
+  const cuuint32_t keys = (cuuint32_t)tile_keys(a.dim);
+  cuuint32_t box[3] = {64, token_last ? 1u : keys, token_last ? keys : 1u};
   cuuint32_t each[3] = {1, 1, 1};
   const CUtensorMapDataType type =
       a.dtype == S2R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -850,7 +899,7 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
   const size_t pairs = (size_t)a.rows * a.heads;
   a.shared_splits = a.own_splits = 0;
   if (a.shared_tokens > 0) {
-    const int tiles = query_tiles(a), keys = (a.shared_tokens + kTileKeys - 1) / kTileKeys;
+    const int tiles = query_tiles(a), keys = (a.shared_tokens + tile_keys(a.dim) - 1) / tile_keys(a.dim);
     a.pair = tiles > 1;
     // the split with the fewest key tiles one after the other: waves of CTAs (one an SM) times the
     // tiles of each plus about 3 tiles' time to start and end it

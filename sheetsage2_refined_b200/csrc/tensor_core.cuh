@@ -74,6 +74,67 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Two floats as one 64-bit operand of the packed float32 instructions.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// 2^x of a pair on the FMA units: x = n + f with n the nearest integer and
+// |f| <= 1/2, 2^f by its series to the fifth power of f ln 2 (the first term
+// left out is (ln2 / 2)^6 / 720 = 2.4e-6 of the result at most), times 2^n.
+// x <= 127; 0 below -126.5; NaN stays NaN.
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float& p0, float& p1) {
+  float x0, x1;
+  unpack2(x, x0, x1);
+  x = pack2(max_nan(x0, -127.f), max_nan(x1, -127.f));
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+  const uint64_t n = add2(x, pack2(kMagic, kMagic));
+  const uint64_t f = add2(x, fma2(n, pack2(-1.f, -1.f), pack2(kMagic, kMagic)));
+  uint64_t q = fma2(f, pack2(1.3333558146e-3f, 1.3333558146e-3f), pack2(9.6181291076e-3f, 9.6181291076e-3f));
+  q = fma2(f, q, pack2(5.5504108665e-2f, 5.5504108665e-2f));
+  q = fma2(f, q, pack2(2.4022650696e-1f, 2.4022650696e-1f));
+  q = fma2(f, q, pack2(6.9314718056e-1f, 6.9314718056e-1f));
+  q = fma2(f, q, pack2(1.f, 1.f));
+  float n0, n1;
+  unpack2(n, n0, n1);
+  // 2^n from its exponent bits (n = -127: 0)
+  const uint64_t scale = pack2(__uint_as_float((__float_as_uint(n0) << 23) + 0x3f800000u),
+                               __uint_as_float((__float_as_uint(n1) << 23) + 0x3f800000u));
+  unpack2(mul2(q, scale), p0, p1);
+}
+
 __device__ __forceinline__ uint32_t pack_pair(bf16, float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
