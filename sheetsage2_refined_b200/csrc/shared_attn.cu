@@ -341,16 +341,16 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 //
 // The queries of one kv head, (row, group member) pairs in order, are tiles of
 // 128: the MMA's M, one tensor-memory lane and one softmax thread each.  A CTA
-// walks its part of the keys in tiles of KT (128 at dim 64, 64 at dim 128), with
-// two streams in flight, each with a score tile S, a weight tile P, an output
-// accumulator O and a warpgroup of its own:
+// walks its part of the keys in tiles of 64, with two streams in flight, each
+// with a score tile S, a weight tile P, an output accumulator O and a warpgroup
+// of its own:
 //
 //   one query tile (PAIR = false): the streams take the even and the odd key
 //     tiles and are joined at the end;
 //   two query tiles (PAIR = true): stream s is query tile s, both walk every
 //     key tile, which is then read once for 256 queries.
 //
-//   S = Q K^T      tcgen05.mma M128 N=KT K=dim, float32 in tensor memory
+//   S = Q K^T      tcgen05.mma M128 N64 K=dim, float32 in tensor memory
 //   p = 2^(c s - m) c = scale log2(e); m trails the running maximum by at most
 //                  2^8, so that O is rescaled only when the maximum moves far
 //                  (Milakov and Gimelshein's online softmax, with slack)
@@ -363,29 +363,42 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 // float32 values; O is float32 throughout.
 //
 // Warp 0 loads K and V tiles by TMA into a ring, warp 1 issues the MMAs, warps
-// 4-7 and 8-11 are the softmax warpgroups.  A softmax thread takes its whole
-// score row into registers and hands S back at once, so that S of the stream's
-// next tile is computed under this tile's exponentials (with S handed back only
-// with P, each stream waited ~1,850 of every ~4,050 cycles for its products).
-// The exponential unit gives 16 results a cycle and SM, which would bound a
-// large call; a part of the exponentials is computed on the FMA units instead.
+// 4-7 and 8-11 are the softmax warpgroups.  What bounds a large call is the chain
+// of one stream, S -> weights -> O: a warp alone runs the exponentials of a tile at
+// half the rate of their unit, so a CTA is kept small enough for two on an SM:
+//
+//   dim 64: P lies in S's columns, 256 columns and 98 KB a CTA, two CTAs an SM,
+//     four streams.  The next S of a stream follows the product that reads P;
+//     both accumulators are 128 x 64, and MMAs of one accumulator shape execute in
+//     order, so S complete also means the last product complete.
+//   dim 128: O alone fills half the tensor memory; one CTA an SM.  S is handed
+//     back as soon as the softmax has it in registers, P has columns of its own,
+//     and S of the next tile is computed under this tile's exponentials.
+//
 // Every mbarrier wait is bounded; on a timeout the CTA marks its rows NaN, drains
 // its copies and MMAs (bounded), frees its tensor memory and returns.
 constexpr int kTileThreads = 384;
 constexpr int kTileRows = 128;  // queries of a tile
-constexpr int kTileCols = 512;  // tensor memory columns: S, O and P of both streams
+constexpr int KT = 64;          // keys of a tile
 constexpr float kMaxSlack = 8.f;
-constexpr int kPolyPairs = 2;  // of every 8 pairs of weights, computed on the FMA units
-
-__host__ __device__ constexpr int tile_keys(int dim) { return dim == 64 ? 128 : 64; }
 
 template <int D, bool PAIR>
-struct TileSmem {
-  static constexpr int kSlot = tile_keys(D) * D * 2;  // a K or V tile: 16 KB
+struct Tile {
+  static constexpr bool kShareS = D == 64;            // P in S's columns, two CTAs an SM
+  static constexpr int kPerSm = kShareS ? 2 : 1;
+  static constexpr int kCols = kShareS ? 256 : 512;   // tensor memory: S0 S1 O0 O1 (P0 P1)
+  static constexpr uint32_t kAtS = 0, kAtO = 2 * KT, kAtP = kShareS ? kAtS : kAtO + 2 * D;
+  static constexpr uint32_t kStepP = kShareS ? KT : KT / 2;
+  static_assert(kAtO + 2 * D <= kCols && kAtP + KT <= kCols, "fits the tensor memory");
+  // registers: the block's at launch, for the issuing warps and for the softmax warps
+  static constexpr int kRegs = kShareS ? 80 : 168, kRegsIssue = kShareS ? 32 : 40, kRegsSoftmax = kShareS ? 104 : 232;
+  static_assert(kRegsIssue + 2 * kRegsSoftmax <= 3 * kRegs, "within what the block was launched with");
+  static constexpr int kBox = KT * 128;        // bytes of 64 channels of a tile
+  static constexpr int kSlot = KT * D * 2;     // a K or V tile
   static constexpr int kQueries = (PAIR ? 2 : 1) * kTileRows * D * 2;
   static constexpr int kSlots = 8;
   static constexpr int kBytes = kQueries + kSlots * kSlot + 1024;  // + alignment slack
-  static_assert(kBytes + 1024 <= 227 * 1024, "fits an SM");
+  static_assert(kPerSm * (kBytes + 2048) <= 228 * 1024, "fits an SM");
   static_assert(kTileRows * (D + 4) * 4 <= kSlots * kSlot, "a stream's partial fits the ring");
 };
 
@@ -398,20 +411,19 @@ struct TileArgs {
 };
 
 template <typename T, int D, bool PAIR>
-__global__ void __launch_bounds__(kTileThreads, 1)
+__global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
     shared_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ TileArgs t) {
-  using Smem = TileSmem<D, PAIR>;
-  constexpr int kSlots = Smem::kSlots, kBoxes = D / 64, KT = tile_keys(D), kBox = KT * 128;
+  using Shape = Tile<D, PAIR>;
+  constexpr int kSlots = Shape::kSlots, kSlot = Shape::kSlot, kBox = Shape::kBox, kBoxes = D / 64;
   constexpr int kQueryBox = kTileRows * 128;
-  constexpr uint32_t kAtS = 0, kAtO = 2 * KT, kAtP = kAtO + 2 * D;  // tensor memory columns, stream 0
-  static_assert(kAtP + KT <= kTileCols, "fits the tensor memory");
+  constexpr bool kShareS = Shape::kShareS;
   const SharedAttnArgs& a = t.a;
   extern __shared__ __align__(1024) unsigned char tile_smem[];
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tile_smem) + 1023) & ~uintptr_t(1023));
   unsigned char* sq = base;                    // query tiles: [tile][box][128 rows][128 bytes]
-  unsigned char* ring = base + Smem::kQueries;  // slot i: the i-th of K0 V0 K1 V1 ...
+  unsigned char* ring = base + Shape::kQueries;  // slot i: the i-th of K0 V0 K1 V1 ...
   __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], s_full[2], s_empty[2], p_full[2], pv_done[2], done;
   __shared__ uint32_t tmem_base;
   __shared__ int aborted;
@@ -439,7 +451,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
-                 "r"(kTileCols)
+                 "r"(Shape::kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -460,10 +472,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto load_tile = [&](int i) {  // the i-th of K0 V0 K1 V1 ...
     const int slot = i % kSlots, token = (t0 + i / 2) * KT;
     const CUtensorMap* map = i & 1 ? &map_v : &map_k;
-    mbar_expect_tx(&full[slot], Smem::kSlot);
+    mbar_expect_tx(&full[slot], kSlot);
 #pragma unroll
     for (int b = 0; b < kBoxes; ++b)
-      tma_load_3d(ring + slot * Smem::kSlot + b * kBox, map, b * 64, t.token_last ? g : token, t.token_last ? token : g,
+      tma_load_3d(ring + slot * kSlot + b * kBox, map, b * 64, t.token_last ? g : token, t.token_last ? token : g,
                   &full[slot]);
   };
   const int ahead = min(2 * nt, kSlots);  // tiles requested before the queries are staged
@@ -510,10 +522,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   pdl_launch_dependents();
   const uint32_t tmem = tmem_base;
 
-  // The block's registers: 168 a thread at launch; 40 for the issuing warps leave 232 for the softmax
-  // (128 * (40 + 232 + 232) = 384 * 168).
+  // The issuing warps give most of their registers to the softmax warps.
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kRegsIssue));
   if (warp == 0) {
     if (lane == 0) {
       // ---- producer
@@ -530,64 +541,61 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int i = max(0, issued - kSlots); i < issued; ++i) mbar_wait(&full[i % kSlots], (i / kSlots) & 1);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---- MMA issuer
-      constexpr uint32_t kFormat = std::is_same<T, bf16>::value ? 1u : 0u;
-      constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, KT, false);
-      constexpr uint32_t kIdescO = umma_idesc(kFormat, kTileRows, D, true);
-      bool ok = true;
-      auto issue_s = [&](int s, int k, int nth) {  // S_s = Q K_k^T, the stream's nth
-        const int i = 2 * k, slot = i % kSlots;
-        if (!ok) return;
-        if ((nth > 0 && !mbar_wait(&s_empty[s], (nth - 1) & 1)) || !mbar_wait(&full[slot], (i / kSlots) & 1) || stopped()) {
-          ok = false;
-          return;
-        }
-        tmem_fence_after();
-        const uint64_t da = umma_desc_sw128(sq + (PAIR ? s * (kTileRows * D * 2) : 0));
-        const uint64_t db = umma_desc_sw128(ring + slot * Smem::kSlot);
+    // ---- MMA issuer: the warp stays converged (what describes an MMA is then warp-uniform), one
+    // lane issues
+    constexpr uint32_t kFormat = std::is_same<T, bf16>::value ? 1u : 0u;
+    constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, KT, false);
+    constexpr uint32_t kIdescO = umma_idesc(kFormat, kTileRows, D, true);
+    bool ok = true;
+    auto issue_s = [&](int s, int k, int nth) {  // S_s = Q K_k^T, the stream's nth
+      const int i = 2 * k, slot = i % kSlots;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(&full[slot], (i / kSlots) & 1) &&
+                                             (kShareS || nth == 0 || mbar_wait_fast(&s_empty[s], (nth - 1) & 1)));
+      if (!ok) return;
+      tmem_fence_after();
+      const uint64_t da = umma_desc_sw128(sq + (PAIR ? s * (kTileRows * D * 2) : 0));
+      const uint64_t db = umma_desc_sw128(ring + slot * kSlot);
+      if (elect_one()) {
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) {  // 16 channels: 32 bytes of a row, a box every 64
-          umma_f16(tmem + kAtS + s * KT, da + (uint64_t)((e / 4) * (kQueryBox >> 4) + (e % 4) * 2),
+        for (int e = 0; e < D / 16; ++e)  // 16 channels: 32 bytes of a row, a box every 64
+          umma_f16(tmem + Shape::kAtS + s * KT, da + (uint64_t)((e / 4) * (kQueryBox >> 4) + (e % 4) * 2),
                    db + (uint64_t)((e / 4) * (kBox >> 4) + (e % 4) * 2), kIdescS, e > 0);
-        }
         umma_commit(&s_full[s]);
         if (!PAIR || s == 1) umma_commit(&empty[slot]);
-      };
-      auto issue_pv = [&](int s, int k, int nth) {  // O_s += P_s V_k, the stream's nth product
-        const int i = 2 * k + 1, slot = i % kSlots;
-        if (!ok) return;
-        if (!mbar_wait(&p_full[s], nth & 1) || !mbar_wait(&full[slot], (i / kSlots) & 1) || stopped()) {
-          ok = false;
-          return;
-        }
-        tmem_fence_after();
-        const uint64_t db = umma_desc_mn_sw128(ring + slot * Smem::kSlot, kBox);
+      }
+      __syncwarp();
+    };
+    auto issue_pv = [&](int s, int k, int nth) {  // O_s += P_s V_k, the stream's nth product
+      const int i = 2 * k + 1, slot = i % kSlots;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(&full[slot], (i / kSlots) & 1) &&
+                                             mbar_wait_fast(&p_full[s], nth & 1));
+      if (!ok) return;
+      tmem_fence_after();
+      const uint64_t db = umma_desc_mn_sw128(ring + slot * kSlot, kBox);
+      if (elect_one()) {
 #pragma unroll
         for (int e = 0; e < KT / 16; ++e)  // 16 keys: 8 columns of packed P, 16 rows of V
-          umma_f16_ta(tmem + kAtO + s * D, tmem + kAtP + s * (KT / 2) + e * 8, db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO,
-                      nth > 0 || e > 0);
+          umma_f16_ta(tmem + Shape::kAtO + s * D, tmem + Shape::kAtP + s * Shape::kStepP + e * 8,
+                      db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO, nth > 0 || e > 0);
         umma_commit(&pv_done[s]);
         if (!PAIR || s == 1) umma_commit(&empty[slot]);
-      };
-      // S runs one tile of its stream ahead of PV
-      if (PAIR) {
-        for (int s = 0; s < 2 && nt > 0; ++s) issue_s(s, 0, 0);
-        for (int k = 0; k < nt; ++k)
-          for (int s = 0; s < 2; ++s) {
-            if (k + 1 < nt) issue_s(s, k + 1, k + 1);
-            issue_pv(s, k, k);
-          }
-      } else {
-        for (int k = 0; k < min(nt, 2); ++k) issue_s(k, k, 0);
-        for (int k = 0; k < nt; ++k) {
-          if (k + 2 < nt) issue_s(k & 1, k + 2, (k >> 1) + 1);
-          issue_pv(k & 1, k, k >> 1);
-        }
       }
-      if (!ok) fail();
-      umma_commit(&done);  // arrives once every MMA issued has completed
-    }
+      __syncwarp();
+    };
+    // a stream's tile n: query tile or key tiles of its parity
+    const int lag = PAIR ? 1 : 2;
+    for (int s = 0; s < 2; ++s)
+      if ((PAIR ? 0 : s) < nt) issue_s(s, PAIR ? 0 : s, 0);
+    for (int k = 0; k < nt; ++k)
+      for (int s = PAIR ? 0 : k & 1; s <= (PAIR ? 1 : k & 1); ++s) {
+        const int n = PAIR ? k : k >> 1;
+        if (!kShareS && k + lag < nt) issue_s(s, k + lag, n + 1);  // S runs one tile ahead
+        issue_pv(s, k, n);
+        if (kShareS && k + lag < nt) issue_s(s, k + lag, n + 1);
+      }
+    if (!ok && lane == 0) fail();
+    if (elect_one()) umma_commit(&done);  // arrives once every MMA issued has completed
+    __syncwarp();
   }
 
   __syncthreads();
@@ -597,13 +605,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   __syncthreads();  // the softmax warps have read O
   if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTileCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kCols) : "memory");
   if (!PAIR) __syncthreads();
   return;
   }
 
   // ---- softmax: thread = query (tensor-memory lane) of stream s
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kRegsSoftmax));
   const int s = (warp >> 2) - 1;
   const int row = (warp & 3) * 32 + lane;
   const int x = (tile0 + (PAIR ? s : 0)) * kTileRows + row;  // query of the kv head
@@ -614,12 +622,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   bool ok = true;
   {
     const float c = a.scale * kLog2e;
-    const uint32_t s_at = tmem + lanes + kAtS + s * KT, o_at = tmem + lanes + kAtO + s * D;
-    const uint32_t p_at = tmem + lanes + kAtP + s * (KT / 2);
+    const uint32_t s_at = tmem + lanes + Shape::kAtS + s * KT, o_at = tmem + lanes + Shape::kAtO + s * D;
+    const uint32_t p_at = tmem + lanes + Shape::kAtP + s * Shape::kStepP;
     const bool live_warp = x - lane < queries;  // some query of the warp exists
     for (int j = 0; j < mine; ++j) {
       const int k = first + j * step;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], j & 1) && !stopped())) {
+      if (!__all_sync(0xffffffffu, mbar_wait_fast(&s_full[s], j & 1))) {
         ok = false;
         break;
       }
@@ -630,21 +638,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int e = 0; e < KT; e += 32) tmem_ld32(s_at + e, *reinterpret_cast<uint32_t(*)[32]>(v + e));
         tmem_wait_ld();
       }
-      tmem_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[s]);
+      if (!kShareS) {
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[s]);
+      }
       const int live = tokens - (t0 + k) * KT;  // keys of the tile, if fewer
       if (live < KT) {
         // V rows behind the last token may hold anything: zero for the product (P is 0 there)
         const int i = 2 * k + 1, slot = i % kSlots;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kSlots) & 1) && !stopped())) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kSlots) & 1))) {
           ok = false;
           break;
         }
         for (int e = live * 8 + row; e < KT * 8; e += kTileRows)
 #pragma unroll
           for (int b = 0; b < kBoxes; ++b)
-            *reinterpret_cast<uint4*>(ring + slot * Smem::kSlot + b * kBox + e * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(ring + slot * kSlot + b * kBox + e * 16) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
       }
       float to = m, keep = 1.f;
@@ -674,15 +684,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < KT; e += 2) {
-          const uint64_t y = fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, shift2);
           float p0, p1;
-          if (e / 2 % 8 < kPolyPairs) {
-            exp2_poly2(y, p0, p1);
-          } else {
-            unpack2(y, p0, p1);
-            p0 = exp2_approx(p0);
-            p1 = exp2_approx(p1);
-          }
+          unpack2(fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, shift2), p0, p1);
+          p0 = exp2_approx(p0);
+          p1 = exp2_approx(p1);
           sum2[e / 2 & 1] = add2(sum2[e / 2 & 1], pack2(p0, p1));
           v[e / 2] = pack_pair(T(), p0, p1);
         }
@@ -690,8 +695,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         unpack2(add2(sum2[0], sum2[1]), x0, x1);
         l += x0 + x1;
       }
-      // P and O are free once the stream's last product has landed
-      if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[s], (j - 1) & 1))) {
+      // P and O are free once the stream's last product has landed (kShareS: it has, before S)
+      if (!kShareS && j > 0 && !__all_sync(0xffffffffu, mbar_wait_fast(&pv_done[s], (j - 1) & 1))) {
         ok = false;
         break;
       }
@@ -729,7 +734,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
     for (int e = 0; e < D; e += 32) {
       uint32_t v[32];
-      tmem_ld32(tmem + lanes + kAtO + s * D + e, v);
+      tmem_ld32(tmem + lanes + Shape::kAtO + s * D + e, v);
       tmem_wait_ld();
 #pragma unroll
       for (int q = 0; q < 32; ++q) o[e + q] = __uint_as_float(v[q]);
@@ -814,8 +819,7 @@ bool encode_shared(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int
   const cuuint64_t row = (cuuint64_t)token * 2, one = (cuuint64_t)(a.kv_heads == 1 ? token : head) * 2;
   cuuint64_t dims[3] = {(cuuint64_t)a.dim, token_last ? heads : tokens, token_last ? tokens : heads};
   cuuint64_t strides[2] = {token_last ? one : row, token_last ? row : one};
-  const cuuint32_t keys = (cuuint32_t)tile_keys(a.dim);
-  cuuint32_t box[3] = {64, token_last ? 1u : keys, token_last ? keys : 1u};
+  cuuint32_t box[3] = {64, token_last ? 1u : (cuuint32_t)KT, token_last ? (cuuint32_t)KT : 1u};
   cuuint32_t each[3] = {1, 1, 1};
   const CUtensorMapDataType type =
       a.dtype == S2R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -854,7 +858,7 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml
       !encode_shared(&map_v, a, a.shared_v, a.v_token, a.v_head, t.token_last))
     return cudaErrorInvalidValue;
   auto* kernel = shared_tile_kernel<T, D, PAIR>;
-  constexpr int smem = TileSmem<D, PAIR>::kBytes;
+  constexpr int smem = Tile<D, PAIR>::kBytes;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int tiles = PAIR ? (query_tiles(a) + 1) / 2 : query_tiles(a);
@@ -899,16 +903,17 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
   const size_t pairs = (size_t)a.rows * a.heads;
   a.shared_splits = a.own_splits = 0;
   if (a.shared_tokens > 0) {
-    const int tiles = query_tiles(a), keys = (a.shared_tokens + tile_keys(a.dim) - 1) / tile_keys(a.dim);
+    const int tiles = query_tiles(a), keys = (a.shared_tokens + KT - 1) / KT;
     a.pair = tiles > 1;
-    // the split with the fewest key tiles one after the other: waves of CTAs (one an SM) times the
-    // tiles of each plus about 3 tiles' time to start and end it
+    // the split with the fewest key tiles one after the other: waves of CTAs times the tiles of
+    // each, plus about 6 tiles' time to start and end it
     const long long ctas = (long long)(a.pair ? (tiles + 1) / 2 : tiles) * a.kv_heads;
+    const long long slots = (long long)sms * (a.dim == 64 ? 2 : 1);
     long long best = -1;
     for (int sp = 1; sp <= keys && sp <= kMaxSharedSplits; ++sp) {
       const int per = (keys + sp - 1) / sp;
       if ((keys + per - 1) / per != sp) continue;  // the same tiles in fewer parts
-      const long long cost = (ctas * sp + sms - 1) / sms * (per + 3);
+      const long long cost = (ctas * sp + slots - 1) / slots * (per + 6);
       if (best < 0 || cost < best) {
         best = cost;
         a.shared_splits = sp;

@@ -12,6 +12,23 @@
 
 namespace s2r {
 
+// mbar_wait whose first tries come without a look at the timer, for waits in
+// the chain of a tile (reading the timer costs hundreds of cycles).
+__device__ __forceinline__ bool mbar_wait_fast(uint64_t* bar, unsigned parity) {
+  const uint32_t addr = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 128; ++i)
+    if (mbar_try(addr, parity)) return true;
+  return mbar_wait(bar, parity);
+}
+
+// One lane of a converged warp (the same one each time).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // 3-D tiled TMA load of the box at (x, y, z); x in elements, a multiple of 64 here.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -98,41 +115,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t y;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
   return y;
-}
-
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t y;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-  return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
-// 2^x of a pair on the FMA units: x = n + f with n the nearest integer and
-// |f| <= 1/2, 2^f by its series to the fifth power of f ln 2 (the first term
-// left out is (ln2 / 2)^6 / 720 = 2.4e-6 of the result at most), times 2^n.
-// x <= 127; 0 below -126.5; NaN stays NaN.
-__device__ __forceinline__ void exp2_poly2(uint64_t x, float& p0, float& p1) {
-  float x0, x1;
-  unpack2(x, x0, x1);
-  x = pack2(max_nan(x0, -127.f), max_nan(x1, -127.f));
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-  const uint64_t n = add2(x, pack2(kMagic, kMagic));
-  const uint64_t f = add2(x, fma2(n, pack2(-1.f, -1.f), pack2(kMagic, kMagic)));
-  uint64_t q = fma2(f, pack2(1.3333558146e-3f, 1.3333558146e-3f), pack2(9.6181291076e-3f, 9.6181291076e-3f));
-  q = fma2(f, q, pack2(5.5504108665e-2f, 5.5504108665e-2f));
-  q = fma2(f, q, pack2(2.4022650696e-1f, 2.4022650696e-1f));
-  q = fma2(f, q, pack2(6.9314718056e-1f, 6.9314718056e-1f));
-  q = fma2(f, q, pack2(1.f, 1.f));
-  float n0, n1;
-  unpack2(n, n0, n1);
-  // 2^n from its exponent bits (n = -127: 0)
-  const uint64_t scale = pack2(__uint_as_float((__float_as_uint(n0) << 23) + 0x3f800000u),
-                               __uint_as_float((__float_as_uint(n1) << 23) + 0x3f800000u));
-  unpack2(mul2(q, scale), p0, p1);
 }
 
 __device__ __forceinline__ uint32_t pack_pair(bf16, float a, float b) {
