@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kOwnThreads)
   bool timeout = false;
   for (int i = 0; i < loaded; ++i) {
     const uint32_t k_at = smem_u32(ring + (i % kOwnStages) * kOwnStage), v_at = k_at + kOwnStage / 2;
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1))) {
+    if (!__all_sync(0xffffffffu, mbar_wait_fast(&full[warp][i % kOwnStages], (i / kOwnStages) & 1))) {
       timeout = true;
       break;
     }
@@ -394,9 +394,10 @@ struct Tile {
   static constexpr int kRegs = kShareS ? 80 : 168, kRegsIssue = kShareS ? 32 : 40, kRegsSoftmax = kShareS ? 104 : 232;
   static_assert(kRegsIssue + 2 * kRegsSoftmax <= 3 * kRegs, "within what the block was launched with");
   static constexpr int kBox = KT * 128;        // bytes of 64 channels of a tile
-  static constexpr int kSlot = KT * D * 2;     // a K or V tile
+  static constexpr int kTile = KT * D * 2;     // a K or V tile
+  static constexpr int kSlot = 2 * kTile;      // K and V of a key tile
   static constexpr int kQueries = (PAIR ? 2 : 1) * kTileRows * D * 2;
-  static constexpr int kSlots = 8;
+  static constexpr int kSlots = 4;
   static constexpr int kBytes = kQueries + kSlots * kSlot + 1024;  // + alignment slack
   static_assert(kPerSm * (kBytes + 2048) <= 228 * 1024, "fits an SM");
   static_assert(kTileRows * (D + 4) * 4 <= kSlots * kSlot, "a stream's partial fits the ring");
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
     shared_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ TileArgs t) {
   using Shape = Tile<D, PAIR>;
-  constexpr int kSlots = Shape::kSlots, kSlot = Shape::kSlot, kBox = Shape::kBox, kBoxes = D / 64;
+  constexpr int kSlots = Shape::kSlots, kSlot = Shape::kSlot, kTile = Shape::kTile, kBox = Shape::kBox, kBoxes = D / 64;
   constexpr int kQueryBox = kTileRows * 128;
   constexpr bool kShareS = Shape::kShareS;
   const SharedAttnArgs& a = t.a;
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tile_smem) + 1023) & ~uintptr_t(1023));
   unsigned char* sq = base;                    // query tiles: [tile][box][128 rows][128 bytes]
-  unsigned char* ring = base + Shape::kQueries;  // slot i: the i-th of K0 V0 K1 V1 ...
+  unsigned char* ring = base + Shape::kQueries;  // slot k % kSlots: K, then V of the CTA's key tile k
   __shared__ __align__(8) uint64_t full[kSlots], empty[kSlots], s_full[2], s_empty[2], p_full[2], pv_done[2], done;
   __shared__ uint32_t tmem_base;
   __shared__ int aborted;
@@ -469,18 +470,21 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
     *(volatile int*)&aborted = 1;
   };
   auto stopped = [&]() { return *(volatile int*)&aborted != 0; };
-  auto load_tile = [&](int i) {  // the i-th of K0 V0 K1 V1 ...
-    const int slot = i % kSlots, token = (t0 + i / 2) * KT;
-    const CUtensorMap* map = i & 1 ? &map_v : &map_k;
-    mbar_expect_tx(&full[slot], kSlot);
+  auto load_tile = [&](int k) {
+    const int token = (t0 + k) * KT;
+    unsigned char* slot = ring + k % kSlots * kSlot;
+    uint64_t* bar = &full[k % kSlots];
+    mbar_expect_tx(bar, kSlot);
 #pragma unroll
     for (int b = 0; b < kBoxes; ++b)
-      tma_load_3d(ring + slot * kSlot + b * kBox, map, b * 64, t.token_last ? g : token, t.token_last ? token : g,
-                  &full[slot]);
+      tma_load_3d(slot + b * kBox, &map_k, b * 64, t.token_last ? g : token, t.token_last ? token : g, bar);
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b)
+      tma_load_3d(slot + kTile + b * kBox, &map_v, b * 64, t.token_last ? g : token, t.token_last ? token : g, bar);
   };
-  const int ahead = min(2 * nt, kSlots);  // tiles requested before the queries are staged
+  const int ahead = min(nt, kSlots);  // tiles requested before the queries are staged
   if (threadIdx.x == 0)
-    for (int i = 0; i < ahead; ++i) load_tile(i);
+    for (int k = 0; k < ahead; ++k) load_tile(k);
 
   // ---- the queries, in the 128-byte-swizzled rows the MMA reads (by the softmax warps, four
   // pieces in flight each)
@@ -529,16 +533,16 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
     if (lane == 0) {
       // ---- producer
       int issued = ahead;
-      for (int i = ahead; i < 2 * nt; ++i) {
-        if (!mbar_wait(&empty[i % kSlots], (i / kSlots - 1) & 1) || stopped()) {
+      for (int k = ahead; k < nt; ++k) {
+        if (!mbar_wait_fast(&empty[k % kSlots], (k / kSlots - 1) & 1) || stopped()) {
           fail();
           break;
         }
-        load_tile(i);
-        issued = i + 1;
+        load_tile(k);
+        issued = k + 1;
       }
       // every copy has landed before the ring is reused or the CTA exits (bounded)
-      for (int i = max(0, issued - kSlots); i < issued; ++i) mbar_wait(&full[i % kSlots], (i / kSlots) & 1);
+      for (int k = max(0, issued - kSlots); k < issued; ++k) mbar_wait(&full[k % kSlots], (k / kSlots) & 1);
     }
   } else if (warp == 1) {
     // ---- MMA issuer: the warp stays converged (what describes an MMA is then warp-uniform), one
@@ -546,39 +550,43 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
     constexpr uint32_t kFormat = std::is_same<T, bf16>::value ? 1u : 0u;
     constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, KT, false);
     constexpr uint32_t kIdescO = umma_idesc(kFormat, kTileRows, D, true);
+    // The issuer's own waits and commits are a tile's critical resource (some 100 cycles each), so there
+    // is one full and one empty barrier per key tile and nothing is waited for twice.
     bool ok = true;
     auto issue_s = [&](int s, int k, int nth) {  // S_s = Q K_k^T, the stream's nth
-      const int i = 2 * k, slot = i % kSlots;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(&full[slot], (i / kSlots) & 1) &&
-                                             (kShareS || nth == 0 || mbar_wait_fast(&s_empty[s], (nth - 1) & 1)));
-      if (!ok) return;
+      if (!PAIR || s == 0) ok = ok && mbar_wait_fast(&full[k % kSlots], (k / kSlots) & 1);
+      if (!kShareS && nth > 0) ok = ok && mbar_wait_fast(&s_empty[s], (nth - 1) & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        return;
+      }
       tmem_fence_after();
       const uint64_t da = umma_desc_sw128(sq + (PAIR ? s * (kTileRows * D * 2) : 0));
-      const uint64_t db = umma_desc_sw128(ring + slot * kSlot);
+      const uint64_t db = umma_desc_sw128(ring + k % kSlots * kSlot);
       if (elect_one()) {
 #pragma unroll
         for (int e = 0; e < D / 16; ++e)  // 16 channels: 32 bytes of a row, a box every 64
           umma_f16(tmem + Shape::kAtS + s * KT, da + (uint64_t)((e / 4) * (kQueryBox >> 4) + (e % 4) * 2),
                    db + (uint64_t)((e / 4) * (kBox >> 4) + (e % 4) * 2), kIdescS, e > 0);
         umma_commit(&s_full[s]);
-        if (!PAIR || s == 1) umma_commit(&empty[slot]);
       }
       __syncwarp();
     };
     auto issue_pv = [&](int s, int k, int nth) {  // O_s += P_s V_k, the stream's nth product
-      const int i = 2 * k + 1, slot = i % kSlots;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait_fast(&full[slot], (i / kSlots) & 1) &&
-                                             mbar_wait_fast(&p_full[s], nth & 1));
-      if (!ok) return;
+      ok = ok && mbar_wait_fast(&p_full[s], nth & 1);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        return;
+      }
       tmem_fence_after();
-      const uint64_t db = umma_desc_mn_sw128(ring + slot * kSlot, kBox);
+      const uint64_t db = umma_desc_mn_sw128(ring + k % kSlots * kSlot + kTile, kBox);
       if (elect_one()) {
 #pragma unroll
         for (int e = 0; e < KT / 16; ++e)  // 16 keys: 8 columns of packed P, 16 rows of V
           umma_f16_ta(tmem + Shape::kAtO + s * D, tmem + Shape::kAtP + s * Shape::kStepP + e * 8,
                       db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO, nth > 0 || e > 0);
-        umma_commit(&pv_done[s]);
-        if (!PAIR || s == 1) umma_commit(&empty[slot]);
+        if (!kShareS) umma_commit(&pv_done[s]);
+        if (!PAIR || s == 1) umma_commit(&empty[k % kSlots]);
       }
       __syncwarp();
     };
@@ -646,15 +654,14 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
       const int live = tokens - (t0 + k) * KT;  // keys of the tile, if fewer
       if (live < KT) {
         // V rows behind the last token may hold anything: zero for the product (P is 0 there)
-        const int i = 2 * k + 1, slot = i % kSlots;
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (i / kSlots) & 1))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[k % kSlots], (k / kSlots) & 1))) {
           ok = false;
           break;
         }
         for (int e = live * 8 + row; e < KT * 8; e += kTileRows)
 #pragma unroll
           for (int b = 0; b < kBoxes; ++b)
-            *reinterpret_cast<uint4*>(ring + slot * kSlot + b * kBox + e * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(ring + k % kSlots * kSlot + kTile + b * kBox + e * 16) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
       }
       float to = m, keep = 1.f;
@@ -672,12 +679,13 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
           for (int q = 0; q < 4; ++q)
             top[q] = max3(top[q], __uint_as_float(v[e + 2 * q]), __uint_as_float(v[e + 2 * q + 1]));
         to = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        move = to > m + kMaxSlack;
-        to = move ? to : m;
-        keep = m == -INFINITY ? 1.f : exp2f(m - to);
-        move = __any_sync(0xffffffffu, move);
-        m = to;
-        l *= keep;
+        move = __any_sync(0xffffffffu, to > m + kMaxSlack);
+        if (move) {
+          to = to > m + kMaxSlack ? to : m;
+          keep = m == -INFINITY ? 1.f : exp2_approx(m - to);
+          m = to;
+          l *= keep;
+        }
         // the weights 2^(c s - m), in pairs
         const float shift = m == -INFINITY ? 0.f : m;
         const uint64_t c2 = pack2(c, c), shift2 = pack2(-shift, -shift);
