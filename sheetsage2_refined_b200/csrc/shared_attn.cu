@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdio>
 #include <mutex>
@@ -37,19 +38,23 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- the rows' own parts
 //
-// A CTA takes one part of one (row, kv head): two warps, which take its
-// 16 KB chunks of K and V (64 tokens at dim 64, 32 at dim 128; a page is a
-// contiguous 64 x dim block per head) in turn, each through a ring of two
-// chunks of its own that one lane fills by TMA with the 128-byte swizzle.  No
-// barrier beyond the warp: memory bounds this part (a key is read for
-// heads / kv_heads queries), so what counts is bytes in flight, 192 KB an SM.
-// The products are mma.sync m16n8k16, rows = the group's queries (8, or 16 with
-// WIDE): a 128-row tcgen05 tile would hold at most 16 live rows and its round
-// trip through tensor memory would sit in the chain of every chunk.
-constexpr int kOwnThreads = 64;
+// The unit of work is one part of one (row, kv head); a warp takes one unit or,
+// of short rows, several in turn, and reads their K and V in 16 KB chunks (64
+// tokens at dim 64, 32 at dim 128; a page is a contiguous 64 x dim block per
+// head) through a ring of two chunks that one lane fills by TMA with the
+// 128-byte swizzle.  The ring runs on from unit to unit, so rows of a page or
+// two cost no start of their own (a CTA per row and head reached 3.3 TB/s on
+// such rows).  Memory bounds this part (a key is read for heads / kv_heads
+// queries), so what counts is bytes in flight, 192 KB an SM, and there is no
+// barrier beyond the warp.  The products are mma.sync m16n8k16, rows = the
+// group's queries (8, or 16 with WIDE): a 128-row tcgen05 tile would hold at
+// most 16 live rows and its round trip through tensor memory would sit in the
+// chain of every chunk.
+constexpr int kOwnThreads = 32;
 constexpr int kOwnWarps = kOwnThreads / 32;
 constexpr int kOwnStages = 2;
 constexpr int kOwnStage = 16384;  // bytes of a chunk, K then V
+constexpr int kOwnPiece = 16;     // tokens of a box of a row's last chunk
 constexpr int kOwnSmem = kOwnWarps * kOwnStages * kOwnStage + 1024;  // + alignment slack
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -78,219 +83,273 @@ __device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (
 template <typename T, int D, bool WIDE>
 __global__ void __launch_bounds__(kOwnThreads)
     own_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                    const __grid_constant__ SharedAttnArgs a, float* part_o, float2* part_ml, int first_part) {
+                    const __grid_constant__ CUtensorMap map_k_piece, const __grid_constant__ CUtensorMap map_v_piece,
+                    const __grid_constant__ SharedAttnArgs a, bool q_pairs, float* part_o, float2* part_ml, int first_part) {
   constexpr int kTokens = kOwnStage / (4 * D);  // of a chunk: 64 or 32
   constexpr int kBoxes = D / 64, kBox = kTokens * 128;
   constexpr int kHalves = WIDE ? 2 : 1;  // live halves of the MMA's 16 rows
   constexpr int kQueries = 8 * kHalves;
   extern __shared__ __align__(1024) unsigned char own_smem[];
   __shared__ __align__(8) uint64_t full[kOwnWarps][kOwnStages];
-  __shared__ float2 sml[kQueries];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(own_smem) + 1023) & ~uintptr_t(1023));
   unsigned char* ring = base + warp * kOwnStages * kOwnStage;
-  const int part = blockIdx.x, splits = gridDim.x, r = blockIdx.z;
-  const int group = a.heads / a.kv_heads, sets = (group + kQueries - 1) / kQueries;
-  const int g = blockIdx.y / sets, h0 = g * group + (blockIdx.y % sets) * kQueries;
-  const int heads = min(kQueries, (g + 1) * group - h0);
+  const int group = a.heads / a.kv_heads, sets = (group + kQueries - 1) / kQueries, splits = a.own_splits;
+  const int per_row = a.kv_heads * sets * splits;
+  const int units = a.rows * per_row, stride = gridDim.x * kOwnWarps;  // (rows x heads <= 2^24, splits <= 32: below 2^31)
 
   if (lane == 0) {
     for (int i = 0; i < kOwnStages; ++i) mbar_init(&full[warp][i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
   }
   __syncwarp();
-  bool broken = false;
-  int n = a.own_len[r];
-  if (n > a.pages_per_row * kPageTokens) {
-    broken = true;
-    if (threadIdx.x == 0 && a.error) atomicExch(a.error, kErrOwnLength);
-  }
-  n = broken || n < 0 ? 0 : n;
-  const int chunks = (n + kTokens - 1) / kTokens, per = (chunks + splits - 1) / splits;
-  const int c0 = min(chunks, part * per) + warp, c1 = min(chunks, (part + 1) * per);
-  const int mine = c1 > c0 ? (c1 - c0 + kOwnWarps - 1) / kOwnWarps : 0;  // chunks of this warp
 
-  // Page numbers of 32 chunks at a time, one a lane.
-  const int32_t* table = a.page_table + r * a.page_stride;
-  int pages = 0, pages_from = -32;
-  auto load_chunk = [&](int i) -> bool {  // the warp's i-th chunk into its stage
-    if (i >= pages_from + 32) {
-      pages_from = i;
-      const int c = c0 + (i + lane) * kOwnWarps;
-      pages = c < c1 ? table[c * kTokens / kPageTokens] : 0;
-    }
-    const int page = __shfl_sync(0xffffffffu, pages, i - pages_from);
-    if (page < 0 || page >= a.own_pages) {
-      if (lane == 0 && a.error) atomicExch(a.error, kErrOwnPage);
-      return false;
-    }
-    if (lane == 0) {
-      unsigned char* stage = ring + (i % kOwnStages) * kOwnStage;
-      uint64_t* bar = &full[warp][i % kOwnStages];
-      const int token = (page * a.kv_heads + g) * kPageTokens + (c0 + i * kOwnWarps) * kTokens % kPageTokens;
-      mbar_expect_tx(bar, kOwnStage);
-#pragma unroll
-      for (int b = 0; b < kBoxes; ++b) tma_load_2d(stage + b * kBox, &map_k, b * 64, token, bar);
-#pragma unroll
-      for (int b = 0; b < kBoxes; ++b) tma_load_2d(stage + kOwnStage / 2 + b * kBox, &map_v, b * 64, token, bar);
-    }
-    return true;
+  // Chunks [c0, c1) of unit u, given its row's length; a length past the page table counts as 0.
+  auto range = [&](int u, int n, int& c0, int& c1) {
+    const int chunks = ((n < 0 || n > a.pages_per_row * kPageTokens ? 0 : n) + kTokens - 1) / kTokens;
+    const int per = (chunks + splits - 1) / splits, part = u % splits;
+    c0 = min(chunks, part * per);
+    c1 = min(chunks, c0 + per);
   };
-  int loaded = 0;  // chunks requested
-  while (loaded < min(mine, kOwnStages) && !broken) {
-    broken = !load_chunk(loaded);
-    loaded += !broken;
-  }
+  auto length = [&](int u) { return u < units ? a.own_len[u / per_row] : 0; };
 
-  // ---- the queries: A operand of rows lane / 4 (and 8 more), 16 channels a step
-  uint32_t qa[D / 16][4];
+  // ---- the loader: walks the warp's units and their chunks up to kOwnStages chunks ahead.  A unit's
+  // length is requested two units ahead and its first page numbers (32 chunks, one a lane) one unit
+  // ahead, so that no unit starts with a wait for them.
+  int lu = blockIdx.x * kOwnWarps + warp, lc, lc1, base_c, n0, n1, n2, pages, pages1;
+  auto first_pages = [&](int u, int n) {
+    int c0, c1;
+    range(u, n, c0, c1);
+    const int c = c0 + lane;
+    return u < units && c < c1 ? a.page_table[(u / per_row) * a.page_stride + c * kTokens / kPageTokens] : 0;
+  };
+  {
+    n0 = length(lu);
+    n1 = length(lu + stride);
+    n2 = length(lu + 2 * stride);
+    range(lu, n0, lc, lc1);
+    base_c = lc;
+    pages = first_pages(lu, n0);
+    pages1 = first_pages(lu + stride, n1);
+  }
+  int loaded = 0;         // chunks requested
+  unsigned bad_stage = 0;  // stages whose page was broken (nothing was loaded)
+  auto load_next = [&]() {  // one more chunk into stage loaded % kOwnStages, if there is one
+    while (lc >= lc1) {
+      if (lu >= units) return;
+      lu += stride;
+      range(lu, n1, lc, lc1);
+      if (lu >= units) {
+        lc = lc1 = 0;
+        return;
+      }
+      base_c = lc;
+      pages = pages1;
+      n0 = n1;
+      n1 = n2;
+      n2 = length(lu + 2 * stride);
+      pages1 = first_pages(lu + stride, n1);
+    }
+    if (lc >= base_c + 32) {
+      base_c = lc;
+      const int c = lc + lane;
+      pages = c < lc1 ? a.page_table[(lu / per_row) * a.page_stride + c * kTokens / kPageTokens] : 0;
+    }
+    const int page = __shfl_sync(0xffffffffu, pages, lc - base_c), st = loaded % kOwnStages;
+    const bool ok = page >= 0 && page < a.own_pages;
+    bad_stage = ok ? bad_stage & ~(1u << st) : bad_stage | 1u << st;
+    if (lane == 0) {
+      unsigned char* stage = ring + st * kOwnStage;
+      uint64_t* bar = &full[warp][st];
+      if (ok) {
+        const int g = lu / (sets * splits) % a.kv_heads;
+        const int token = (page * a.kv_heads + g) * kPageTokens + lc * kTokens % kPageTokens;
+        const int live = n0 - lc * kTokens;
+        if (live > kTokens - kOwnPiece) {
+          mbar_expect_tx(bar, kOwnStage);
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e)
+          for (int b = 0; b < kBoxes; ++b) tma_load_2d(stage + b * kBox, &map_k, b * 64, token, bar);
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      const int row = lane / 4 + (f & 1) * 8, at = e * 16 + (f >> 1) * 8 + (lane & 3) * 2;
-      qa[e][f] = 0;
-      if ((f & 1) < kHalves && row < heads) {
-        const unsigned short* src =
-            reinterpret_cast<const unsigned short*>(static_cast<const T*>(a.q) + r * a.q_row + (h0 + row) * a.q_head + at);
-        qa[e][f] = src[0] | (uint32_t)src[1] << 16;
+          for (int b = 0; b < kBoxes; ++b) tma_load_2d(stage + kOwnStage / 2 + b * kBox, &map_v, b * 64, token, bar);
+        } else {  // a row's last chunk: only the pieces that hold tokens
+          const int n = (live + kOwnPiece - 1) / kOwnPiece;
+          mbar_expect_tx(bar, n * kOwnPiece * D * 4);
+          for (int x = 0; x < n; ++x)
+#pragma unroll
+            for (int b = 0; b < kBoxes; ++b) {
+              unsigned char* dst = stage + b * kBox + x * (kOwnPiece * 128);
+              tma_load_2d(dst, &map_k_piece, b * 64, token + x * kOwnPiece, bar);
+              tma_load_2d(dst + kOwnStage / 2, &map_v_piece, b * 64, token + x * kOwnPiece, bar);
+            }
+        }
+      } else {
+        mbar_arrive(bar);
+        if (a.error) atomicExch(a.error, kErrOwnPage);
       }
     }
-  const float c = a.scale * kLog2e;
-  float o[D / 8][4], m[kHalves], l[kHalves];
+    ++lc;
+    ++loaded;
+  };
 #pragma unroll
-  for (int e = 0; e < D / 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
-#pragma unroll
-  for (int f = 0; f < kHalves; ++f) m[f] = -INFINITY, l[f] = 0.f;
+  for (int i = 0; i < kOwnStages; ++i) load_next();
 
-  bool timeout = false;
-  for (int i = 0; i < loaded; ++i) {
-    const uint32_t k_at = smem_u32(ring + (i % kOwnStages) * kOwnStage), v_at = k_at + kOwnStage / 2;
-    if (!__all_sync(0xffffffffu, mbar_wait_fast(&full[warp][i % kOwnStages], (i / kOwnStages) & 1))) {
-      timeout = true;
-      break;
-    }
-    const int live = n - (c0 + i * kOwnWarps) * kTokens;  // tokens of the chunk, if fewer
-    if (live < kTokens) {  // V rows behind the last token may hold anything: zero for the product
-      for (int x = live * 8 + lane; x < kTokens * 8; x += 32)
-#pragma unroll
-        for (int b = 0; b < kBoxes; ++b)
-          *reinterpret_cast<uint4*>(ring + (i % kOwnStages) * kOwnStage + kOwnStage / 2 + b * kBox + x * 16) =
-              make_uint4(0, 0, 0, 0);
-      __syncwarp();
-    }
-    // S = Q K^T, 8 keys a tile
-    float s[kTokens / 8][4];
-#pragma unroll
-    for (int j = 0; j < kTokens / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+  // A unit's queries: the A operand of rows lane / 4 (and 8 more), 16 channels a step.
+  auto load_queries = [&](int u, uint32_t (&qa)[D / 16][4]) {
+    const int g = u / (sets * splits) % a.kv_heads, h0 = g * group + u / splits % sets * kQueries;
+    const int heads = min(kQueries, (g + 1) * group - h0);
+    const T* q = static_cast<const T*>(a.q) + (int64_t)(u / per_row) * a.q_row + (int64_t)h0 * a.q_head;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e)
 #pragma unroll
-      for (int j = 0; j < kTokens / 8; j += 2) {
-        const int key = j * 8 + (lane & 7) + (lane >> 4) * 8, piece = e * 2 + ((lane >> 3) & 1);
-        uint32_t b[4];
-        ldmatrix4(b, k_at + (piece / 8) * kBox + sw128_off(key, piece % 8));
-        mma16816(T(), s[j], qa[e], b[0], b[1]);
-        mma16816(T(), s[j + 1], qa[e], b[2], b[3]);
+      for (int f = 0; f < 4; ++f) {
+        const int row = lane / 4 + (f & 1) * 8, at = e * 16 + (f >> 1) * 8 + (lane & 3) * 2;
+        qa[e][f] = 0;
+        if ((f & 1) < kHalves && u < units && row < heads) {
+          const unsigned short* src = reinterpret_cast<const unsigned short*>(q + row * a.q_head + at);
+          qa[e][f] = q_pairs ? *reinterpret_cast<const uint32_t*>(src) : src[0] | (uint32_t)src[1] << 16;
+        }
       }
-    if (live < kTokens) {
+  };
+  const float c = a.scale * kLog2e;
+  uint32_t qa[D / 16][4], qn[D / 16][4];
+  int u = blockIdx.x * kOwnWarps + warp, n_unit = length(u);
+  load_queries(u, qa);
+  int used = 0;  // chunks consumed
+  bool timeout = false;
+  for (; u < units && !timeout; u += stride) {
+    int c0, c1;
+    const int n = n_unit;
+    range(u, n, c0, c1);
+    n_unit = length(u + stride);
+    load_queries(u + stride, qn);  // in flight under this unit
+    bool broken = n > a.pages_per_row * kPageTokens;
+    if (broken && lane == 0 && a.error) atomicExch(a.error, kErrOwnLength);
+    float o[D / 8][4], m[kHalves], l[kHalves];
 #pragma unroll
-      for (int j = 0; j < kTokens / 8; ++j)
+    for (int e = 0; e < D / 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
 #pragma unroll
-        for (int f = 0; f < 4; ++f)
-          if (j * 8 + (lane & 3) * 2 + (f & 1) >= live) s[j][f] = -INFINITY;
+    for (int f = 0; f < kHalves; ++f) m[f] = -INFINITY, l[f] = 0.f;
+
+    for (int k = c0; k < c1; ++k, ++used) {
+      const int st = used % kOwnStages;
+      unsigned char* stage = ring + st * kOwnStage;
+      const uint32_t k_at = smem_u32(stage), v_at = k_at + kOwnStage / 2;
+      if (!__all_sync(0xffffffffu, mbar_wait_fast(&full[warp][st], (used / kOwnStages) & 1))) {
+        timeout = true;
+        break;
+      }
+      if (bad_stage >> st & 1) {
+        broken = true;
+        load_next();
+        continue;
+      }
+      const int live = n - k * kTokens;  // tokens of the chunk, if fewer
+      if (live < kTokens) {  // V rows behind the last token may hold anything: zero for the product
+        for (int x = live * 8 + lane; x < kTokens * 8; x += 32)
+#pragma unroll
+          for (int b = 0; b < kBoxes; ++b)
+            *reinterpret_cast<uint4*>(stage + kOwnStage / 2 + b * kBox + x * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();  // (the stage is filled again by TMA)
+        __syncwarp();
+      }
+      // S = Q K^T, 8 keys a tile
+      float s[kTokens / 8][4];
+#pragma unroll
+      for (int j = 0; j < kTokens / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+        for (int j = 0; j < kTokens / 8; j += 2) {
+          const int key = j * 8 + (lane & 7) + (lane >> 4) * 8, piece = e * 2 + ((lane >> 3) & 1);
+          uint32_t b[4];
+          ldmatrix4(b, k_at + (piece / 8) * kBox + sw128_off(key, piece % 8));
+          mma16816(T(), s[j], qa[e], b[0], b[1]);
+          mma16816(T(), s[j + 1], qa[e], b[2], b[3]);
+        }
+      if (live < kTokens) {
+#pragma unroll
+        for (int j = 0; j < kTokens / 8; ++j)
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            if (j * 8 + (lane & 3) * 2 + (f & 1) >= live) s[j][f] = -INFINITY;
+      }
+      // online softmax of each row (4 lanes hold it)
+      uint32_t pa[kTokens / 16][4];
+#pragma unroll
+      for (int f = 0; f < kHalves; ++f) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kTokens / 8; ++j) top = fmaxf(top, fmaxf(s[j][2 * f], s[j][2 * f + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = fmaxf(top * c, m[f]);
+        if (__any_sync(0xffffffffu, top > m[f])) {
+          const float keep = m[f] == -INFINITY ? 1.f : exp2_approx(m[f] - top);
+          l[f] *= keep;
+#pragma unroll
+          for (int e = 0; e < D / 8; ++e) o[e][2 * f] *= keep, o[e][2 * f + 1] *= keep;
+          m[f] = top;
+        }
+        const float shift = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int j = 0; j < kTokens / 8; ++j) {
+          const float p0 = exp2_approx(fmaf(s[j][2 * f], c, -shift)), p1 = exp2_approx(fmaf(s[j][2 * f + 1], c, -shift));
+          l[f] += p0 + p1;  // (this lane's keys; the row's lanes are added at the end)
+          pa[j / 2][(j & 1) * 2 + f] = pack_pair(T(), p0, p1);
+        }
+      }
+      if (!WIDE) {
+#pragma unroll
+        for (int j = 0; j < kTokens / 16; ++j) pa[j][1] = pa[j][3] = 0;
+      }
+      // O += P V, 8 channels a tile
+#pragma unroll
+      for (int j = 0; j < kTokens / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < D / 8; e += 2) {
+          const int key = j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, piece = e + (lane >> 4);
+          uint32_t b[4];
+          ldmatrix4_trans(b, v_at + (piece / 8) * kBox + sw128_off(key, piece % 8));
+          mma16816(T(), o[e], pa[j], b[0], b[1]);
+          mma16816(T(), o[e + 1], pa[j], b[2], b[3]);
+        }
+      __syncwarp();  // every lane has read the stage
+      load_next();
     }
-    // online softmax of each row (4 lanes hold it)
-    uint32_t pa[kTokens / 16][4];
+    // ---- the unit's sums
+    const int g = u / (sets * splits) % a.kv_heads, h0 = g * group + u / splits % sets * kQueries;
+    const int heads = min(kQueries, (g + 1) * group - h0);
 #pragma unroll
     for (int f = 0; f < kHalves; ++f) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < kTokens / 8; ++j) top = fmaxf(top, fmaxf(s[j][2 * f], s[j][2 * f + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top * c, m[f]);
-      if (__any_sync(0xffffffffu, top > m[f])) {
-        const float keep = m[f] == -INFINITY ? 1.f : exp2f(m[f] - top);
-        l[f] *= keep;
-#pragma unroll
-        for (int e = 0; e < D / 8; ++e) o[e][2 * f] *= keep, o[e][2 * f + 1] *= keep;
-        m[f] = top;
-      }
-      const float shift = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int j = 0; j < kTokens / 8; ++j) {
-        const float p0 = exp2_approx(fmaf(s[j][2 * f], c, -shift)), p1 = exp2_approx(fmaf(s[j][2 * f + 1], c, -shift));
-        l[f] += p0 + p1;  // (this lane's keys; the row's lanes are added at the end)
-        pa[j / 2][(j & 1) * 2 + f] = pack_pair(T(), p0, p1);
-      }
-    }
-    if (!WIDE) {
-#pragma unroll
-      for (int j = 0; j < kTokens / 16; ++j) pa[j][1] = pa[j][3] = 0;
-    }
-    // O += P V, 8 channels a tile
-#pragma unroll
-    for (int j = 0; j < kTokens / 16; ++j)
-#pragma unroll
-      for (int e = 0; e < D / 8; e += 2) {
-        const int key = j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, piece = e + (lane >> 4);
-        uint32_t b[4];
-        ldmatrix4_trans(b, v_at + (piece / 8) * kBox + sw128_off(key, piece % 8));
-        mma16816(T(), o[e], pa[j], b[0], b[1]);
-        mma16816(T(), o[e + 1], pa[j], b[2], b[3]);
-      }
-    __syncwarp();  // every lane has read the stage
-    if (loaded < mine && !broken) {
-      broken = !load_chunk(loaded);
-      loaded += !broken;
-    }
-  }
-  if (timeout) {  // the copies in flight land before the CTA may exit (bounded)
-    for (int i = max(0, loaded - kOwnStages); i < loaded; ++i) mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1);
-    if (lane == 0 && a.error) atomicExch(a.error, kErrSharedWait);
-    broken = true;
-  }
-#pragma unroll
-  for (int f = 0; f < kHalves; ++f) {
-    l[f] += __shfl_xor_sync(0xffffffffu, l[f], 1);
-    l[f] += __shfl_xor_sync(0xffffffffu, l[f], 2);
-    if (broken) l[f] = __uint_as_float(0x7fc00000u);  // a row with broken pages comes out as NaN
-  }
-  // ---- warp 1's sums join warp 0's
-  __syncthreads();  // both warps are done with their stages
-  float* so = reinterpret_cast<float*>(base);  // [kQueries][D + 8]
-#pragma unroll
-  for (int f = 0; f < kHalves; ++f) {
-    const int row = lane / 4 + 8 * f;
-    if (warp == 1) {
-#pragma unroll
-      for (int e = 0; e < D / 8; ++e)
-        *reinterpret_cast<float2*>(so + row * (D + 8) + e * 8 + (lane & 3) * 2) = make_float2(o[e][2 * f], o[e][2 * f + 1]);
-      if ((lane & 3) == 0) sml[row] = make_float2(m[f], l[f]);
-    }
-  }
-  __syncthreads();
-  if (warp == 0) {
-#pragma unroll
-    for (int f = 0; f < kHalves; ++f) {
+      l[f] += __shfl_xor_sync(0xffffffffu, l[f], 1);
+      l[f] += __shfl_xor_sync(0xffffffffu, l[f], 2);
+      if (broken || timeout) l[f] = __uint_as_float(0x7fc00000u);  // a row with broken pages comes out as NaN
       const int row = lane / 4 + 8 * f;
       if (row >= heads) continue;
-      const float2 ml = sml[row];
-      const float top = fmaxf(m[f], ml.x);
-      const float f0 = m[f] == -INFINITY ? 0.f : exp2f(m[f] - top), f1 = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-      const float sum = (m[f] == -INFINITY ? l[f] : l[f] * f0) + (ml.x == -INFINITY ? ml.y : ml.y * f1);
-      const size_t dst = ((size_t)(first_part + part) * a.rows + r) * a.heads + h0 + row;
-      if ((lane & 3) == 0) part_ml[dst] = make_float2(top, sum);
-      if (top == -INFINITY) continue;
+      const size_t dst = ((size_t)(first_part + u % splits) * a.rows + u / per_row) * a.heads + h0 + row;
+      if ((lane & 3) == 0) part_ml[dst] = make_float2(m[f], l[f]);
+      if (m[f] == -INFINITY) continue;
 #pragma unroll
-      for (int e = 0; e < D / 8; ++e) {
-        const float2 x = *reinterpret_cast<const float2*>(so + row * (D + 8) + e * 8 + (lane & 3) * 2);
-        *reinterpret_cast<float2*>(part_o + dst * D + e * 8 + (lane & 3) * 2) =
-            make_float2(fmaf(x.x, f1, o[e][2 * f] * f0), fmaf(x.y, f1, o[e][2 * f + 1] * f0));
-      }
+      for (int e = 0; e < D / 8; ++e)
+        *reinterpret_cast<float2*>(part_o + dst * D + e * 8 + (lane & 3) * 2) = make_float2(o[e][2 * f], o[e][2 * f + 1]);
     }
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) qa[e][f] = qn[e][f];
+  }
+  if (timeout) {  // mark what is left, let the copies in flight land before the CTA exits (bounded)
+    if (lane == 0 && a.error) atomicExch(a.error, kErrSharedWait);
+    for (int i = used; i < loaded; ++i) mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1);
+    for (; u < units; u += stride)
+      for (int row = lane; row < kQueries; row += 32) {
+        const int g = u / (sets * splits) % a.kv_heads, h0 = g * group + u / splits % sets * kQueries;
+        if (h0 + row < (g + 1) * group)
+          part_ml[((size_t)(first_part + u % splits) * a.rows + u / per_row) * a.heads + h0 + row] =
+              make_float2(-INFINITY, __uint_as_float(0x7fc00000u));
+      }
   }
   pdl_launch_dependents();
   pdl_wait();  // this kernel runs beside the shared part; the join waits for both
@@ -836,13 +895,13 @@ bool encode_shared(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A pool of own K or V as rows of `dim` channels, read in boxes of 64 channels x one chunk's tokens.
-bool encode_pool(CUtensorMap* map, const SharedAttnArgs& a, const void* p) {
+// A pool of own K or V as rows of `dim` channels, read in boxes of 64 channels x `tokens`.
+bool encode_pool(CUtensorMap* map, const SharedAttnArgs& a, const void* p, int tokens) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = map_encoder();
   if (!enc) return false;
   cuuint64_t dims[2] = {(cuuint64_t)a.dim, (cuuint64_t)a.own_pages * a.kv_heads * kPageTokens};
   cuuint64_t strides[1] = {(cuuint64_t)a.dim * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)(kOwnStage / (4 * a.dim))};
+  cuuint32_t box[2] = {64, (cuuint32_t)tokens};
   cuuint32_t each[2] = {1, 1};
   const CUtensorMapDataType type =
       a.dtype == S2R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -875,14 +934,25 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml
 
 template <typename T, int D, bool WIDE>
 cudaError_t launch_own(const SharedAttnArgs& a, float* o, float2* ml, cudaStream_t s, bool pdl) {
-  CUtensorMap map_k, map_v;
-  if (!encode_pool(&map_k, a, a.own_k) || !encode_pool(&map_v, a, a.own_v)) return cudaErrorInvalidValue;
+  CUtensorMap map_k, map_v, map_k_piece, map_v_piece;
+  constexpr int kTokens = kOwnStage / (4 * D);
+  if (!encode_pool(&map_k, a, a.own_k, kTokens) || !encode_pool(&map_v, a, a.own_v, kTokens) ||
+      !encode_pool(&map_k_piece, a, a.own_k, kOwnPiece) || !encode_pool(&map_v_piece, a, a.own_v, kOwnPiece))
+    return cudaErrorInvalidValue;
+  const bool q_pairs = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && a.q_row % 2 == 0 && a.q_head % 2 == 0;
   auto* kernel = own_attn_kernel<T, D, WIDE>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOwnSmem);
   if (e != cudaSuccess) return e;
-  const int group = a.heads / a.kv_heads, queries = WIDE ? 16 : 8;
-  const dim3 grid(a.own_splits, a.kv_heads * ((group + queries - 1) / queries), a.rows);
-  return launch(kernel, grid, kOwnThreads, kOwnSmem, s, pdl, map_k, map_v, a, o, ml, a.shared_splits);
+  const long long group = a.heads / a.kv_heads, queries = WIDE ? 16 : 8;
+  const long long units = (long long)a.rows * a.kv_heads * ((group + queries - 1) / queries) * a.own_splits;
+  // a warp takes one unit of long rows (the hardware evens out their lengths; a persistent grid with
+  // units dealt in turn was a quarter slower), or several of short ones, 16 chunks' room in all, as
+  // long as that leaves six warps an SM
+  const long long room = std::max<long long>(1, (long long)a.pages_per_row * (a.dim / 64) / a.own_splits);
+  const long long each = std::max<long long>(1, std::min<long long>(16 / room, units / (6 * 148))) * kOwnWarps;
+  const dim3 grid((unsigned)((units + each - 1) / each));
+  return launch(kernel, grid, kOwnThreads, kOwnSmem, s, pdl, map_k, map_v, map_k_piece, map_v_piece, a, q_pairs, o, ml,
+                a.shared_splits);
 }
 
 template <typename T, int D>
@@ -929,9 +999,11 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     }
   }
   if (a.own_k) {
-    // three CTAs fit an SM; twice that evens out rows of different lengths
+    // six warps an SM, two units for each
+    const int group = a.heads / a.kv_heads, queries = group > 8 ? 16 : 8;
+    const long long pieces = (long long)a.rows * a.kv_heads * ((group + queries - 1) / queries);
     int sp = 1;
-    while (sp < 32 && (long long)a.rows * a.kv_heads * sp < 6ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
+    while (sp < 32 && pieces * sp < 12ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
     a.own_splits = sp;
   }
   const size_t parts = a.shared_splits + a.own_splits;
