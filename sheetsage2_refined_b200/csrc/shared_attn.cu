@@ -366,32 +366,63 @@ __device__ __forceinline__ void store_out(const SharedAttnArgs& a, int r, int h,
   if (a.lse && first) a.lse[(size_t)r * a.heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Joins the parts of every (row, head): a warp each.
+// Joins the parts of every (row, head): a warp each.  The lanes fetch the parts' (m, l) at once, then
+// the parts' sums come eight in flight (one after the other, 30 parts took 9 us).
+constexpr int kJoinAhead = 8;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SharedAttnArgs a, const float* part_o,
                                                    const float2* part_ml, int parts) {
-  pdl_launch_dependents();
-  pdl_wait();
+  constexpr int kEach = D / 32, kRounds = (kMaxSharedSplits + kMaxOwnSplits + 31) / 32;
   const int lane = threadIdx.x & 31;
   const int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), pairs = (int64_t)a.rows * a.heads;
+  pdl_launch_dependents();
+  pdl_wait();
   if (pair >= pairs) return;
-  constexpr int kEach = D / 32;
+  float2 ml[kRounds];
   float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, part_ml[p * pairs + pair].x);
-  float sum = 0.f, acc[kEach];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int p = i * 32 + lane;
+    ml[i] = p < parts ? part_ml[p * pairs + pair] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[i].x);
+  }
+  top = warp_max(top);
+  float sum = 0.f, weight[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    // an empty part (its o is not written): l is 0, or NaN where something broke
+    weight[i] = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - top);
+    sum += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * weight[i];
+  }
+  sum = warp_sum(sum);
+  float acc[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) acc[e] = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = part_ml[p * pairs + pair];
-    if (ml.x == -INFINITY) {  // an empty part (its o is not written): l is 0, or NaN where something broke
-      sum += ml.y;
-      continue;
-    }
-    const float f = exp2f(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    const float* src = part_o + (size_t)(p * pairs + pair) * D + lane * kEach;
+  const float* src = part_o + (size_t)pair * D + lane * kEach;
+  for (int p0 = 0; p0 < parts; p0 += kJoinAhead) {
+    float w[kJoinAhead], x[kJoinAhead][kEach];
+    const float mine = p0 < 32 ? weight[0] : p0 < 64 ? weight[1] : weight[kRounds - 1];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) acc[e] = fmaf(src[e], f, acc[e]);
+    for (int u = 0; u < kJoinAhead; ++u) {
+      w[u] = __shfl_sync(0xffffffffu, mine, (p0 + u) & 31);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) x[u][e] = 0.f;
+      if (w[u] != 0.f) {  // (parts behind the last weigh 0)
+        const float* at = src + (size_t)(p0 + u) * pairs * D;
+        if constexpr (kEach == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(at);
+          x[u][0] = v.x, x[u][1] = v.y;
+        } else {
+          const float4 v = *reinterpret_cast<const float4*>(at);
+          x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) acc[e] = fmaf(x[u][e], w[u], acc[e]);
   }
   store_out<T>(a, (int)(pair / a.heads), (int)(pair % a.heads), lane * kEach, acc, sum, top, lane == 0);
 }
@@ -864,6 +895,20 @@ cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Allow a kernel its dynamic shared memory, once per device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel* kernel, int smem, std::atomic<bool> (&done)[64]) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 64 && done[device].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)  // every kernel of a call wants the same split of an SM's memory
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, (int)cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && device < 64) done[device].store(true, std::memory_order_release);
+  return e;
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -926,7 +971,8 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml
     return cudaErrorInvalidValue;
   auto* kernel = shared_tile_kernel<T, D, PAIR>;
   constexpr int smem = Tile<D, PAIR>::kBytes;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<bool> done[64];
+  const cudaError_t e = allow_smem(kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int tiles = PAIR ? (query_tiles(a) + 1) / 2 : query_tiles(a);
   return launch(kernel, dim3(a.shared_splits, tiles, a.kv_heads), kTileThreads, smem, s, pdl, map_k, map_v, t);
@@ -941,7 +987,8 @@ cudaError_t launch_own(const SharedAttnArgs& a, float* o, float2* ml, cudaStream
     return cudaErrorInvalidValue;
   const bool q_pairs = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && a.q_row % 2 == 0 && a.q_head % 2 == 0;
   auto* kernel = own_attn_kernel<T, D, WIDE>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOwnSmem);
+  static std::atomic<bool> done[64];
+  const cudaError_t e = allow_smem(kernel, kOwnSmem, done);
   if (e != cudaSuccess) return e;
   const long long group = a.heads / a.kv_heads, queries = WIDE ? 16 : 8;
   const long long units = (long long)a.rows * a.kv_heads * ((group + queries - 1) / queries) * a.own_splits;
@@ -1003,7 +1050,7 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     const int group = a.heads / a.kv_heads, queries = group > 8 ? 16 : 8;
     const long long pieces = (long long)a.rows * a.kv_heads * ((group + queries - 1) / queries);
     int sp = 1;
-    while (sp < 32 && pieces * sp < 12ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
+    while (sp < kMaxOwnSplits && pieces * sp < 12ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
     a.own_splits = sp;
   }
   const size_t parts = a.shared_splits + a.own_splits;

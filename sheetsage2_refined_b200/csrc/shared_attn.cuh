@@ -12,6 +12,7 @@ constexpr int kErrOwnPage = 11;    // a page of a row's own K/V outside the pool
 constexpr int kErrOwnLength = 12;  // a row longer than its page table
 constexpr int kErrSharedWait = 13;  // a wait of the shared part timed out
 constexpr int kMaxSharedSplits = 64;
+constexpr int kMaxOwnSplits = 32;
 
 struct SharedAttnArgs {
   int dtype;  // s2r_dtype: bf16 or f16

@@ -26,6 +26,8 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.S2R_F32, torch.bfloat16: _lib.S2R_BF16, torch.float16: _lib.S2R_F16}
 _MASKS = (torch.uint8, torch.bool)
+_NO_OWN = (None, None, 0, 0, None, 0, None)
+_workspace: dict = {}  # bytes by (device, sizes)
 
 
 def _bad(name: str, t, dtype, shape, device) -> ValueError:
@@ -48,15 +50,23 @@ def _vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torc
     return t.data_ptr()
 
 
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without a Stream object, where this torch has it (a few microseconds a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
 def _call(fn, args, device: torch.device) -> None:
     """Run a C entry point with the tensors' device current and its current stream."""
 
     index = device.index
     if torch.cuda.current_device() == index:
-        code = fn(C.byref(args), torch.cuda.current_stream(index).cuda_stream)
+        code = fn(C.byref(args), _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            code = fn(C.byref(args), torch.cuda.current_stream(index).cuda_stream)
+            code = fn(C.byref(args), _raw_stream(index))
     if code:
         _lib.check(code)
 
@@ -100,20 +110,21 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top
         out = torch.empty(rows, dtype=torch.int64, device=device)
     if logprobs is None:
         logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-    each, values = [], []
-    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(value, torch.Tensor):
-            each.append(_vector(name, value, rows, dtype, device))
-            values.append(0)
-        else:
-            each.append(None)
-            values.append(value if name != "top_k" else max(-1, min(int(value), 2**31 - 1)))
+    each_t = each_k = each_p = each_m = None  # per-row parameters
+    if isinstance(temperature, torch.Tensor):
+        each_t, temperature = _vector("temperature", temperature, rows, torch.float32, device), 0.0
+    if isinstance(top_k, torch.Tensor):
+        each_k, top_k = _vector("top_k", top_k, rows, torch.int32, device), 0
+    if isinstance(top_p, torch.Tensor):
+        each_p, top_p = _vector("top_p", top_p, rows, torch.float32, device), 0.0
+    if isinstance(min_p, torch.Tensor):
+        each_m, min_p = _vector("min_p", min_p, rows, torch.float32, device), 0.0
     lib = _lib.load()
     _call(lib.s2r_sample, _lib.SampleArgs(
         logits.data_ptr(), row_stride if rows > 1 else 0, _DTYPES[logits.dtype], rows, vocab,
         None if bias is None else _vector("bias", bias, vocab, torch.float32, device), mask, mask_stride or 0,
-        _vector("uniforms", uniforms, rows, torch.float32, device), *each, *values,
+        _vector("uniforms", uniforms, rows, torch.float32, device), each_t, each_k, each_p, each_m, temperature,
+        max(-1, min(int(top_k), 2**31 - 1)), top_p, min_p,
         _vector("out", out, rows, torch.int64, device), _vector("logprobs", logprobs, rows, torch.float32, device)),
         device)
     return out, logprobs
@@ -147,55 +158,68 @@ def shared_attention(q: torch.Tensor, shared_k: torch.Tensor, shared_v: torch.Te
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3:
         raise ValueError("q must be a [rows, heads, dim] CUDA tensor")
     dtype, device = q.dtype, q.device
-    if dtype not in (torch.bfloat16, torch.float16):
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"q of {dtype}: bfloat16 or float16 expected")
-    rows, heads, dim = q.shape
+    shape = q.shape
+    rows, heads, dim = shape
+    q_row, q_head, one = q.stride()
+    if one != 1:
+        raise _bad("q", q, dtype, shape, device)
+    shared = getattr(shared_k, "shape", ())
     for name, t in (("shared_k", shared_k), ("shared_v", shared_v)):
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.dim() != 3 or (
-                t.shape != shared_k.shape or t.shape[2] != dim or t.stride(2) != 1):
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != shared or (
+                len(shared) != 3 or shared[2] != dim or t.stride(2) != 1):
             raise _bad(name, t, dtype, ("tokens", "kv_heads", dim), device)
-    if q.stride(2) != 1:
-        raise _bad("q", q, dtype, (rows, heads, dim), device)
-    tokens, kv_heads, _ = shared_k.shape
-    own_args = (None, None, 0, 0, None, 0, None)
+    tokens, kv_heads, _ = shared
+    k_token, k_head, _ = shared_k.stride()
+    v_token, v_head, _ = shared_v.stride()
+    own_args, pages = _NO_OWN, 0
     if own_k is not None or own_v is not None or page_table is not None or own_len is not None:
         if own_k is None or own_v is None or page_table is None or own_len is None:
             raise ValueError("own_k, own_v, page_table and own_len go together")
-        shape = (own_k.shape[0] if isinstance(own_k, torch.Tensor) and own_k.dim() else 0, kv_heads,
-                 _lib.S2R_PAGE_TOKENS, dim)
+        pool = (own_k.shape[0] if isinstance(own_k, torch.Tensor) and own_k.dim() else 0, kv_heads,
+                _lib.S2R_PAGE_TOKENS, dim)
         for name, t in (("own_k", own_k), ("own_v", own_v)):
-            if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape or (
+            if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != pool or (
                     not t.is_contiguous()):
-                raise _bad(name, t, dtype, shape, device)
-        if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or (
+                raise _bad(name, t, dtype, pool, device)
+        if not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or (
                 page_table.device != device or page_table.dim() != 2 or page_table.shape[0] != rows or (
                     page_table.shape[1] > 1 and page_table.stride(1) != 1)):
             raise _bad("page_table", page_table, torch.int32, (rows, "pages"), device)
-        own_args = (own_k.data_ptr(), own_v.data_ptr(), shape[0], page_table.shape[1], page_table.data_ptr(),
+        pages = page_table.shape[1]
+        own_args = (own_k.data_ptr(), own_v.data_ptr(), pool[0], pages, page_table.data_ptr(),
                     page_table.stride(0) if rows > 1 else 0, _vector("own_len", own_len, rows, torch.int32, device))
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=dtype, device=device)
-    elif not isinstance(out, torch.Tensor) or out.dtype != dtype or out.device != device or (
-            out.shape != q.shape or out.stride(2) != 1):
-        raise _bad("out", out, dtype, (rows, heads, dim), device)
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif not isinstance(out, torch.Tensor) or out.dtype is not dtype or out.device != device or (
+            out.shape != shape or out.stride(2) != 1):
+        raise _bad("out", out, dtype, shape, device)
     if lse is None:
         lse = torch.empty((rows, heads), dtype=torch.float32, device=device)
-    elif not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 or lse.device != device or (
+    elif not isinstance(lse, torch.Tensor) or lse.dtype is not torch.float32 or lse.device != device or (
             lse.shape != (rows, heads) or not lse.is_contiguous()):
         raise _bad("lse", lse, torch.float32, (rows, heads), device)
-    k_token, k_head, _ = shared_k.stride()
-    v_token, v_head, _ = shared_v.stride()
+    out_row, out_head, _ = out.stride()
     args = _lib.SharedAttentionArgs(
-        _DTYPES[dtype], rows, heads, kv_heads, dim, dim**-0.5 if scale is None else scale,
-        q.data_ptr(), q.stride(0), q.stride(1), shared_k.data_ptr(), shared_v.data_ptr(), k_token, k_head, v_token,
-        v_head, tokens, None if shared_len is None else _vector("shared_len", shared_len, 1, torch.int32, device),
-        *own_args, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), None, 0,
+        _DTYPES[dtype], rows, heads, kv_heads, dim, dim**-0.5 if scale is None else scale, q.data_ptr(), q_row, q_head,
+        shared_k.data_ptr(), shared_v.data_ptr(), k_token, k_head, v_token, v_head, tokens,
+        None if shared_len is None else _vector("shared_len", shared_len, 1, torch.int32, device), *own_args,
+        out.data_ptr(), out_row, out_head, lse.data_ptr(), None, 0,
         None if error is None else _vector("error", error, 1, torch.int32, device))
     lib = _lib.load()
-    with torch.cuda.device(device):
-        need = C.c_int64()
-        _lib.check(lib.s2r_shared_attention_workspace(C.byref(args), C.byref(need)))
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), need.value
-        _call(lib.s2r_shared_attention, args, device)
+    # the workspace a call needs is a function of its sizes: asked for once
+    sizes = (device.index, rows, heads, kv_heads, dim, tokens, pages)
+    need = _workspace.get(sizes)
+    if need is None:
+        count = C.c_int64()
+        with torch.cuda.device(device):
+            _lib.check(lib.s2r_shared_attention_workspace(C.byref(args), C.byref(count)))
+        if len(_workspace) >= 4096:
+            _workspace.clear()
+        need = _workspace[sizes] = count.value
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    _call(lib.s2r_shared_attention, args, device)
     return out, lse
