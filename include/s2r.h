@@ -74,6 +74,11 @@ typedef struct s2r_config {
                                        with batch >= 16 the step projections run on tcgen05 tensor
                                        cores) */
 
+#define S2R_FLAG_SHARED_WINDOW 64u /* every slot decodes one and the same window (several readings of it, or
+                                      one per prompt set): the engine holds one copy of its cross K/V and
+                                      the cross attention reads it once for all slots (s2r_shared_attention).
+                                      Steps run on the tensor-core kernels at any batch; needs width >= 128 */
+
 /* One decoder layer's float32 parameters, named as in
  * TokenDecoder.state_dict() (decoder.py:28-84).  Linear weights are
  * [out, in] row-major, as torch stores them. */
@@ -186,6 +191,10 @@ int32_t s2r_load_frame_tables(s2r_ctx* ctx, int32_t slot, const float* const* ta
  * tensor cores (the arithmetic of the reference's own prefill, so equal to
  * forcing the prefix token by token within the parity tolerance), shorter
  * ones on the decode step's kernels (equal bit for bit).
+ * With S2R_FLAG_SHARED_WINDOW the first load brings the window; later loads
+ * pass `memory` NULL (memory_dtype, memory_frames and frames are then ignored)
+ * and start another reading of it.  Loading another window fails with
+ * S2R_ESTATE while any other slot is loaded, a NULL memory while no window is.
  * Replaces BatchDecoder.load (engine.py:180-232) without rescoring tables. */
 int32_t s2r_load_slot(s2r_ctx* ctx, int32_t slot, const void* memory, int32_t memory_dtype,
                       int32_t memory_frames, int32_t frames, const int64_t* prefix, int32_t n_prefix,
@@ -194,6 +203,30 @@ int32_t s2r_load_slot(s2r_ctx* ctx, int32_t slot, const void* memory, int32_t me
 /* Advance every slot by `n_steps` tokens; finished slots stay put.  No host
  * synchronisation.  Replaces BatchDecoder.run (engine.py:234-246). */
 int32_t s2r_step(s2r_ctx* ctx, int32_t n_steps, void* stream);
+
+/* How a sampled step draws: s2r_sample's parameters per slot [batch] (device
+ * memory), or NULL for the value given below, and the uniforms of every step. */
+typedef struct s2r_sampling {
+  const float* uniforms; /* [n_steps, batch] in [0, 1), device memory, read when the steps run */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all; /* >= 0; 0: greedy */
+  int32_t top_k_all;     /* >= 0; 0: no limit */
+  float top_p_all;       /* 0 .. 1; 1: no limit */
+  float min_p_all;       /* 0 .. 1; 0: no limit */
+  float* logprobs;       /* [n_steps, batch] device memory, or NULL */
+} s2r_sampling;
+
+/* Advance every slot by `n_steps` tokens drawn as s2r_sample does, from the
+ * logits that s2r_step takes the argmax of: mode bias and rescoring added, the
+ * grammar mask applied.  Temperature 0 gives s2r_step's tokens.  Each live
+ * slot's log-probabilities are summed since its load (buffer "logprob", f64),
+ * to rank readings by.  Finished slots stay put (their entries of `logprobs`
+ * mean nothing).  No host synchronisation.  No counterpart in the reference,
+ * which decodes greedily (engine.py:349-350). */
+int32_t s2r_step_sampled(s2r_ctx* ctx, int32_t n_steps, const s2r_sampling* how, void* stream);
 
 /* One step with test hooks (host arrays, each may be NULL): `forced[slot]` >=
  * 0 commits that token instead of the greedy choice (teacher forcing);
@@ -250,8 +283,8 @@ int32_t s2r_take_ready(s2r_ctx* ctx, int32_t slot, int64_t* tokens, int32_t capa
  * 4 f64, 5 i32) of a named engine buffer, for zero-copy views: "token",
  * "position", "finished", "ended", "in_shift", "shift_run", "payload",
  * "last_field", "incomplete", "g", "count", "target", "stop", "out",
- * "frames", "cross_k" / "cross_v" (layer 0's cross K/V, bf16
- * [batch][heads][frames][64], for inspection). Replaces reads of BatchDecoder.state / .out
+ * "frames", "logprob", "cross_k" / "cross_v" (layer 0's cross K/V, bf16
+ * [batch][heads][frames][64], batch 1 with a shared window, for inspection). Replaces reads of BatchDecoder.state / .out
  * (engine.py:138-144). */
 int32_t s2r_get_buffer(s2r_ctx* ctx, const char* name, void** ptr, int64_t* numel, int32_t* dtype);
 

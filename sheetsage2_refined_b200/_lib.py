@@ -18,6 +18,7 @@ S2R_NO_TARGET = (1 << 63) - 1
 S2R_PAGE_TOKENS = 64
 S2R_FLAG_NO_PDL, S2R_FLAG_NO_GRAPH = 1, 2
 S2R_FLAG_NO_TENSOR_CORE = 32
+S2R_FLAG_SHARED_WINDOW = 64
 DTYPE_CODES = {0: "<f4", 1: "<V2", 2: "<i8", 3: "|u1", 4: "<f8", 5: "<i4"}
 
 _fp = C.POINTER(C.c_float)
@@ -104,6 +105,21 @@ class SampleArgs(C.Structure):
     ]
 
 
+class Sampling(C.Structure):
+    _fields_ = [
+        ("uniforms", C.c_void_p),
+        ("temperature", C.c_void_p),
+        ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p),
+        ("temperature_all", C.c_float),
+        ("top_k_all", C.c_int32),
+        ("top_p_all", C.c_float),
+        ("min_p_all", C.c_float),
+        ("logprobs", C.c_void_p),
+    ]
+
+
 class SharedAttentionArgs(C.Structure):
     _fields_ = [
         ("dtype", C.c_int32),
@@ -153,6 +169,7 @@ SIGNATURES = {
     "s2r_load_slot": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32,
                                   C.POINTER(C.c_int64), C.c_int32, C.c_double, C.c_int64, C.c_void_p]),
     "s2r_step": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p]),
+    "s2r_step_sampled": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(Sampling), C.c_void_p]),
     "s2r_step_debug": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "s2r_poll_finished": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "s2r_take": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(C.c_int64), C.c_int32, C.POINTER(C.c_int32),

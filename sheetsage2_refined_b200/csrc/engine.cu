@@ -33,6 +33,8 @@
 #include "kernels.h"
 #include "logits.cuh"
 #include "proj.cuh"
+#include "sample.cuh"
+#include "shared_attn.cuh"
 
 using namespace s2r;
 
@@ -208,6 +210,17 @@ struct s2r_ctx {
   bf16* xln = nullptr;             // [maxM][KP] LayerNorm'd rows, the X operand of LN'd projections
   bf16* mem_bf16 = nullptr;        // [F][D] float32 encoder memory rounded to bf16
   bf16* wckv_all = nullptr;        // [L][2D][D]: every layer's [Wck; Wcv] (layers[l].wckv points into it)
+  // one window's cross K/V for every slot (S2R_FLAG_SHARED_WINDOW): its frames (0: none loaded) and
+  // the workspace of the shared cross attention
+  bool shared = false;
+  int window_frames = 0;
+  void* shared_ws = nullptr;
+  // sampled steps: the graph up to the held logits, the drawn tokens and their log-probabilities
+  cudaGraphExec_t held_graph = nullptr;
+  bool held_dirty = true;
+  int64_t* drawn = nullptr;
+  float* drawn_logprob = nullptr;
+  double* logprob = nullptr;  // [B] sums since the slots' loads
   // profiling: when set, an event is recorded after every launch of a step
   std::vector<std::pair<int, cudaEvent_t>>* prof = nullptr;
 };
@@ -283,6 +296,16 @@ __global__ void slice_major_kernel(const bf16* __restrict__ in, bf16* __restrict
     const int n = (int)(rest % D), sl = (int)(rest / D);
     out[i] = in[(size_t)n * FFN + sl * kSliceCols + j];
   }
+}
+
+// Commit of a sampled step: the drawn tokens (a.forced) in place of the greedy ones, and their
+// log-probabilities added up per live slot.
+__global__ void __launch_bounds__(256) commit_sampled_kernel(const __grid_constant__ LogitsArgs a,
+                                                             const float* __restrict__ logprob, double* sum) {
+  for (int s = threadIdx.x; s < a.M; s += blockDim.x)
+    if (a.st.finished[s] == 0) sum[s] += (double)logprob[s];
+  __syncthreads();
+  commit_rows(a);
 }
 
 // Copy float32 weights (host or device) into `dst` as bfloat16, through a
@@ -675,6 +698,42 @@ int launch_attn(s2r_ctx* c, RowMap rm, int M, int layer, bool cross, cudaStream_
   return S2R_OK;
 }
 
+// The shared window's cross attention for M rows (decode rows or a short prefill chunk): every row
+// attends over the one window's frames (st.frames[0], read on the device), read once for all rows.
+SharedAttnArgs shared_cross_args(const s2r_ctx* c, int M, int layer) {
+  const LayerBufs& w = c->layers[layer];
+  SharedAttnArgs a{};
+  a.dtype = S2R_BF16;
+  a.rows = M;
+  a.heads = a.kv_heads = c->H;
+  a.dim = kHeadDim;
+  a.scale = 0.125f;  // head_dim ** -0.5
+  a.q = c->q;
+  a.q_row = c->D;
+  a.q_head = kHeadDim;
+  a.shared_k = w.ck;
+  a.shared_v = w.cv;
+  a.k_token = a.v_token = kHeadDim;
+  a.k_head = a.v_head = (int64_t)c->F * kHeadDim;
+  a.shared_tokens = c->F;
+  a.shared_len = c->st.frames;
+  a.out = c->att;
+  a.out_row = c->D;
+  a.out_head = kHeadDim;
+  a.workspace = c->shared_ws;
+  a.error = c->dev_error;
+  return a;
+}
+
+int launch_shared_cross(s2r_ctx* c, int M, int layer, cudaStream_t s) {
+  SharedAttnArgs a = shared_cross_args(c, M, layer);
+  plan_shared_attn(a, c->num_sms);
+  a.pdl = next_pdl(c);
+  const char* why = "";
+  const int rc = launch_shared_attn(a, s, &why);
+  return rc == S2R_OK ? rc : fail(rc, "shared cross attention: %s", why);
+}
+
 // Attention of a prefill chunk on tensor cores (prefill_attn.cuh): the chunk's
 // M rows (positions pos0 .. pos0 + M - 1 of one slot) of every head against
 // the slot's keys, key tiles split over a cluster of up to 8 CTAs per head.
@@ -688,13 +747,13 @@ int launch_prefill_attn(s2r_ctx* c, RowMap rm, int M, int layer, bool cross, cud
   const LayerBufs& w = c->layers[layer];
   CUtensorMap map_q, map_k, map_v;
   TRY(encode_rows(&map_q, c->q, c->D, (uint64_t)M, (uint64_t)c->D * sizeof(bf16), kPfRows));
-  const uint64_t key_rows = cross ? (uint64_t)c->B * c->H * c->F : (uint64_t)c->n_pages * c->H * kPageTokens;
+  const uint64_t key_rows = cross ? (uint64_t)(c->shared ? 1 : c->B) * c->H * c->F : (uint64_t)c->n_pages * c->H * kPageTokens;
   TRY(encode_rows(&map_k, cross ? w.ck : w.kpool, kHeadDim, key_rows, kHeadDim * sizeof(bf16), kPfKeys));
   TRY(encode_rows(&map_v, cross ? w.cv : w.vpool, kHeadDim, key_rows, kHeadDim * sizeof(bf16), kPfKeys));
   PrefillAttnArgs a{};
   a.rows = M;
   a.pos0 = rm.pos0;
-  a.slot = rm.slot;
+  a.slot = cross && c->shared ? 0 : rm.slot;
   a.cross = cross;
   a.H = c->H;
   a.D = c->D;
@@ -875,7 +934,9 @@ int enqueue_layer(s2r_ctx* c, RowMap rm, int M, int l, bool last_kv_only, cudaSt
     TRY(launch_proj(c, a, IN_LN, EPI_BF16, s));
     TRY(mark(c, K_CROSS_Q, s));
   }
-  TRY(pf_tile ? launch_prefill_attn(c, rm, M, l, true, s) : launch_attn(c, rm, M, l, true, s));  // 5. cross-attention
+  TRY(pf_tile ? launch_prefill_attn(c, rm, M, l, true, s)  // 5. cross-attention
+      : c->shared ? launch_shared_cross(c, M, l, s)
+                  : launch_attn(c, rm, M, l, true, s));
   TRY(mark(c, K_CROSS_ATTN, s));
   {                                        // 6. cross out-projection + residual
     ProjArgs a = proj_base(c);
@@ -960,10 +1021,8 @@ struct PrefillOnTensorCores {
   }
 };
 
-int enqueue_step(s2r_ctx* c, cudaStream_t s, const int64_t* forced, float* logits, int64_t* greedy) {
-  RowMap rm{0, 0, 0, nullptr};
-  c->fence_next = true;
-  for (int l = 0; l < c->L; ++l) TRY(enqueue_layer(c, rm, c->B, l, false, s));
+// What the logits kernels and the commit of a step read and write.
+LogitsArgs logits_args(s2r_ctx* c, const int64_t* forced, float* logits, int64_t* greedy) {
   LogitsArgs a{};
   a.M = c->B;
   a.V = c->V;
@@ -988,6 +1047,16 @@ int enqueue_step(s2r_ctx* c, cudaStream_t s, const int64_t* forced, float* logit
   a.greedy_out = greedy;
   a.rs = c->rs;
   a.ahead = l2_ahead_of(c, 0, kAheadQkv);  // the next step's first kernel
+  return a;
+}
+
+// `hold`: a sampled step up to its masked logits, with nothing committed.
+int enqueue_step(s2r_ctx* c, cudaStream_t s, const int64_t* forced, float* logits, int64_t* greedy, bool hold = false) {
+  RowMap rm{0, 0, 0, nullptr};
+  c->fence_next = true;
+  for (int l = 0; l < c->L; ++l) TRY(enqueue_layer(c, rm, c->B, l, false, s));
+  LogitsArgs a = logits_args(c, forced, logits, greedy);
+  a.hold = hold;
   if (c->tc) {
     ProjArgs p = proj_base(c);
     p.rm = rm;
@@ -1013,14 +1082,13 @@ int enqueue_step(s2r_ctx* c, cudaStream_t s, const int64_t* forced, float* logit
   return S2R_OK;
 }
 
-int ensure_graph(s2r_ctx* c) {
-  if (!c->graph_dirty && c->graph) return S2R_OK;
-  if (c->graph) {
-    cudaGraphExecDestroy(c->graph);
-    c->graph = nullptr;
+int capture_step(s2r_ctx* c, cudaGraphExec_t* exec, bool hold) {
+  if (*exec) {
+    cudaGraphExecDestroy(*exec);
+    *exec = nullptr;
   }
   CK(cudaStreamBeginCapture(c->cap_stream, cudaStreamCaptureModeThreadLocal));
-  int rc = enqueue_step(c, c->cap_stream, nullptr, nullptr, nullptr);
+  int rc = enqueue_step(c, c->cap_stream, nullptr, hold ? c->dbg_logits : nullptr, nullptr, hold);
   cudaGraph_t graph = nullptr;
   cudaError_t e = cudaStreamEndCapture(c->cap_stream, &graph);
   if (rc != S2R_OK) {
@@ -1028,10 +1096,23 @@ int ensure_graph(s2r_ctx* c) {
     return rc;
   }
   if (e != cudaSuccess) return fail(S2R_ECUDA, "graph capture: %s", cudaGetErrorString(e));
-  e = cudaGraphInstantiate(&c->graph, graph, 0);
+  e = cudaGraphInstantiate(exec, graph, 0);
   cudaGraphDestroy(graph);
   if (e != cudaSuccess) return fail(S2R_ECUDA, "graph instantiate: %s", cudaGetErrorString(e));
+  return S2R_OK;
+}
+
+int ensure_graph(s2r_ctx* c) {
+  if (!c->graph_dirty && c->graph) return S2R_OK;
+  TRY(capture_step(c, &c->graph, false));
   c->graph_dirty = false;
+  return S2R_OK;
+}
+
+int ensure_held_graph(s2r_ctx* c) {
+  if (!c->held_dirty && c->held_graph) return S2R_OK;
+  TRY(capture_step(c, &c->held_graph, true));
+  c->held_dirty = false;
   return S2R_OK;
 }
 
@@ -1094,7 +1175,7 @@ int setup_tensor_core(s2r_ctx* c) {
   const bool allowed = !(c->cfg.flags & S2R_FLAG_NO_TENSOR_CORE);
   if (allowed && !tensor_map_encoder()) return fail(S2R_ECUDA, "the driver has no cuTensorMapEncodeTiled");
   c->tc_cross = allowed;
-  c->tc = allowed && c->B >= kTcMinBatch && c->D >= kTcBlockN;
+  c->tc = allowed && (c->B >= kTcMinBatch || c->shared) && c->D >= kTcBlockN;
   c->tc_prefill = allowed && !c->tc && c->D >= kTcBlockN;
   c->tc_nb = c->B <= 64 ? 64 : c->B <= 128 ? 128 : 256;  // prefill chunks of more rows take several row tiles
   if (!allowed) return S2R_OK;
@@ -1126,6 +1207,7 @@ int check_device_error(s2r_ctx* c, cudaStream_t s) {
               : err == kErrGemmWait  ? "a wait of the tensor-core projection timed out"
               : err == kErrPrefillWait ? "a wait of the prefill attention timed out"
               : err == kErrFfnStage  ? "a bulk copy of the fused FFN did not complete in time"
+              : err == kErrSharedWait ? "a wait of the shared cross attention timed out"
               : err == kErrAccRange  ? "an out-projection partial was too large (or NaN) for the fixed-point sum"
                                      : "unknown code");
 }
@@ -1165,8 +1247,12 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
   if (g->kind == S2R_GRAMMAR_TABLE && (!g->table || g->states <= 0))
     return fail(S2R_EINVAL, "table grammar needs a table and states > 0");
   if (!w->layers) return fail(S2R_EINVAL, "weights.layers is NULL");
-  if ((uint32_t)k.flags & ~(S2R_FLAG_NO_PDL | S2R_FLAG_NO_GRAPH | S2R_FLAG_NO_TENSOR_CORE))
+  if ((uint32_t)k.flags & ~(S2R_FLAG_NO_PDL | S2R_FLAG_NO_GRAPH | S2R_FLAG_NO_TENSOR_CORE | S2R_FLAG_SHARED_WINDOW))
     return fail(S2R_EINVAL, "unknown flag bits 0x%x", (unsigned)k.flags);
+  if (k.flags & S2R_FLAG_SHARED_WINDOW) {
+    if (k.flags & S2R_FLAG_NO_TENSOR_CORE) return fail(S2R_ENOTSUP, "a shared window needs the tensor-core kernels");
+    if (k.width < kTcBlockN) return fail(S2R_ENOTSUP, "a shared window needs a width of at least %d", kTcBlockN);
+  }
 
   int ndev = 0;
   CK(cudaGetDeviceCount(&ndev));
@@ -1189,6 +1275,7 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
   c->n_pages = k.kv_pages > 0 ? k.kv_pages : k.batch * c->pps;
   c->pdl = !(k.flags & S2R_FLAG_NO_PDL);
   c->use_graph = !(k.flags & S2R_FLAG_NO_GRAPH);
+  c->shared = (k.flags & S2R_FLAG_SHARED_WINDOW) != 0;
   cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, device);
   cudaDeviceGetAttribute(&c->smem_per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, device);
   auto cleanup = [&](int rc) {
@@ -1226,7 +1313,7 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
   // launch projects a window for all layers
   TRYC(dalloc(c, &c->wckv_all, (size_t)c->L * 2 * D * D));
   const size_t pool = (size_t)c->n_pages * c->H * kPageTokens * kHeadDim;
-  const size_t cross = (size_t)c->B * c->H * c->F * kHeadDim;
+  const size_t cross = (size_t)(c->shared ? 1 : c->B) * c->H * c->F * kHeadDim;
   for (int l = 0; l < c->L; ++l) {
     const s2r_layer_weights& lw = w->layers[l];
     LayerBufs& b = c->layers[l];
@@ -1334,6 +1421,22 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
     CKC(cudaMemcpy(c->order_self, ident.data(), c->B * sizeof(int32_t), cudaMemcpyHostToDevice));
     CKC(cudaMemcpy(c->order_cross, ident.data(), c->B * sizeof(int32_t), cudaMemcpyHostToDevice));
   }
+  if (c->shared) {  // the shared cross attention of a step and of a short prefill chunk
+    size_t most = 0;
+    for (int m = 1; m <= kFusedPrefillMaxRows; ++m) {
+      SharedAttnArgs a = shared_cross_args(c, m, 0);
+      most = std::max(most, plan_shared_attn(a, c->num_sms));
+    }
+    SharedAttnArgs a = shared_cross_args(c, c->B, 0);
+    most = std::max(most, plan_shared_attn(a, c->num_sms));
+    char* ws = nullptr;
+    TRYC(dalloc(c, &ws, most));
+    c->shared_ws = ws;
+  }
+  TRYC(dalloc(c, &c->drawn, c->B));
+  TRYC(dalloc(c, &c->drawn_logprob, c->B));
+  TRYC(dalloc(c, &c->logprob, c->B));
+  CKC(cudaMemset(c->logprob, 0, (size_t)c->B * sizeof(double)));
   TRYC(dalloc(c, &c->keys, (size_t)c->B * kKeyStride));
   TRYC(dalloc(c, &c->counter, 1));
   TRYC(dalloc(c, &c->dev_error, 1));
@@ -1440,6 +1543,7 @@ int32_t s2r_destroy(s2r_ctx* c) {
   cudaSetDevice(c->device);
   cudaDeviceSynchronize();
   if (c->graph) cudaGraphExecDestroy(c->graph);
+  if (c->held_graph) cudaGraphExecDestroy(c->held_graph);
   if (c->cap_stream) cudaStreamDestroy(c->cap_stream);
   if (c->order_copied) cudaEventDestroy(c->order_copied);
   if (c->h_order) cudaFreeHost(c->h_order);
@@ -1463,7 +1567,7 @@ int32_t s2r_set_logit_bias(s2r_ctx* c, const float* bias) {
   } else {
     CK(cudaMemset(c->bias, 0, (size_t)c->V * sizeof(float)));
   }
-  if (c->has_bias != (bias != nullptr)) c->graph_dirty = true;
+  if (c->has_bias != (bias != nullptr)) c->graph_dirty = c->held_dirty = true;
   c->has_bias = bias != nullptr;
   return S2R_OK;
 }
@@ -1475,7 +1579,7 @@ int32_t s2r_set_rescore(s2r_ctx* c, const s2r_rescore* in) {
   bool on = false;
   if (in)
     for (int t = 0; t < S2R_FRAME_TERMS; ++t) on = on || in->weight[t] != 0.f;
-  c->graph_dirty = true;
+  c->graph_dirty = c->held_dirty = true;
   if (!on) {
     c->rs.on = 0;
     return S2R_OK;
@@ -1554,7 +1658,16 @@ int32_t s2r_load_slot(s2r_ctx* c, int32_t slot, const void* memory, int32_t memo
                       void* stream) {
   if (!c) return fail(S2R_EINVAL, "NULL engine");
   if (slot < 0 || slot >= c->B) return fail(S2R_EINVAL, "slot %d out of range [0, %d)", slot, c->B);
-  if (!memory || (memory_dtype != S2R_F32 && memory_dtype != S2R_BF16)) return fail(S2R_EINVAL, "bad memory argument");
+  const bool reuse = c->shared && !memory;  // another reading of the window already loaded
+  if (reuse) {
+    if (c->window_frames == 0) return fail(S2R_ESTATE, "no window is loaded: the first load needs its memory");
+    frames = memory_frames = c->window_frames;
+  } else if (!memory || (memory_dtype != S2R_F32 && memory_dtype != S2R_BF16)) {
+    return fail(S2R_EINVAL, "bad memory argument");
+  }
+  if (c->shared && !reuse)
+    for (int i = 0; i < c->B; ++i)
+      if (i != slot && c->loaded[i]) return fail(S2R_ESTATE, "slot %d still decodes the window: take it before loading another", i);
   if (frames < 1 || frames > memory_frames || frames > c->F)
     return fail(S2R_EINVAL, "frames %d must be in [1, min(memory_frames %d, engine frames %d)]", frames, memory_frames, c->F);
   if (!prefix || n_prefix < 1) return fail(S2R_EINVAL, "empty prefix");
@@ -1586,8 +1699,16 @@ int32_t s2r_load_slot(s2r_ctx* c, int32_t slot, const void* memory, int32_t memo
   TRY(upload_page_row(c, slot, s));
 
   SlotState& st = c->st;
-  TRY(put<int32_t>(st.frames, slot, frames, s));
-  c->h_frames[slot] = frames;
+  if (c->shared && !reuse) {  // every slot's frames are the window's
+    const std::vector<int32_t> all(c->B, frames);
+    CK(cudaMemcpyAsync(st.frames, all.data(), c->B * sizeof(int32_t), cudaMemcpyHostToDevice, s));
+    std::fill(c->h_frames.begin(), c->h_frames.end(), frames);
+    c->window_frames = frames;
+  } else if (!c->shared) {
+    TRY(put<int32_t>(st.frames, slot, frames, s));
+    c->h_frames[slot] = frames;
+  }
+  TRY(put<double>(c->logprob, slot, 0.0, s));
   TRY(put<double>(st.stop, slot, stop_seconds, s));
   TRY(put<int64_t>(st.target, slot, target, s));
   TRY(put<int64_t>(st.g, slot, gs.g, s));
@@ -1624,8 +1745,8 @@ int32_t s2r_load_slot(s2r_ctx* c, int32_t slot, const void* memory, int32_t memo
   }
   // cross K/V of the window (decoder.py:98-116), written straight into the slot
   const size_t elem = memory_dtype == S2R_F32 ? 4 : 2;
-  CK(cudaMemcpyAsync(c->mem_stage, memory, (size_t)frames * D * elem, cudaMemcpyDefault, s));
-  if (c->tc_cross) {
+  if (!reuse) CK(cudaMemcpyAsync(c->mem_stage, memory, (size_t)frames * D * elem, cudaMemcpyDefault, s));
+  if (c->tc_cross && !reuse) {
     const bf16* x = static_cast<const bf16*>(c->mem_stage);
     if (memory_dtype == S2R_F32) {
       const size_t n = (size_t)frames * D;
@@ -1634,7 +1755,7 @@ int32_t s2r_load_slot(s2r_ctx* c, int32_t slot, const void* memory, int32_t memo
       CK(cudaGetLastError());
       x = c->mem_bf16;
     }
-    TRY(launch_crosskv(c, x, frames, slot, s));
+    TRY(launch_crosskv(c, x, frames, c->shared ? 0 : slot, s));
   }
   for (int l = 0; l < c->L && !c->tc_cross; ++l) {
     ProjArgs a = proj_base(c);
@@ -1688,6 +1809,57 @@ int32_t s2r_step(s2r_ctx* c, int32_t n_steps, void* stream) {
     for (int i = 0; i < n_steps; ++i) TRY(enqueue_step(c, s, nullptr, nullptr, nullptr));
   }
   CK(cudaGetLastError());
+  return S2R_OK;
+}
+
+int32_t s2r_step_sampled(s2r_ctx* c, int32_t n_steps, const s2r_sampling* how, void* stream) {
+  if (!c || !how) return fail(S2R_EINVAL, "NULL argument");
+  if (n_steps <= 0) return S2R_OK;
+  if (!how->uniforms) return fail(S2R_EINVAL, "s2r_step_sampled: uniforms is NULL");
+  if (c->V > S2R_SAMPLE_MAX_VOCAB) return fail(S2R_ENOTSUP, "sampling takes at most %d tokens", S2R_SAMPLE_MAX_VOCAB);
+  if ((!how->temperature && !(how->temperature_all >= 0.f)) || (!how->top_k && how->top_k_all < 0) ||
+      (!how->top_p && !(how->top_p_all >= 0.f && how->top_p_all <= 1.f)) ||
+      (!how->min_p && !(how->min_p_all >= 0.f && how->min_p_all <= 1.f)))
+    return fail(S2R_EINVAL, "s2r_step_sampled: temperature >= 0, top_k >= 0, top_p and min_p in [0, 1] expected");
+  CK(cudaSetDevice(c->device));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int slot = 0; slot < c->B; ++slot) {
+    if (!c->loaded[slot]) continue;
+    c->bound[slot] = std::min(c->bound[slot] + n_steps, c->T - 1);
+    bool changed = false;
+    TRY(grow_pages(c, slot, c->bound[slot], &changed));
+    if (changed) TRY(upload_page_row(c, slot, s));
+  }
+  TRY(upload_row_order(c, s));
+  if (c->use_graph) TRY(ensure_held_graph(c));
+  SampleArgs a{};
+  a.logits = c->dbg_logits;
+  a.dtype = S2R_F32;
+  a.logits_stride = c->V;
+  a.rows = c->B;
+  a.vocab = c->V;
+  a.temperature = how->temperature;
+  a.top_k = how->top_k;
+  a.top_p = how->top_p;
+  a.min_p = how->min_p;
+  a.temperature_all = how->temperature_all;
+  a.top_k_all = how->top_k_all;
+  a.top_p_all = how->top_p_all;
+  a.min_p_all = how->min_p_all;
+  a.tokens = c->drawn;
+  for (int i = 0; i < n_steps; ++i) {
+    if (c->use_graph)
+      CK(cudaGraphLaunch(c->held_graph, s));
+    else
+      TRY(enqueue_step(c, s, nullptr, c->dbg_logits, nullptr, true));
+    a.uniforms = how->uniforms + (size_t)i * c->B;
+    a.logprobs = how->logprobs ? how->logprobs + (size_t)i * c->B : c->drawn_logprob;
+    const char* why = "";
+    const int rc = launch_sample(a, s, &why);
+    if (rc != S2R_OK) return fail(rc, "s2r_step_sampled: %s", why);
+    commit_sampled_kernel<<<1, 256, 0, s>>>(logits_args(c, c->drawn, nullptr, nullptr), a.logprobs, c->logprob);
+    CK(cudaGetLastError());
+  }
   return S2R_OK;
 }
 
@@ -1845,7 +2017,7 @@ int32_t s2r_take_ready(s2r_ctx* c, int32_t slot, int64_t* tokens, int32_t capaci
 int32_t s2r_get_buffer(s2r_ctx* c, const char* name, void** ptr, int64_t* numel, int32_t* dtype) {
   if (!c || !name || !ptr || !numel || !dtype) return fail(S2R_EINVAL, "NULL argument");
   const SlotState& st = c->st;
-  const int64_t B = c->B;
+  const int64_t B = c->B, windows = c->shared ? 1 : B;
   struct Entry {
     const char* name;
     void* p;
@@ -1857,8 +2029,9 @@ int32_t s2r_get_buffer(s2r_ctx* c, const char* name, void** ptr, int64_t* numel,
       {"payload", st.payload, B, 2},      {"last_field", st.last_field, B, 2}, {"incomplete", st.incomplete, B, 2},
       {"g", st.g, B, 2},                  {"count", st.count, B, 2},         {"target", st.target, B, 2},
       {"stop", st.stop, B, 4},            {"out", st.out, B * c->T, 2},      {"frames", st.frames, B, 5},
-      {"cross_k", c->layers[0].ck, B * c->H * c->F * kHeadDim, 1},
-      {"cross_v", c->layers[0].cv, B * c->H * c->F * kHeadDim, 1},
+      {"cross_k", c->layers[0].ck, windows * c->H * c->F * kHeadDim, 1},
+      {"cross_v", c->layers[0].cv, windows * c->H * c->F * kHeadDim, 1},
+      {"logprob", c->logprob, B, 4},
   };
   // "cross_k.<layer>" / "cross_v.<layer>": any layer's cross K/V
   for (const char* which : {"cross_k.", "cross_v."}) {
@@ -1868,7 +2041,7 @@ int32_t s2r_get_buffer(s2r_ctx* c, const char* name, void** ptr, int64_t* numel,
       const long l = std::strtol(name + n, &end, 10);
       if (end == name + n || *end != '\0' || l < 0 || l >= c->L) return fail(S2R_EINVAL, "no buffer named '%s'", name);
       *ptr = which[6] == 'k' ? c->layers[l].ck : c->layers[l].cv;
-      *numel = B * c->H * c->F * kHeadDim;
+      *numel = windows * c->H * c->F * kHeadDim;
       *dtype = 1;
       return S2R_OK;
     }
@@ -1902,7 +2075,7 @@ int32_t s2r_profile_step(s2r_ctx* c, float* ms, double* bytes, int32_t* launches
     if (!fin[b]) {
       ++active;
       self_kv += (double)(pos[b] + 1) * H * kHeadDim * 2 * 2;
-      cross_kv += (double)frames[b] * H * kHeadDim * 2 * 2;
+      if (!c->shared || active == 1) cross_kv += (double)frames[b] * H * kHeadDim * 2 * 2;  // (a shared window once)
     }
   double per[K_CLASSES] = {
       3 * D * D * 2 + 3 * D * 2 + M * D * 8 + M * 3 * D * 2,  // qkv: W, b, r in, x out, q/k/v out
@@ -1992,6 +2165,11 @@ int32_t s2r_profile_step(s2r_ctx* c, float* ms, double* bytes, int32_t* launches
 int32_t s2r_step_launches(s2r_ctx* c) {
   if (!c) return 0;
   // tensor-core engines add a LayerNorm launch before each LayerNorm'd projection and the logits
+  // (a shared window's cross attention: one launch more where it splits the frames, to join the parts)
+  if (c->shared) {
+    SharedAttnArgs a = shared_cross_args(c, c->B, 0);
+    return (plan_shared_attn(a, c->num_sms) ? 12 : 11) * c->L + 2;
+  }
   if (c->tc) return 11 * c->L + 2;
   // attention fused with its out-projection; the cross q launch folds into
   // the cross attention when that computes its own query rows

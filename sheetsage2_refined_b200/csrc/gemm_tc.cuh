@@ -141,9 +141,10 @@ __device__ __forceinline__ void tc_store(const TcArgs& t, int m, int n, float v)
 __device__ __forceinline__ unsigned long long tc_logit_key(const TcArgs& t, uint32_t rule, const RescoreRow& rr, int m,
                                                            int n, float v, float bias) {
   const float logit = round_bf16(v);
-  if (t.lg.logits_out) t.lg.logits_out[(size_t)m * t.lg.V + n] = logit;
+  if (t.lg.logits_out) t.lg.logits_out[(size_t)m * t.lg.V + n] = t.lg.hold ? -INFINITY : logit;
   if (!token_allowed(t.lg.gr, rule, t.lg.V, n)) return 0ull;
   const float x = rescored_token(t.lg.rs, n) ? rescore_logit_call(t.lg.rs, rr, m, n, logit + bias) : logit + bias;
+  if (t.lg.hold) t.lg.logits_out[(size_t)m * t.lg.V + n] = x;
   return argmax_key(x, n);
 }
 
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     if (!is_last) return;
     __threadfence();
-    commit_rows(t.lg);
+    if (!t.lg.hold) commit_rows(t.lg);
     if (threadIdx.x == 0) *t.lg.counter = 0u;
   }
 }

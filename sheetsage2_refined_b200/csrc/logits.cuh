@@ -68,7 +68,9 @@ struct LogitsArgs {
   unsigned long long* keys;  // [M * kKeyStride] (row m at m * kKeyStride), zero between steps
   unsigned int* counter;     // zero between steps
   const int64_t* forced;     // [M] or null: commit forced[m] >= 0 instead of the greedy token
-  float* logits_out;         // [M, V] or null: raw logits
+  float* logits_out;         // [M, V] or null: raw logits, or with `hold` the masked ones
+  int hold;                  // a sampled step: logits_out receives what the choice is made from (bias and
+                             // rescoring added, -inf where the grammar masks) and nothing is committed
   int64_t* greedy_out;       // [M] or null
   Rescore rs;                // frame-head rescoring (rs.on == 0: none)
   L2Ahead ahead;              // what the next step's first kernel reads, prefetched into the L2
@@ -377,11 +379,12 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
           acc = warp_sum(acc);
           if (i < mc) {
             const float logit = round_bf16(acc);
-            if (a.logits_out && lane == 0) a.logits_out[(size_t)(m0 + i) * a.V + v] = logit;
+            if (a.logits_out && lane == 0) a.logits_out[(size_t)(m0 + i) * a.V + v] = a.hold ? -INFINITY : logit;
             const bool ok =
                 a.gr.kind == 1 ? a.gr.table[(size_t)rule[i] * a.V + v] != 0 : ((rule[i] >> cls) & 1u) != 0;
             if (ok) {
               const float x = rescored ? rescore_logit_call(a.rs, rrow[i], m0 + i, v, logit + bias) : logit + bias;
+              if (a.hold && lane == 0) a.logits_out[(size_t)(m0 + i) * a.V + v] = x;
               const unsigned long long k = argmax_key(x, v);
               best[i] = k > best[i] ? k : best[i];
             }
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kLogitsThreads) logits_kernel(const __grid_con
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  commit_rows(a);
+  if (!a.hold) commit_rows(a);
   if (threadIdx.x == 0) *a.counter = 0u;
 }
 

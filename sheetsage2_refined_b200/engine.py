@@ -21,6 +21,13 @@ Differences from the reference, all outside the numerics of a step:
 * ``load`` rejects ``frames < 1`` (the reference produces NaN there) and a
   prefix that does not leave room for one more token (the reference indexes
   past ``out``).
+* ``shared_window=True`` builds an engine whose slots all decode one window
+  (several readings of it, or one per prompt set): the first ``load`` brings
+  the memory, later ones pass ``memory=None``.  The cross K/V is held and read
+  once for all slots.
+* ``run_sampled`` advances the slots with tokens drawn at a temperature from
+  given uniforms (the reference decodes greedily); ``logprob`` holds each
+  slot's summed log-probability.
 * ``BUCKETS`` is kept for callers that read it; the engine attends over each
   slot's exact length, so it plays no part.
 """
@@ -95,7 +102,7 @@ class BatchDecoder:
 
     def __init__(self, decoder, vocab, *, batch: int, frames: int, prompts=FULL_PROMPTS, mode_bias=None,
                  frame_weight=None, dtype=torch.bfloat16, grammar=None, kv_pages: int = 0, flags: int = 0,
-                 device=None):
+                 device=None, shared_window: bool = False):
         if not torch.cuda.is_available():
             raise RuntimeError("the B200 decode engine needs a CUDA device; it has no CPU path")
         lib = _lib.load()
@@ -103,6 +110,9 @@ class BatchDecoder:
             raise RuntimeError("libs2r.so ABI version mismatch")
         self._lib = lib
         self.decoder, self.dtype, self.batch, self.frames = decoder, dtype, batch, frames
+        self.shared_window = bool(shared_window) or bool(flags & _lib.S2R_FLAG_SHARED_WINDOW)
+        if self.shared_window:
+            flags |= _lib.S2R_FLAG_SHARED_WINDOW
         config = _config_of(decoder)
         self.config = config
         self.max_tokens = config.max_tokens
@@ -180,6 +190,7 @@ class BatchDecoder:
         self.state["in_shift"] = self.state["in_shift"].view(torch.bool)
         self.state["finished"] = self.state["finished"].view(torch.bool)
         self.stop = self._view("stop")
+        self.logprob = self._view("logprob")
         self.out = self._view("out").view(batch, self.max_tokens)
         self.bound = [0] * batch
         self.loaded = [False] * batch
@@ -288,8 +299,26 @@ class BatchDecoder:
 
     def load(self, slot: int, memory, prefix: list[int], stop_seconds: float | None, frames: int | None = None,
              frame_logp=None, target: int | None = None) -> None:
-        """Start ``slot`` on a window (engine.py:180-232): ``memory`` ``[1, F, D]`` or ``[F, D]``."""
+        """Start ``slot`` on a window (engine.py:180-232): ``memory`` ``[1, F, D]`` or ``[F, D]``.
 
+        With ``shared_window``, ``memory=None`` starts another reading of the
+        window already loaded (``frames`` is then the window's).
+        """
+
+        if OUT not in prefix:
+            raise ValueError("prefix must contain <out>")
+        toks = (C.c_int64 * len(prefix))(*[int(t) for t in prefix])
+        stop = float("inf") if stop_seconds is None else float(stop_seconds)
+        tgt = _lib.S2R_NO_TARGET if target is None else int(target)
+        if memory is None:
+            if not self.shared_window:
+                raise ValueError("memory=None needs an engine with shared_window=True")
+            tables = self._load_frame_tables(slot, frame_logp) if self.rescore else None
+            _lib.check(self._lib.s2r_load_slot(self._ctx, slot, None, _lib.S2R_BF16, 0, 0, toks, len(prefix), stop, tgt,
+                                               self._stream()))
+            self._retain((tables,))
+            self.bound[slot], self.loaded[slot] = len(prefix) - 1, True
+            return
         frames = self.frames if frames is None else frames
         if isinstance(memory, np.ndarray):
             memory = torch.from_numpy(memory)
@@ -300,11 +329,6 @@ class BatchDecoder:
             mem = mem.to(self.device)
         mem = mem.contiguous()
         dtype = _lib.S2R_F32 if mem.dtype == torch.float32 else _lib.S2R_BF16
-        if OUT not in prefix:
-            raise ValueError("prefix must contain <out>")
-        toks = (C.c_int64 * len(prefix))(*[int(t) for t in prefix])
-        stop = float("inf") if stop_seconds is None else float(stop_seconds)
-        tgt = _lib.S2R_NO_TARGET if target is None else int(target)
         tables = self._load_frame_tables(slot, frame_logp) if self.rescore else None
         _lib.check(self._lib.s2r_load_slot(self._ctx, slot, C.c_void_p(mem.data_ptr()), dtype, mem.shape[0], frames,
                                            toks, len(prefix), stop, tgt, self._stream()))
@@ -315,6 +339,44 @@ class BatchDecoder:
         """Advance every slot by ``steps`` tokens (engine.py:234-246)."""
 
         _lib.check(self._lib.s2r_step(self._ctx, int(steps), self._stream()))
+        self.bound = [min(b + steps, self.max_tokens - 1) if on else b for b, on in zip(self.bound, self.loaded)]
+
+    def run_sampled(self, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                    logprobs: torch.Tensor | None = None) -> None:
+        """Advance every slot by ``uniforms.shape[0]`` drawn tokens.
+
+        ``uniforms`` ``[steps, batch]`` float32 in [0, 1) on the engine's
+        device.  The parameters are numbers or per-slot tensors, as in
+        ``ops.sample``; they apply to the masked, biased and rescored logits
+        that ``run`` takes the argmax of, so ``temperature=0`` gives ``run``'s
+        tokens.  ``logprobs`` ``[steps, batch]`` float32 receives every draw's
+        log-probability; ``logprob`` sums those of live slots.
+        """
+
+        def each(name, value, dtype):
+            if not isinstance(value, torch.Tensor):
+                return None, value
+            if value.dtype != dtype or value.device != self.device or value.shape != (self.batch,) or (
+                    not value.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of {self.batch} values on {self.device}")
+            return value.data_ptr(), 0
+
+        if not isinstance(uniforms, torch.Tensor) or uniforms.dim() != 2 or uniforms.shape[1] != self.batch:
+            raise ValueError(f"uniforms must be a [steps, {self.batch}] tensor")
+        for name, t in (("uniforms", uniforms), ("logprobs", logprobs)):
+            if t is not None and (t.dtype != torch.float32 or t.device != self.device or t.shape != uniforms.shape or
+                                  not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous float32 [steps, {self.batch}] tensor on {self.device}")
+        t_each, t_all = each("temperature", temperature, torch.float32)
+        k_each, k_all = each("top_k", top_k, torch.int32)
+        p_each, p_all = each("top_p", top_p, torch.float32)
+        m_each, m_all = each("min_p", min_p, torch.float32)
+        steps = uniforms.shape[0]
+        how = _lib.Sampling(uniforms.data_ptr(), t_each, k_each, p_each, m_each, t_all,
+                            max(-1, min(int(k_all), 2**31 - 1)), p_all, m_all,
+                            None if logprobs is None else logprobs.data_ptr())
+        _lib.check(self._lib.s2r_step_sampled(self._ctx, steps, C.byref(how), self._stream()))
+        self._retain((uniforms, logprobs, temperature, top_k, top_p, min_p))  # the queued steps read them
         self.bound = [min(b + steps, self.max_tokens - 1) if on else b for b, on in zip(self.bound, self.loaded)]
 
     def step_debug(self, forced=None, want_logits: bool = True):

@@ -16,6 +16,8 @@ the host at the end.
   batching: every free slot is loaded with the next song, the engine runs
   ``poll_every`` steps, finished slots are taken and refilled
   (transcribe.py:279-362 for songs of one window each).
+* ``decode_readings`` draws several transcriptions of one window on an engine
+  with a shared window and ranks them by log-probability.
 * ``decode_box`` is the whole box job on the calling rank: its LPT share of
   the songs through ``decode_songs``, then the gather on rank 0.
 """
@@ -217,3 +219,48 @@ def decode_box(engine, songs: list, costs, poll_every: int = 32, stats: DecodeSt
     share = partition_songs(costs, world)[rank]
     local = decode_songs(engine, {i: songs[i] for i in share}, poll_every, stats)
     return gather_to_rank0(local)
+
+
+@dataclass
+class Reading:
+    """One sampled reading of a window: its tokens (ending in <eos>), why it ended and its log-probability."""
+
+    tokens: list
+    ended: str
+    logprob: float
+
+
+def decode_readings(engine, song: Song, readings: int, *, generator=None, temperature: float = 1.0, top_k: int = 0,
+                    top_p: float = 1.0, min_p: float = 0.0, poll_every: int = 32) -> list[Reading]:
+    """Draw ``readings`` transcriptions of one window, the most probable first.
+
+    ``engine`` is a ``BatchDecoder`` with ``shared_window=True`` and no slot
+    loaded; more readings than slots are decoded as slots finish.  The draws
+    come from ``generator`` (a torch generator on the engine's device; None:
+    torch's default), ``poll_every`` steps at a time.  ``temperature=0`` decodes
+    greedily.
+    """
+
+    import torch
+
+    if not getattr(engine, "shared_window", False):
+        raise ValueError("decode_readings needs an engine with shared_window=True")
+    if readings < 1 or poll_every < 1:
+        raise ValueError("readings and poll_every must be >= 1")
+    if any(engine.loaded):
+        raise ValueError("decode_readings needs an engine with no slot loaded")
+    started, memory, done = 0, song.memory, []
+    while len(done) < readings:
+        for slot in engine.free_slots():
+            if started == readings:
+                break
+            engine.load(slot, memory, song.prefix, song.stop_seconds, song.frames, song.frame_logp, song.target)
+            memory = None  # later readings share the window
+            started += 1
+        uniforms = torch.rand((poll_every, engine.batch), generator=generator, device=engine.device)
+        engine.run_sampled(uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        for slot in engine.finished():
+            logprob = float(engine.logprob[slot])
+            tokens, ended = engine.take(slot)
+            done.append(Reading(tokens, ended, logprob))
+    return sorted(done, key=lambda reading: -reading.logprob)

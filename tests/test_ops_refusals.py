@@ -85,3 +85,62 @@ def test_shared_attention_wrapper_refuses_host_tensors():
     t = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         ops.shared_attention(t, t, t)
+
+
+def test_sampled_step_and_shared_window_refusals():
+    lib = _lib.load()
+    assert lib.s2r_step_sampled(None, 1, C.byref(_lib.Sampling()), None) == _lib.S2R_EINVAL
+    grammar, weights = _lib.GrammarDesc(kind=1, states=1, table=16), _lib.Weights()
+    weights.layers = (_lib.LayerWeights * 1)()
+    ctx = C.c_void_p()
+    for width, flags, word in ((64, 64, b"width of at least"), (256, 64 | 32, b"tensor-core"), (256, 4, b"flag bits")):
+        cfg = _lib.Config(vocab_size=512, width=width, layers=1, heads=width // 64, ffn_width=1024, max_tokens=64,
+                          batch=1, frames=8, flags=flags)
+        rc = lib.s2r_create(C.byref(cfg), C.byref(weights), C.byref(grammar), 0, C.byref(ctx))
+        assert rc in (_lib.S2R_ENOTSUP, _lib.S2R_EINVAL) and word in lib.s2r_last_error()
+
+
+class FakeEngine:
+    """Enough of ``BatchDecoder`` for ``decode_readings``: slot s ends after s + 2 polls."""
+
+    def __init__(self, batch, shared=True):
+        self.batch, self.shared_window, self.device = batch, shared, "cpu"
+        self.loaded, self.left, self.logprob = [False] * batch, [0] * batch, [0.0] * batch
+        self.memories, self.polls = [], 0
+
+    def free_slots(self):
+        return [s for s in range(self.batch) if not self.loaded[s]]
+
+    def load(self, slot, memory, prefix, stop, frames, logp, target):
+        self.memories.append(memory)
+        self.loaded[slot], self.left[slot], self.logprob[slot] = True, slot + 2, -float(len(self.memories))
+
+    def run_sampled(self, uniforms, **kw):
+        assert uniforms.shape == (4, self.batch) and 0 <= float(uniforms.min()) and float(uniforms.max()) < 1
+        self.left = [n - 1 for n in self.left]
+        self.polls += 1
+
+    def finished(self):
+        return [s for s in range(self.batch) if self.loaded[s] and self.left[s] <= 0]
+
+    def take(self, slot):
+        self.loaded[slot] = False
+        return [1, 2], "eos"
+
+
+def test_decode_readings_refills_slots_and_ranks():
+    from sheetsage2_refined_b200.shard import Song, decode_readings
+
+    eng = FakeEngine(3)
+    got = decode_readings(eng, Song("memory", [1, 3]), 8, poll_every=4)
+    assert [r.logprob for r in got] == [-float(i) for i in range(1, 9)]
+    assert eng.memories == ["memory"] + [None] * 7  # the window is brought once
+    for bad in (dict(readings=0), dict(readings=1, poll_every=0)):
+        with pytest.raises(ValueError):
+            decode_readings(FakeEngine(2), Song("m"), **bad)
+    with pytest.raises(ValueError, match="shared_window"):
+        decode_readings(FakeEngine(2, shared=False), Song("m"), 1)
+    busy = FakeEngine(2)
+    busy.loaded[1] = True
+    with pytest.raises(ValueError, match="no slot loaded"):
+        decode_readings(busy, Song("m"), 1)
