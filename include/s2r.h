@@ -74,11 +74,6 @@ typedef struct s2r_config {
                                        with batch >= 16 the step projections run on tcgen05 tensor
                                        cores) */
 
-#define S2R_FLAG_SHARED_WINDOW 64u /* every slot decodes one and the same window (several readings of it, or
-                                      one per prompt set): the engine holds one copy of its cross K/V and
-                                      the cross attention reads it once for all slots (s2r_shared_attention).
-                                      Steps run on the tensor-core kernels at any batch; needs width >= 128 */
-
 /* One decoder layer's float32 parameters, named as in
  * TokenDecoder.state_dict() (decoder.py:28-84).  Linear weights are
  * [out, in] row-major, as torch stores them. */
@@ -130,6 +125,15 @@ const char* s2r_last_error(void);
  * Replaces BatchDecoder.__init__ (engine.py:55-149). */
 int32_t s2r_create(const s2r_config* config, const s2r_weights* weights, const s2r_grammar* grammar,
                    int32_t device, s2r_ctx** out);
+
+/* The same for an engine whose slots all decode one and the same window
+ * (several readings of it, or one per prompt set): it holds one copy of the
+ * window's cross K/V, and its cross attention reads that once for all slots
+ * (s2r_shared_attention).  Its steps run on the tensor-core kernels at any
+ * batch, so the width must be at least 128 and S2R_FLAG_NO_TENSOR_CORE is
+ * refused (S2R_ENOTSUP).  No counterpart in the reference. */
+int32_t s2r_create_shared(const s2r_config* config, const s2r_weights* weights, const s2r_grammar* grammar,
+                          int32_t device, s2r_ctx** out);
 
 /* Free everything the engine owns.  Replaces dropping the engine
  * (transcribe.py:212 frees the old caches before a rebuild). */
@@ -191,7 +195,7 @@ int32_t s2r_load_frame_tables(s2r_ctx* ctx, int32_t slot, const float* const* ta
  * tensor cores (the arithmetic of the reference's own prefill, so equal to
  * forcing the prefix token by token within the parity tolerance), shorter
  * ones on the decode step's kernels (equal bit for bit).
- * With S2R_FLAG_SHARED_WINDOW the first load brings the window; later loads
+ * On an engine of s2r_create_shared the first load brings the window; later loads
  * pass `memory` NULL (memory_dtype, memory_frames and frames are then ignored)
  * and start another reading of it.  Loading another window fails with
  * S2R_ESTATE while any other slot is loaded, a NULL memory while no window is.

@@ -18,7 +18,6 @@ S2R_NO_TARGET = (1 << 63) - 1
 S2R_PAGE_TOKENS = 64
 S2R_FLAG_NO_PDL, S2R_FLAG_NO_GRAPH = 1, 2
 S2R_FLAG_NO_TENSOR_CORE = 32
-S2R_FLAG_SHARED_WINDOW = 64
 DTYPE_CODES = {0: "<f4", 1: "<V2", 2: "<i8", 3: "|u1", 4: "<f8", 5: "<i4"}
 
 _fp = C.POINTER(C.c_float)
@@ -162,6 +161,8 @@ SIGNATURES = {
     "s2r_last_error": (C.c_char_p, []),
     "s2r_create": (C.c_int32, [C.POINTER(Config), C.POINTER(Weights), C.POINTER(GrammarDesc), C.c_int32,
                                C.POINTER(C.c_void_p)]),
+    "s2r_create_shared": (C.c_int32, [C.POINTER(Config), C.POINTER(Weights), C.POINTER(GrammarDesc), C.c_int32,
+                                      C.POINTER(C.c_void_p)]),
     "s2r_destroy": (C.c_int32, [C.c_void_p]),
     "s2r_set_logit_bias": (C.c_int32, [C.c_void_p, C.c_void_p]),
     "s2r_set_rescore": (C.c_int32, [C.c_void_p, C.POINTER(Rescore)]),

@@ -210,7 +210,7 @@ struct s2r_ctx {
   bf16* xln = nullptr;             // [maxM][KP] LayerNorm'd rows, the X operand of LN'd projections
   bf16* mem_bf16 = nullptr;        // [F][D] float32 encoder memory rounded to bf16
   bf16* wckv_all = nullptr;        // [L][2D][D]: every layer's [Wck; Wcv] (layers[l].wckv points into it)
-  // one window's cross K/V for every slot (S2R_FLAG_SHARED_WINDOW): its frames (0: none loaded) and
+  // one window's cross K/V for every slot (s2r_create_shared): its frames (0: none loaded) and
   // the workspace of the shared cross attention
   bool shared = false;
   int window_frames = 0;
@@ -1230,7 +1230,8 @@ int32_t s2r_abi_version(void) { return S2R_ABI_VERSION; }
 
 const char* s2r_last_error(void) { return g_last_error.c_str(); }
 
-int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_grammar* g, int32_t device, s2r_ctx** out) {
+static int32_t create_engine(const s2r_config* cfg, const s2r_weights* w, const s2r_grammar* g, int32_t device, s2r_ctx** out,
+                             bool shared) {
   if (!cfg || !w || !g || !out) return fail(S2R_EINVAL, "s2r_create: NULL argument");
   *out = nullptr;
   const s2r_config k = *cfg;
@@ -1247,9 +1248,9 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
   if (g->kind == S2R_GRAMMAR_TABLE && (!g->table || g->states <= 0))
     return fail(S2R_EINVAL, "table grammar needs a table and states > 0");
   if (!w->layers) return fail(S2R_EINVAL, "weights.layers is NULL");
-  if ((uint32_t)k.flags & ~(S2R_FLAG_NO_PDL | S2R_FLAG_NO_GRAPH | S2R_FLAG_NO_TENSOR_CORE | S2R_FLAG_SHARED_WINDOW))
+  if ((uint32_t)k.flags & ~(S2R_FLAG_NO_PDL | S2R_FLAG_NO_GRAPH | S2R_FLAG_NO_TENSOR_CORE))
     return fail(S2R_EINVAL, "unknown flag bits 0x%x", (unsigned)k.flags);
-  if (k.flags & S2R_FLAG_SHARED_WINDOW) {
+  if (shared) {
     if (k.flags & S2R_FLAG_NO_TENSOR_CORE) return fail(S2R_ENOTSUP, "a shared window needs the tensor-core kernels");
     if (k.width < kTcBlockN) return fail(S2R_ENOTSUP, "a shared window needs a width of at least %d", kTcBlockN);
   }
@@ -1275,7 +1276,7 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
   c->n_pages = k.kv_pages > 0 ? k.kv_pages : k.batch * c->pps;
   c->pdl = !(k.flags & S2R_FLAG_NO_PDL);
   c->use_graph = !(k.flags & S2R_FLAG_NO_GRAPH);
-  c->shared = (k.flags & S2R_FLAG_SHARED_WINDOW) != 0;
+  c->shared = shared;
   cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, device);
   cudaDeviceGetAttribute(&c->smem_per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, device);
   auto cleanup = [&](int rc) {
@@ -1536,6 +1537,15 @@ int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_gramma
   return S2R_OK;
 #undef TRYC
 #undef CKC
+}
+
+int32_t s2r_create(const s2r_config* cfg, const s2r_weights* w, const s2r_grammar* g, int32_t device, s2r_ctx** out) {
+  return create_engine(cfg, w, g, device, out, false);
+}
+
+int32_t s2r_create_shared(const s2r_config* cfg, const s2r_weights* w, const s2r_grammar* g, int32_t device,
+                          s2r_ctx** out) {
+  return create_engine(cfg, w, g, device, out, true);
 }
 
 int32_t s2r_destroy(s2r_ctx* c) {

@@ -110,9 +110,7 @@ class BatchDecoder:
             raise RuntimeError("libs2r.so ABI version mismatch")
         self._lib = lib
         self.decoder, self.dtype, self.batch, self.frames = decoder, dtype, batch, frames
-        self.shared_window = bool(shared_window) or bool(flags & _lib.S2R_FLAG_SHARED_WINDOW)
-        if self.shared_window:
-            flags |= _lib.S2R_FLAG_SHARED_WINDOW
+        self.shared_window = bool(shared_window)
         config = _config_of(decoder)
         self.config = config
         self.max_tokens = config.max_tokens
@@ -172,7 +170,8 @@ class BatchDecoder:
                           batch=batch, frames=frames, kv_pages=kv_pages, flags=flags)
         ctx = C.c_void_p()
         with torch.cuda.device(self.device):
-            _lib.check(lib.s2r_create(C.byref(cfg), C.byref(w), C.byref(gd), self.device.index or 0, C.byref(ctx)))
+            create = lib.s2r_create_shared if self.shared_window else lib.s2r_create
+            _lib.check(create(C.byref(cfg), C.byref(w), C.byref(gd), self.device.index or 0, C.byref(ctx)))
         self._ctx = ctx
         del keep
         if self.mode_bias is not None:

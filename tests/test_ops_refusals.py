@@ -93,10 +93,10 @@ def test_sampled_step_and_shared_window_refusals():
     grammar, weights = _lib.GrammarDesc(kind=1, states=1, table=16), _lib.Weights()
     weights.layers = (_lib.LayerWeights * 1)()
     ctx = C.c_void_p()
-    for width, flags, word in ((64, 64, b"width of at least"), (256, 64 | 32, b"tensor-core"), (256, 4, b"flag bits")):
+    for width, flags, word in ((64, 0, b"width of at least"), (256, 32, b"tensor-core"), (256, 4, b"flag bits")):
         cfg = _lib.Config(vocab_size=512, width=width, layers=1, heads=width // 64, ffn_width=1024, max_tokens=64,
                           batch=1, frames=8, flags=flags)
-        rc = lib.s2r_create(C.byref(cfg), C.byref(weights), C.byref(grammar), 0, C.byref(ctx))
+        rc = lib.s2r_create_shared(C.byref(cfg), C.byref(weights), C.byref(grammar), 0, C.byref(ctx))
         assert rc in (_lib.S2R_ENOTSUP, _lib.S2R_EINVAL) and word in lib.s2r_last_error()
 
 
