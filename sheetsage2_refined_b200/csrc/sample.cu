@@ -13,20 +13,25 @@
 //           before temperature and filters, to rank readings by.
 //
 // Every filter keeps a prefix of one order, so what is kept is "values above a
-// threshold, and the first few of the threshold's ties".  The threshold is
-// found in two exchanges: a histogram of counts (top-k) or weights (top-p) over
-// 1024 bins linear in M - x, which a decoder's logits fill evenly, then the
-// tokens of the bin in which the sum crosses its target, gathered and sorted.
-// When that bin holds more than 2048 tokens (masses of equal values) a radix
-// search over the 32-bit images of the values takes over.
+// threshold, and the first few of the threshold's ties".  Most draws keep few
+// tokens, and those are found by a sieve: where k lanes hold a value of at least
+// L, so do k tokens, so the k-th largest of what each lane holds at most bounds
+// the k-th largest token from below, and little more than k tokens pass it.  Up
+// to 2048 of them are gathered and finished by one CTA.  Top-p alone tries the
+// same with the bound of 128 lanes: a decoder's nucleus is a few tokens.  Where
+// the sieve passes too many, or too little weight, the threshold is searched
+// among all: a histogram of counts (top-k) or weights (top-p) over 1024 bins
+// linear in M - x, then the tokens of the bin in which the sum crosses its
+// target, gathered and sorted; and when that bin holds too many (masses of equal
+// values), radix rounds over the images.
 //
 // Weights are fixed-point integers, rint(exp(.) * 2^(61 - bits(vocab))), with
 // the exponential in 64 bits: which token is drawn depends on which side of a
 // border a running sum falls, integer sums do not depend on the order in
 // which threads add, and the rounding (2^-46 of the largest weight at 32,576
 // tokens) is far below what a 32-bit sum could resolve.  Tokens whose weight
-// rounds to 0 cannot be drawn and are left out from the start.  With top-k the
-// counts come first, so that only the k survivors need the exponential.
+// rounds to 0 cannot be drawn.  With top-k only what passed the sieve needs the
+// exponential.
 //
 // A row is one thread-block cluster of C CTAs, each holding a contiguous
 // share of the vocabulary as images in shared memory; sums cross the cluster
@@ -55,22 +60,25 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 1024;  // of either histogram
 constexpr int kSampleBinBits = 10;
 constexpr int kSampleMaxSplits = 16;
-constexpr int kSampleListMax = 1024;   // tokens of the crossing bin that are gathered and sorted
-constexpr int kSampleFinishMax = 256;  // kept tokens that one CTA finishes alone
+constexpr int kSampleNucleus = 128;   // lanes whose bound the sieve takes for top-p alone
 constexpr uint32_t kImgNegInf = 0x007fffffu;  // image of -inf: tokens at or below it are never drawn
 constexpr uint32_t kImgPosInf = 0xff800000u;
 
+// Tokens of a list that is gathered: past the sieve, or of the crossing bin.  (Few splits come with
+// large shares of the vocabulary and many rows: half the lists let two CTAs fit an SM.)
+__host__ __device__ constexpr int list_max(int splits) { return splits >= 4 ? 2048 : 1024; }
+
+template <int C>
 struct alignas(16) SampleShared {  // (the images behind it are stored four at a time)
   u64 hist[2][kSampleBins];             // by parity of the exchange, so one cluster barrier each suffices
-  u64 cross[kSampleListMax];            // this CTA's tokens of the crossing bin
-  u64 survive[kSampleFinishMax];        // ... and of it and the bins above
-  u64 sorted[kSampleListMax];           // the cluster's, in order
+  u64 list[list_max(C)];                // this CTA's tokens past the sieve, or of the crossing bin
+  u64 sorted[list_max(C)];              // the cluster's
   u64 inbox[2][kSampleMaxSplits][2];    // what the peers sent, by parity of the exchange
   u64 part[kSampleWarps];               // per-warp values of a block reduction
   u64 scan[kSampleWarps];
   double pow2[64];                      // 2^(j / 64)
   u64 found[2];
-  unsigned crossing, surviving;
+  unsigned listed, counts[kSampleWarps];
 };
 
 // Order-preserving image of a float (select.cuh): -0 as +0, every NaN on top.
@@ -88,54 +96,81 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
-// This warp's images [w0, w1) of the allowed tokens (0: masked) into shared memory, and the largest
-// and the lowest drawable of each lane.  VEC: the row's logits, mask and bias allow four tokens a load.
+// What a lane knows of its tokens after loading them: the largest and the lowest drawable image, and
+// z = sum exp(x - m) over the allowed with m the largest value (kept up as the sum of a running softmax).
+struct LaneStats {
+  uint32_t top = 0, bottom = 0xffffffffu;
+  float m = -INFINITY, z = 0.f;
+};
+
+// This warp's images [w0, w1) of the allowed tokens (0: masked) into shared memory.  VEC: the row's
+// logits, mask and bias allow four tokens a load.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_images(const T* __restrict__ logits, const float* __restrict__ bias,
                                             const uint8_t* __restrict__ allowed, uint32_t* img, int w0, int w1,
-                                            uint32_t& top, uint32_t& bottom) {
-  constexpr int kEach = VEC ? 4 : 1;
+                                            LaneStats& st) {
+  constexpr int kEach = VEC ? 4 : 1, kBatch = VEC ? 4 : 2;  // loads in flight a lane: kBatch of each kind
   const int lane = threadIdx.x & 31;
-#pragma unroll 4
-  for (int i = w0 + lane * kEach; i < w1; i += 32 * kEach) {
-    float x[kEach];
-    bool ok[kEach];
-    if constexpr (VEC) {
-      alignas(16) T raw[4];
-      if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<uint4*>(raw) = __ldg(reinterpret_cast<const uint4*>(logits + i));
-      else
-        *reinterpret_cast<uint2*>(raw) = __ldg(reinterpret_cast<const uint2*>(logits + i));
-      const uint32_t m = allowed ? __ldg(reinterpret_cast<const uint32_t*>(allowed + i)) : 0xffffffffu;
-      const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll 1
+  for (int i0 = w0 + lane * kEach; i0 < w1; i0 += 32 * kEach * kBatch) {
+    alignas(16) T raw[kBatch][kEach];
+    float4 b[VEC ? kBatch : 1];
+    float b1[kBatch];
+    uint32_t mask[kBatch];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = bias ? __fadd_rn(to_float(raw[j]), bb[j]) : to_float(raw[j]);
-        ok[j] = ((m >> (8 * j)) & 0xffu) != 0;
+    for (int q = 0; q < kBatch; ++q) {
+      const int i = i0 + q * 32 * kEach;
+      mask[q] = 0;
+      if (i >= w1) continue;
+      if constexpr (VEC) {
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<uint4*>(raw[q]) = __ldg(reinterpret_cast<const uint4*>(logits + i));
+        else
+          *reinterpret_cast<uint2*>(raw[q]) = __ldg(reinterpret_cast<const uint2*>(logits + i));
+        mask[q] = allowed ? __ldg(reinterpret_cast<const uint32_t*>(allowed + i)) : 0xffffffffu;
+        b[q] = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        raw[q][0] = logits[i];
+        mask[q] = allowed ? allowed[i] : 1u;
+        b1[q] = bias ? bias[i] : 0.f;
       }
-    } else {
-      x[0] = to_float(logits[i]);
-      if (bias) x[0] = __fadd_rn(x[0], bias[i]);
-      ok[0] = !allowed || allowed[i];
     }
-    uint32_t u[kEach];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      u[j] = ok[j] ? value_image(x[j]) : 0u;
-      top = u[j] > top ? u[j] : top;
-      if (u[j] > kImgNegInf) bottom = u[j] < bottom ? u[j] : bottom;
+    for (int q = 0; q < kBatch; ++q) {
+      const int i = i0 + q * 32 * kEach;
+      if (i >= w1) break;
+      float x[kEach];
+      uint32_t u[kEach];
+      float m = st.m;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const float add = VEC ? (j == 0 ? b[q].x : j == 1 ? b[q].y : j == 2 ? b[q].z : b[q].w) : b1[q];
+        const bool ok = ((mask[q] >> (8 * j)) & 0xffu) != 0;
+        x[j] = bias ? __fadd_rn(to_float(raw[q][j]), add) : to_float(raw[q][j]);
+        u[j] = ok ? value_image(x[j]) : 0u;
+        st.top = u[j] > st.top ? u[j] : st.top;
+        if (u[j] > kImgNegInf) st.bottom = u[j] < st.bottom ? u[j] : st.bottom;
+        x[j] = ok ? x[j] : -INFINITY;
+        m = fmaxf(m, x[j]);
+      }
+      if (m != -INFINITY) {
+        float z = st.z * __expf(st.m - m);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) z += __expf(x[j] - m);
+        st.z = z;
+        st.m = m;
+      }
+      if constexpr (VEC)
+        *reinterpret_cast<uint4*>(img + i) = make_uint4(u[0], u[1], u[2], u[3]);
+      else
+        img[i] = u[0];
     }
-    if constexpr (VEC)
-      *reinterpret_cast<uint4*>(img + i) = make_uint4(u[0], u[1], u[2], u[3]);
-    else
-      img[i] = u[0];
   }
 }
 
 template <typename T>
 __device__ __forceinline__ void load_images(const SampleArgs& a, int r, int first, uint32_t* img, int w0, int w1,
-                                            uint32_t& top, uint32_t& bottom) {
+                                            LaneStats& st) {
   const T* logits = static_cast<const T*>(a.logits) + (size_t)r * a.logits_stride + first;
   const uint8_t* allowed = a.allowed ? a.allowed + (size_t)r * a.allowed_stride + first : nullptr;
   const float* bias = a.bias ? a.bias + first : nullptr;
@@ -145,22 +180,28 @@ __device__ __forceinline__ void load_images(const SampleArgs& a, int r, int firs
   int from = w0;
   if (vec) {
     from = w0 + (w1 - w0) / 4 * 4;
-    load_images<T, true>(logits, bias, allowed, img, w0, from, top, bottom);
+    load_images<T, true>(logits, bias, allowed, img, w0, from, st);
   }
-  load_images<T, false>(logits, bias, allowed, img, from, w1, top, bottom);
+  load_images<T, false>(logits, bias, allowed, img, from, w1, st);
+}
+
+// The warps' partials, one a lane (twice over a warp), added up by every warp for itself.
+__device__ __forceinline__ u64 sum_partials(u64 v) {
+#pragma unroll
+  for (int o = kSampleWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 // One row's search state; every thread of the cluster (of C CTAs) holds the same values.
 template <int C>
 struct RowSampler {
-  SampleShared& sh;
+  SampleShared<C>& sh;
   const uint32_t* img;  // this CTA's images
   int first;            // its share of the vocabulary
   int rank;
   int w0, w1;           // this warp's part of the share
   int turn = 0;         // exchanges done (parity of the buffers)
   float best;
-  float cut;     // tokens with best - x >= cut weigh nothing
   double inv_t;  // 1 / (T ln 2)
   int scale_bits;
 
@@ -182,10 +223,7 @@ struct RowSampler {
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = v;
     __syncthreads();
-    u64 s = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) s += sh.part[w];
-    return s;
+    return sum_partials(sh.part[threadIdx.x & (kSampleWarps - 1)]);
   }
   // Send a block-uniform pair to every CTA of the cluster; behind the barrier inbox[r] holds rank
   // r's.  Senders write into the peers' memory, so what follows reads only this CTA's own.
@@ -199,6 +237,23 @@ struct RowSampler {
     }
     barrier();
     return box;
+  }
+
+  // Bins of best - x, `per_unit` to a unit, the largest values in bin 0.
+  float per_unit;
+  __device__ int bin_of(uint32_t u) const { return min(kSampleBins - 1, (int)((best - image_value(u)) * per_unit)); }
+  // The lowest image whose bin is at most `b` (the bins fall as the images rise): 32 probes a round,
+  // by every warp for itself.
+  __device__ uint32_t bin_floor(int b) const {
+    uint32_t lo = kImgNegInf + 1, n = value_image(best) - kImgNegInf;  // candidates lo .. lo + n - 1; the last one is in
+    while (n > 1) {
+      const uint32_t step = (n + 31) / 32, at = lo + min((uint32_t)(threadIdx.x & 31) * step + step - 1, n - 1);
+      const unsigned in = __ballot_sync(0xffffffffu, bin_of(at) <= b);
+      const uint32_t skip = (uint32_t)(__ffs(in) - 1) * step;  // the first group whose last candidate is in
+      lo += skip;
+      n = min(step, n - skip);
+    }
+    return lo;
   }
 
   // rint(exp((x - best) / T) * 2^scale_bits): y = (x - best) / (T ln 2) = k / 64 + f, 2^y =
@@ -236,7 +291,7 @@ struct RadixResult {
 };
 template <bool COUNT, int C>
 __device__ __noinline__ RadixResult shrink_radix(RowSampler<C> row, Kept kept, u64 target) {
-  SampleShared& sh = row.sh;
+  SampleShared<C>& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t lo = kept.lo + (kept.last < 0 ? 1u : 0u), hi = value_image(row.best);  // open range, both inclusive
   u64 above = 0;                                                                    // sum over images > hi
@@ -395,7 +450,8 @@ __device__ __forceinline__ int gather(RowSampler<C>& row, const u64* list, const
 }
 
 // Inclusive sums over the block's threads.
-__device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* all) {
+template <int C>
+__device__ __forceinline__ u64 block_scan(SampleShared<C>& sh, u64 v, u64* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -404,14 +460,15 @@ __device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* all) {
   }
   if (lane == 31) sh.scan[warp] = v;
   __syncthreads();
-  u64 sum = 0;
+  u64 w = sh.scan[lane & (kSampleWarps - 1)];  // the warps' sums, scanned by every warp for itself
 #pragma unroll
-  for (int w = 0; w < kSampleWarps; ++w) {
-    if (w < warp) v += sh.scan[w];
-    sum += sh.scan[w];
+  for (int o = 1; o < kSampleWarps; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, w, o, kSampleWarps);
+    if ((lane & (kSampleWarps - 1)) >= o) w += x;
   }
-  *all = sum;
-  return v;
+  *all = __shfl_sync(0xffffffffu, w, kSampleWarps - 1);
+  const u64 below = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+  return warp ? v + below : v;
 }
 
 __device__ __forceinline__ u64 share_of(float share, u64 all) {  // the least sum that holds a share
@@ -419,22 +476,153 @@ __device__ __forceinline__ u64 share_of(float share, u64 all) {  // the least su
   return goal < 1.0 ? 1ull : goal >= (double)all ? all : (u64)goal;
 }
 
-struct DrawArgs {  // what is left of a row once its survivors are gathered
+// This CTA's sum of the threads' parts, in a fixed order.
+template <int C>
+__device__ __forceinline__ float block_sum_f32(SampleShared<C>& sh, float z) {
+  z = warp_sum(z);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = __float_as_uint(z);
+  __syncthreads();
+  z = __uint_as_float((uint32_t)sh.part[threadIdx.x & (kSampleWarps - 1)]);
+#pragma unroll
+  for (int o = kSampleWarps / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  return z;
+}
+
+struct DrawArgs {  // a row's filters and its uniform
   int k;
   float p, uniform;
   u64 floor_w;
 };
 
-enum Shrunk { kShrunkAll, kShrunk, kShrunkDone };
+// The integer target of the running sums: the token's sum is the first above it.
+__device__ __forceinline__ u64 draw_target(float uniform, u64 total) {
+  const u64 goal = uniform > 0.f ? (u64)((double)uniform * (double)total) : 0ull;
+  return goal >= total ? total - 1 : goal;
+}
+
+// The key in bin `bin` of the n gathered tokens at which a filter's running sum (COUNT: of tokens, `above`
+// before the bin; else of weights, `above_w` before it) reaches `target`: the bin's tokens are listed and
+// each adds up what lies above it among them.  `through`: the weight up to and with that key.
+template <bool COUNT, int C>
+__device__ u64 cross_key(RowSampler<C>& row, int n, int bin, u64 above, u64 above_w, u64 target, uint16_t* places,
+                         u64* through) {
+  SampleShared<C>& sh = row.sh;
+  const u64* weight = sh.list;
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kSampleThreads)
+    if (row.bin_of((uint32_t)(sh.sorted[i] >> 32)) == bin) places[atomicAdd(&sh.listed, 1u)] = (uint16_t)i;
+  __syncthreads();
+  const int c = (int)sh.listed;
+  for (int x = threadIdx.x; x < c; x += kSampleThreads) {
+    const int i = places[x];
+    const u64 key = sh.sorted[i];
+    u64 rank = 0, w = 0;
+    for (int y = 0; y < c; ++y) {
+      const int j = places[y];
+      if (sh.sorted[j] > key) {
+        ++rank;
+        w += weight[j];
+      }
+    }
+    const u64 before = COUNT ? above + rank : above_w + w;
+    if (before < target && before + (COUNT ? 1ull : weight[i]) >= target) {
+      sh.found[0] = key;
+      sh.found[1] = above_w + w + weight[i];
+    }
+  }
+  __syncthreads();
+  *through = sh.found[1];
+  const u64 key = sh.found[0];
+  __syncthreads();
+  return key;
+}
+
+// All filters and the draw on the n gathered tokens of sh.sorted, in index order (rank 0's CTA alone).  They
+// hold the k largest (COUNT), or are all there are above some value: then the prefix that reaches
+// `target` is kept, if they reach it; else the answer is false.  Leaves the drawn token's key in
+// sh.found[0].  The thresholds come from one histogram of the gathered tokens, counts and weights.
+template <bool COUNT, int C>
+__device__ __noinline__ bool finish(RowSampler<C> row, int n, uint32_t lowest, u64 target, const DrawArgs& d) {
+  SampleShared<C>& sh = row.sh;
+  constexpr int kEach = list_max(C) / kSampleThreads;
+  // the histograms' memory is free here: counts, low and high words of the weights, places of a bin's tokens
+  uint32_t* hist = reinterpret_cast<uint32_t*>(sh.hist[0]);
+  uint16_t* places = reinterpret_cast<uint16_t*>(hist + 3 * kSampleBins);
+  static_assert(3 * kSampleBins * sizeof(uint32_t) + list_max(C) * sizeof(uint16_t) <= sizeof(sh.hist), "fits");
+  u64* weight = sh.list;  // by place
+  row.per_unit = fminf((float)kSampleBins / (row.best - image_value(lowest)), 3e38f);
+  for (int b = threadIdx.x; b < 3 * kSampleBins; b += kSampleThreads) hist[b] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kSampleThreads) {
+    const uint32_t u = (uint32_t)(sh.sorted[i] >> 32);
+    const u64 w = row.weight(u);
+    uint32_t* bin = hist + row.bin_of(u);
+    weight[i] = w;
+    atomicAdd(bin, 1u);
+    const uint32_t low = (uint32_t)w, old = atomicAdd(bin + kSampleBins, low);
+    const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
+    if (high) atomicAdd(bin + 2 * kSampleBins, high);
+  }
+  __syncthreads();
+  const int b0 = 2 * (int)threadIdx.x;
+  const u64 c0 = hist[b0], c1 = hist[b0 + 1];
+  const u64 v0 = hist[kSampleBins + b0] | (u64)hist[2 * kSampleBins + b0] << 32;
+  const u64 v1 = hist[kSampleBins + b0 + 1] | (u64)hist[2 * kSampleBins + b0 + 1] << 32;
+  u64 all = 0, total = 0;
+  const u64 run_c = block_scan(sh, c0 + c1, &all) - c0 - c1;
+  __syncthreads();
+  const u64 run_w = block_scan(sh, v0 + v1, &total) - v0 - v1;
+  u64 least = 0;  // tokens with a key from here on are kept
+  if (COUNT && n > d.k) {
+    const u64 k = (u64)d.k;
+    if (run_c < k && run_c + c0 + c1 >= k) {
+      const bool second = run_c + c0 < k;
+      sh.part[0] = b0 + second;
+      sh.part[1] = second ? run_c + c0 : run_c;
+      sh.part[2] = second ? run_w + v0 : run_w;
+    }
+    __syncthreads();
+    least = cross_key<true>(row, n, (int)sh.part[0], sh.part[1], sh.part[2], k, places, &total);
+  }
+  if (!COUNT || d.p < 1.f) {
+    if (COUNT) target = share_of(d.p, total);
+    if (total < target) return false;
+    if (run_w < target && run_w + v0 + v1 >= target) {
+      const bool second = run_w + v0 < target;
+      sh.part[0] = b0 + second;
+      sh.part[2] = second ? run_w + v0 : run_w;
+    }
+    __syncthreads();
+    const u64 key = cross_key<false>(row, n, (int)sh.part[0], 0, sh.part[2], target, places, &total);
+    least = key > least ? key : least;
+  }
+  // running sums in index order
+  const int i0 = kEach * (int)threadIdx.x;
+  u64 w[kEach], mine = 0, sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    w[e] = i0 + e < n && sh.sorted[i0 + e] >= least ? weight[i0 + e] : 0ull;
+    if (w[e] < d.floor_w) w[e] = 0;
+    mine += w[e];
+  }
+  u64 begin = block_scan(sh, mine, &sum) - mine;
+  const u64 goal = draw_target(d.uniform, sum);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (w[e] && begin <= goal && begin + w[e] > goal) sh.found[0] = sh.sorted[i0 + e];
+    begin += w[e];
+  }
+  __syncthreads();
+  return true;
+}
 
 // Cuts `kept` to its first k tokens (COUNT) or to the shortest prefix that holds a share p of its
-// weight, from the histogram that fill_histogram left in sh.hist[(turn - 1) & 1] behind a barrier
-// (`per_unit` bins per unit of best - x).  Where at most kSampleFinishMax tokens lie in the crossing
-// bin and above, rank 0 applies all filters to them, draws the token and leaves it in sh.found:
-// its key and kShrunkDone.  `z_sum`: in this CTA's sum of exponentials, out the row's.
+// weight, from the histogram that fill_histogram left in sh.hist[(turn - 1) & 1] behind a barrier.
 template <bool COUNT, int C>
-__device__ Shrunk shrink(RowSampler<C>& row, Kept& kept, float per_unit, const DrawArgs& d, float& z_sum) {
-  SampleShared& sh = row.sh;
+__device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d) {
+  SampleShared<C>& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const u64* hist = sh.hist[(row.turn - 1) & 1];
   constexpr int kPer = kSampleBins / kSampleThreads;  // bin 0 holds the largest values
@@ -453,11 +641,11 @@ __device__ Shrunk shrink(RowSampler<C>& row, Kept& kept, float per_unit, const D
       v1 += x.y;
     }
   }
-  if (threadIdx.x == 0) sh.crossing = sh.surviving = 0;
+  if (threadIdx.x == 0) sh.listed = 0;
   u64 all = 0;
   const u64 incl = block_scan(sh, v0 + v1, &all);
-  u64 target = COUNT ? (u64)d.k : share_of(d.p, all);
-  if (COUNT && target >= all) return kShrunkAll;  // nothing to leave out
+  const u64 target = COUNT ? (u64)d.k : share_of(d.p, all);
+  if (target > all) return;  // nothing to leave out (counts only)
   const u64 run = incl - v0 - v1;
   if (run < target && incl >= target) {
     const bool second = run + v0 < target;
@@ -467,77 +655,32 @@ __device__ Shrunk shrink(RowSampler<C>& row, Kept& kept, float per_unit, const D
   __syncthreads();
   const int bin = (int)sh.found[0];
   const u64 above = sh.found[1];
-  // ---- the tokens of the crossing bin, and with those above it
+  // ---- the tokens of the crossing bin
+  const uint32_t lowest = row.bin_floor(bin);
   for (int i = row.w0 + lane; i < row.w1; i += 32) {
     const uint32_t u = row.img[i];
-    if (u <= kImgNegInf) continue;
-    const float gap = row.best - image_value(u);
-    const int b = min(kSampleBins - 1, (int)(gap * per_unit));
-    if (gap < row.cut && b <= bin && kept.has(u, row.first + i)) {
-      const u64 key = ((u64)u << 32) | (uint32_t)~(uint32_t)(row.first + i);
-      const unsigned s = atomicAdd(&sh.surviving, 1u);
-      if (s < (unsigned)kSampleFinishMax) sh.survive[s] = key;
-      if (b == bin) {
-        const unsigned at = atomicAdd(&sh.crossing, 1u);
-        if (at < (unsigned)kSampleListMax) sh.cross[at] = key;
-      }
+    if (u >= lowest && row.bin_of(u) == bin && kept.has(u, row.first + i)) {
+      const unsigned at = atomicAdd(&sh.listed, 1u);
+      if (at < (unsigned)list_max(C)) sh.list[at] = ((u64)u << 32) | (uint32_t)~(uint32_t)(row.first + i);
     }
   }
   __syncthreads();
-  const u64(*box)[2] = row.exchange(((u64)sh.surviving << 32) | sh.crossing, __float_as_uint(z_sum));
-  unsigned n_survive = 0, n_cross = 0, survive[C], cross[C];
-  float z = 0.f;
+  const u64(*box)[2] = row.exchange(sh.listed, 0);
+  unsigned n = 0, count[C];
 #pragma unroll
-  for (int r = 0; r < C; ++r) {
-    survive[r] = (unsigned)(box[r][0] >> 32);
-    cross[r] = (unsigned)box[r][0];
-    n_survive += survive[r];
-    n_cross += cross[r];
-    z += __uint_as_float((uint32_t)box[r][1]);
-  }
-  z_sum = z;
-  if (n_survive <= (unsigned)kSampleFinishMax) {
-    if (row.rank != 0) return kShrunkDone;
-    const int padded = gather(row, sh.survive, survive, n_survive);
-    sort_descending(sh.sorted, padded);
-    const int i = (int)threadIdx.x;
-    const u64 key = i < (int)n_survive ? sh.sorted[i] : 0ull;
-    u64 w = key && (!COUNT || i < d.k) ? row.weight((uint32_t)(key >> 32)) : 0ull;
-    if (!COUNT || d.p < 1.f) {
-      u64 sum = 0;
-      const u64 to = block_scan(sh, w, &sum);
-      if (to - w >= (COUNT ? share_of(d.p, sum) : target)) w = 0;
-      __syncthreads();
-    }
-    if (w < d.floor_w) w = 0;
-    u64 total = 0;
-    block_scan(sh, w, &total);
-    // running sums in index order: the entry whose own weight crosses the target
-    if (i < kSampleFinishMax) sh.cross[i] = w;
-    __syncthreads();
-    u64 goal = d.uniform > 0.f ? (u64)((double)d.uniform * (double)total) : 0ull;
-    goal = goal >= total ? total - 1 : goal;
-    if (w) {
-      u64 to = 0;
-      for (int j = 0; j < (int)n_survive; ++j)
-        if ((uint32_t)sh.sorted[j] >= (uint32_t)key) to += sh.cross[j];  // the low word holds ~index
-      if (to > goal && to - w <= goal) sh.found[0] = key;
-    }
-    __syncthreads();
-    return kShrunkDone;
-  }
-  if (n_cross > (unsigned)kSampleListMax) {
+  for (int r = 0; r < C; ++r) n += count[r] = (unsigned)box[r][0];
+  if (n > (unsigned)list_max(C)) {
     const RadixResult res = shrink_radix<COUNT, C>(row, kept, target);
     kept = res.kept;
     row.turn = res.turn;
-    return kShrunk;
+    return;
   }
-  const int padded = gather(row, sh.cross, cross, n_cross);
+  const int padded = gather(row, sh.list, count, n);
   sort_descending(sh.sorted, padded);
   if (warp == 0) {  // the entry at which the running sum reaches the target
     u64 before = above;
-    for (int i0 = 0; i0 < (int)n_cross; i0 += 32) {
-      const u64 key = i0 + lane < (int)n_cross ? sh.sorted[i0 + lane] : 0ull;
+    for (int i0 = 0; i0 < (int)n; i0 += 32) {
+      const u64 key = i0 + lane < (int)n ? sh.sorted[i0 + lane] : 0ull;
       u64 s = key ? (COUNT ? 1ull : row.weight((uint32_t)(key >> 32))) : 0ull;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -555,54 +698,115 @@ __device__ Shrunk shrink(RowSampler<C>& row, Kept& kept, float per_unit, const D
   __syncthreads();
   kept.lo = (uint32_t)(sh.found[0] >> 32);
   kept.last = (int)~(uint32_t)sh.found[0];
-  return kShrunk;
 }
 
-// Bins of best - x over the row's kept tokens, of counts or weights, behind one cluster barrier.
-// SUM: on the way, this thread's part of sum exp(x - best) over the allowed tokens.
-template <bool COUNT, bool SUM, int C>
-__device__ float fill_histogram(RowSampler<C>& row, const Kept& kept, float per_unit) {
+// Histogram of the row's kept tokens, of counts or weights, behind a barrier.
+template <bool COUNT, int C>
+__device__ void fill_histogram(RowSampler<C>& row, const Kept& kept) {
   u64* hist = row.sh.hist[row.turn & 1];
   constexpr int kWords = kSampleBins * (COUNT ? 1 : 2);
+  __syncthreads();
   for (int b = threadIdx.x; b < kWords; b += kSampleThreads) reinterpret_cast<uint32_t*>(hist)[b] = 0;
   __syncthreads();
-  float z = 0.f;
-#pragma unroll 2
-  for (int i = row.w0 + (int)(threadIdx.x & 31); i < row.w1; i += 32) {
-    const uint32_t u = row.img[i];
-    if (u <= kImgNegInf) continue;
-    const float gap = row.best - image_value(u);
-    if (SUM) z += __expf(-gap);
-    if (!(gap < row.cut) || !kept.has(u, row.first + i)) continue;
-    uint32_t* bin = reinterpret_cast<uint32_t*>(hist) + min(kSampleBins - 1, (int)(gap * per_unit)) * (COUNT ? 1 : 2);
-    if (COUNT) {
-      atomicAdd(bin, 1u);
-    } else {  // 64-bit sum from 32-bit atomics: exactly the add that wraps the low word carries
-      const u64 w = row.weight(u);
-      const uint32_t low = (uint32_t)w, old = atomicAdd(bin, low);
-      const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
-      if (high) atomicAdd(bin + 1, high);
+  for (int i = row.w0 + (int)(threadIdx.x & 31); i < row.w1; i += 128) {
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = i + 32 * e < row.w1 ? row.img[i + 32 * e] : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (u[e] <= kImgNegInf || !kept.has(u[e], row.first + i + 32 * e)) continue;
+      uint32_t* bin = reinterpret_cast<uint32_t*>(hist) + row.bin_of(u[e]) * (COUNT ? 1 : 2);
+      if (COUNT) {
+        atomicAdd(bin, 1u);
+      } else {  // 64-bit sum from 32-bit atomics: exactly the add that wraps the low word carries
+        const u64 w = row.weight(u[e]);
+        const uint32_t low = (uint32_t)w, old = atomicAdd(bin, low);
+        const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
+        if (high) atomicAdd(bin + 1, high);
+      }
     }
   }
-  return z;
+  ++row.turn;
+  row.barrier();
 }
 
-// This CTA's sum of the threads' parts, in a fixed order.
-__device__ __forceinline__ float block_sum_f32(SampleShared& sh, float z) {
-  z = warp_sum(z);
-  if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = __float_as_uint(z);
+// A bound below the row's k-th largest value from what each lane holds at most: where k lanes reach a
+// bin, so do k tokens.  The lowest drawable value if fewer lanes hold any.
+template <int C>
+__device__ uint32_t sieve(RowSampler<C>& row, uint32_t lane_top, uint32_t bottom, int k) {
+  SampleShared<C>& sh = row.sh;
+  uint32_t* hist = reinterpret_cast<uint32_t*>(sh.hist[row.turn & 1]);
+  ++row.turn;
+  hist[threadIdx.x] = hist[threadIdx.x + kSampleThreads] = 0;
+  static_assert(kSampleBins == 2 * kSampleThreads, "two bins a thread");
+  if (threadIdx.x == 0) sh.found[0] = kSampleBins;
   __syncthreads();
-  z = 0.f;
+  if (lane_top > kImgNegInf) atomicAdd(hist + row.bin_of(lane_top), 1u);
+  row.barrier();
+  uint32_t v0 = 0, v1 = 0;
 #pragma unroll
-  for (int w = 0; w < kSampleWarps; ++w) z += __uint_as_float((uint32_t)sh.part[w]);
-  return z;
+  for (int r = 0; r < C; ++r) {
+    const uint2 x = reinterpret_cast<const uint2*>(row.peer(hist, r))[threadIdx.x];
+    v0 += x.x;
+    v1 += x.y;
+  }
+  u64 all = 0;
+  const u64 incl = block_scan(sh, (u64)(v0 + v1), &all), run = incl - v0 - v1;
+  if (run < (u64)k && incl >= (u64)k) sh.found[0] = 2 * threadIdx.x + (run + v0 < (u64)k);
+  __syncthreads();
+  const int bin = (int)sh.found[0];
+  if (bin >= kSampleBins) return bottom;
+  // the bin's lower edge, or a little below it: more than the roundings of bin_of, 2^-23 each of the
+  // gap, of its product and of the edge
+  const float gap = (float)(bin + 1) / row.per_unit, edge = row.best - gap * 1.000001f;
+  return max(value_image(edge - (fabsf(edge) + fabsf(row.best)) * 1e-6f), bottom);
+}
+
+// The CTA's tokens from image `lowest` on into sh.list, in index order; how many, or more than
+// list_max(C) where they do not fit.  WEIGH: `sum` receives the CTA's weight sum over all tokens.
+template <bool WEIGH, int C>
+__device__ unsigned collect(RowSampler<C>& row, uint32_t lowest, u64& sum) {
+  SampleShared<C>& sh = row.sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned count = 0;
+  u64 weight = 0;
+#pragma unroll 4
+  for (int i = row.w0 + lane; i < row.w1; i += 32) {
+    const uint32_t u = row.img[i];
+    count += u >= lowest;
+    if (WEIGH) weight += row.weight(u);
+  }
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (lane == 0) sh.counts[warp] = count;
+  if (WEIGH)
+    sum = row.block_sum(weight);
+  else
+    __syncthreads();
+  const unsigned c = lane < kSampleWarps ? sh.counts[lane] : 0u;
+  unsigned from = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0u);
+  const unsigned all = __reduce_add_sync(0xffffffffu, c);
+  if (all > (unsigned)list_max(C)) return list_max(C) + 1;
+  for (int i0 = row.w0; count && i0 < row.w1; i0 += 128) {
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = i0 + lane + 32 * e < row.w1 ? row.img[i0 + lane + 32 * e] : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned in = __ballot_sync(0xffffffffu, u[e] >= lowest);
+      if (in >> lane & 1)
+        sh.list[from + __popc(in & ((1u << lane) - 1))] =
+            ((u64)u[e] << 32) | (uint32_t)~(uint32_t)(row.first + i0 + lane + 32 * e);
+      from += __popc(in);
+    }
+  }
+  return all;  // (published by the exchange's barrier)
 }
 
 template <int C>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char sample_smem[];
-  SampleShared& sh = *reinterpret_cast<SampleShared*>(sample_smem);
-  uint32_t* img = reinterpret_cast<uint32_t*>(sample_smem + sizeof(SampleShared));
+  SampleShared<C>& sh = *reinterpret_cast<SampleShared<C>*>(sample_smem);
+  uint32_t* img = reinterpret_cast<uint32_t*>(sample_smem + sizeof(SampleShared<C>));
   const int rank = (int)(blockIdx.x % C), r = (int)(blockIdx.x / C);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = min(a.vocab, rank * a.chunk), n = min(a.vocab - first, a.chunk);
@@ -610,32 +814,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const int w0 = min(n, warp * per_warp), w1 = min(n, w0 + per_warp);
   if (threadIdx.x < 64) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
   pdl_wait();
-
-  // ---- images of the allowed tokens; the largest and the lowest drawable value
-  uint32_t top = 0, bottom = 0xffffffffu;
-  if (a.dtype == S2R_F32)
-    load_images<float>(a, r, first, img, w0, w1, top, bottom);
-  else if (a.dtype == S2R_BF16)
-    load_images<bf16>(a, r, first, img, w0, w1, top, bottom);
-  else
-    load_images<__half>(a, r, first, img, w0, w1, top, bottom);
   const float t = a.temperature ? a.temperature[r] : a.temperature_all;
+  const double inv_t = 1.4426950408889634 / (double)t;  // (a long chain: under the loads)
+  // ---- images of the allowed tokens; the largest and the lowest drawable value
+  LaneStats st;
+  if (a.dtype == S2R_F32)
+    load_images<float>(a, r, first, img, w0, w1, st);
+  else if (a.dtype == S2R_BF16)
+    load_images<bf16>(a, r, first, img, w0, w1, st);
+  else
+    load_images<__half>(a, r, first, img, w0, w1, st);
   DrawArgs d;
   d.k = a.top_k ? a.top_k[r] : a.top_k_all;
   d.p = a.top_p ? a.top_p[r] : a.top_p_all;
   d.uniform = a.uniforms[r];
   const float m = a.min_p ? a.min_p[r] : a.min_p_all;
   RowSampler<C> row{sh, img, first, rank, w0, w1};
+  uint32_t top = __reduce_max_sync(0xffffffffu, st.top), bottom = __reduce_min_sync(0xffffffffu, st.bottom);
   {
-    top = __reduce_max_sync(0xffffffffu, top);
-    bottom = __reduce_min_sync(0xffffffffu, bottom);
     if (lane == 0) sh.part[warp] = ((u64)top << 32) | bottom;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) {
-      top = max(top, (uint32_t)(sh.part[w] >> 32));
-      bottom = min(bottom, (uint32_t)sh.part[w]);
-    }
+    const u64 x = sh.part[lane & (kSampleWarps - 1)];
+    top = __reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32));
+    bottom = __reduce_min_sync(0xffffffffu, (uint32_t)x);
     const u64(*box)[2] = row.exchange(((u64)top << 32) | bottom, 0);
 #pragma unroll
     for (int p = 0; p < C; ++p) {
@@ -645,27 +846,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   }
   const bool finite = top > kImgNegInf && top < kImgPosInf;
   row.best = finite ? image_value(top) : 0.f;
-  row.inv_t = 1.4426950408889634 / (double)t;
+  row.inv_t = inv_t;
   row.scale_bits = a.scale_bits;
-  row.cut = a.cut * t;
   const bool greedy = !finite || !(t > 0.f);
   d.floor_w = m > 0.f ? (u64)ceil((double)fminf(m, 1.f) * (double)(1ull << a.scale_bits)) : 0ull;
-  float z = 0.f;
+  // this CTA's sum of exp(x - best) over the allowed tokens
+  bool summed = false;  // z is the row's
+  float z = block_sum_f32(sh, finite && st.m != -INFINITY ? st.z * __expf(st.m - row.best) : 0.f);
 
   if (greedy) {
     uint32_t lowest = 0xffffffffu;
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const uint32_t u = img[i];
-      if (u == top) lowest = min(lowest, (uint32_t)(first + i));
-      if (finite && u > kImgNegInf) z += __expf(image_value(u) - row.best);
-    }
-    __syncthreads();
-    z = block_sum_f32(sh, z);
+    for (int i = w0 + lane; i < w1; i += 32)
+      if (img[i] == top) lowest = min(lowest, (uint32_t)(first + i));
     lowest = __reduce_min_sync(0xffffffffu, lowest);
     if (lane == 0) sh.scan[warp] = lowest;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSampleWarps; ++w) lowest = min(lowest, (uint32_t)sh.scan[w]);
+    lowest = __reduce_min_sync(0xffffffffu, (uint32_t)sh.scan[lane & (kSampleWarps - 1)]);
     const u64(*box)[2] = row.exchange(lowest, __float_as_uint(z));
     z = 0.f;
 #pragma unroll
@@ -684,48 +880,50 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     return;  // (nothing reads a peer's memory: what was sent landed before the barrier)
   }
 
-  // ---- the filters; the sum of exp(x - best) on the way of the first pass
-  Kept kept;
-  const float span = row.best - image_value(bottom);
-  float per_unit = fminf((float)kSampleBins / fminf(row.cut, span), 3e38f);
+  // ---- the filters
   const bool by_count = d.k > 0 && d.k < a.vocab, by_share = d.p < 1.f;
-  Shrunk done = kShrunkAll;
-  bool summed = false;  // z is the row's sum
-  if (by_count) {
-    z = fill_histogram<true, true>(row, kept, per_unit);
-    z = block_sum_f32(sh, z);
-    ++row.turn;
-    row.barrier();
-    done = shrink<true>(row, kept, per_unit, d, z);
-    summed = done != kShrunkAll;
-    if (done == kShrunk) {
-      const float left = row.best - image_value(kept.lo);
-      per_unit = fminf((float)kSampleBins / left, 3e38f);
+  // tokens a.cut temperatures below the best weigh nothing
+  row.per_unit = fminf((float)kSampleBins / fminf(a.cut * t, row.best - image_value(bottom)), 3e38f);
+  if (by_count || by_share) {
+    const uint32_t lowest = sieve(row, st.top, bottom, by_count ? d.k : kSampleNucleus);
+    u64 sum = 0;
+    const unsigned mine = by_count ? collect<false>(row, lowest, sum) : collect<true>(row, lowest, sum);
+    const u64(*box)[2] = row.exchange(sum, ((u64)mine << 32) | __float_as_uint(z));
+    unsigned total = 0, count[C];
+    sum = 0;
+    z = 0.f;
+#pragma unroll
+    for (int p = 0; p < C; ++p) {
+      sum += box[p][0];
+      total += count[p] = (unsigned)(box[p][1] >> 32);
+      z += __uint_as_float((uint32_t)box[p][1]);
     }
-  }
-  if (by_share && done != kShrunkDone) {
-    if (by_count) {
-      __syncthreads();
-      fill_histogram<false, false>(row, kept, per_unit);
-    } else {
-      z = fill_histogram<false, true>(row, kept, per_unit);
-      z = block_sum_f32(sh, z);
-    }
-    ++row.turn;
-    row.barrier();
-    float sum = summed ? 0.f : z;
-    done = shrink<false>(row, kept, per_unit, d, sum);
-    if (!summed) z = sum;
     summed = true;
-  }
-  if (done == kShrunkDone) {
-    if (rank == 0 && threadIdx.x == 0) {
-      const u64 key = sh.found[0];
-      a.tokens[r] = (int64_t)~(uint32_t)key;
-      if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
+    if (total <= (unsigned)list_max(C)) {
+      bool found = false;
+      if (rank == 0) {
+        gather(row, sh.list, count, total);
+        found = by_count ? finish<true, C>(row, (int)total, lowest, 0, d)
+                         : finish<false, C>(row, (int)total, lowest, share_of(d.p, sum), d);
+        if (found && threadIdx.x == 0) {
+          const u64 key = sh.found[0];
+          a.tokens[r] = (int64_t)~(uint32_t)key;
+          if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
+        }
+      }
+      if (row.exchange(found, 0)[0][0]) return;  // (rank 0's answer; it has read the peers' lists)
     }
-    row.barrier();  // rank 0 has read the peers' lists
-    return;
+  }
+  Kept kept;
+  if (by_count) {
+    fill_histogram<true>(row, kept);
+    shrink<true>(row, kept, d);
+    if (kept.lo > kImgNegInf)
+      row.per_unit = fminf((float)kSampleBins / (row.best - image_value(kept.lo)), 3e38f);
+  }
+  if (by_share) {
+    fill_histogram<false>(row, kept);
+    shrink<false>(row, kept, d);
   }
 
   // ---- the token: running sums in index order
@@ -735,20 +933,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     return w >= d.floor_w ? w : 0ull;
   };
   u64 sum = 0, before = 0;
-  const bool add_z = !by_count && !by_share;
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t u = img[i];
-    if (add_z && u > kImgNegInf) z += __expf(image_value(u) - row.best);
-    sum += kept_weight(i, u);
-  }
-  __syncthreads();
-  if (add_z) z = block_sum_f32(sh, z);
+#pragma unroll 2
+  for (int i = w0 + lane; i < w1; i += 32) sum += kept_weight(i, img[i]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const u64 mine = sum;
   const u64 block = row.block_sum(lane == 0 ? mine : 0ull);
-  u64 run = 0;
-  for (int w = 0; w < warp; ++w) run += sh.part[w];
+  u64 run = sum_partials((lane & (kSampleWarps - 1)) < warp ? sh.part[lane & (kSampleWarps - 1)] : 0ull);
   u64 total = 0;
   {
     const u64(*box)[2] = row.exchange(block, __float_as_uint(z));
@@ -762,8 +953,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     if (!summed) z = sum_z;
   }
   run += before;
-  u64 target = d.uniform > 0.f ? (u64)((double)d.uniform * (double)total) : 0ull;
-  target = target >= total ? total - 1 : target;
+  const u64 target = draw_target(d.uniform, total);
   if (run <= target && target < run + mine) {
     for (int i0 = w0; i0 < w1; i0 += 32) {
       const int i = i0 + lane;
@@ -787,7 +977,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   }
 }
 
-static_assert(sizeof(SampleShared) % 16 == 0, "images start 16-byte aligned");
+static_assert(sizeof(SampleShared<1>) % 16 == 0 && sizeof(SampleShared<4>) % 16 == 0, "images start 16-byte aligned");
 
 constexpr int kSampleMaxChunk = 40960;  // tokens of one CTA: 160 KB of images
 
@@ -803,16 +993,21 @@ SampleFn sample_fn(int splits) {
   }
 }
 
+size_t shared_bytes(int splits) {
+  return splits == 1 ? sizeof(SampleShared<1>) : splits == 2 ? sizeof(SampleShared<2>) : sizeof(SampleShared<4>);
+}
+
 int sample_chunk(int vocab, int splits) {  // a multiple of 32 tokens a warp
   const int per = (vocab + splits - 1) / splits;
   return (per + kSampleWarps * 32 - 1) / (kSampleWarps * 32) * (kSampleWarps * 32);
 }
 
-// CTAs per row: enough that a CTA's share fits its shared memory, then more while the rows leave
-// SMs idle (two CTAs fit one) and a share is worth splitting.
+// CTAs per row: enough that two of them fit an SM (1,024 rows of 32,576 tokens: one CTA a row takes 181 us,
+// two 146 us, four 240 us, more of it in barriers), then more while the rows leave SMs idle and a
+// share is worth splitting.
 int sample_splits(int rows, int vocab, int sms) {
   int c = 1;
-  while (c < kSampleMaxSplits && sample_chunk(vocab, c) > kSampleMaxChunk) c *= 2;
+  while (c < kSampleMaxSplits && shared_bytes(c) + sample_chunk(vocab, c) * sizeof(uint32_t) > 112 * 1024) c *= 2;
   while (c < 8 && (long long)rows * c * 2 <= 2 * sms && vocab / (2 * c) >= 2048) c *= 2;
   return c;
 }
@@ -833,7 +1028,7 @@ const SampleDevice& sample_device(int device) {
   if (ready[device].load(std::memory_order_relaxed)) return dev;
   dev.error = cudaDeviceGetAttribute(&dev.sms, cudaDevAttrMultiProcessorCount, device);
   for (int c = 1; c <= kSampleMaxSplits && dev.error == cudaSuccess; c *= 2) {
-    const int smem = (int)(sizeof(SampleShared) + kSampleMaxChunk * sizeof(uint32_t));
+    const int smem = (int)(shared_bytes(c) + kSampleMaxChunk * sizeof(uint32_t));
     dev.error = cudaFuncSetAttribute(sample_fn(c), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (dev.error == cudaSuccess && c > 8)
       dev.error = cudaFuncSetAttribute(sample_fn(c), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -863,7 +1058,7 @@ int launch_sample(SampleArgs a, cudaStream_t stream, const char** why) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * splits);
   cfg.blockDim = dim3(kSampleThreads);
-  cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)a.chunk * sizeof(uint32_t);
+  cfg.dynamicSmemBytes = shared_bytes(splits) + (size_t)a.chunk * sizeof(uint32_t);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;

@@ -111,6 +111,23 @@ def test_draws_match_the_definition(rows, vocab, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,vocab", [(1, 32576), (150, 9000), (300, 32576), (3, 131071)])
+@pytest.mark.parametrize("t,k,p,m", [(1.0, 700, 1.0, 0.0), (1.5, 1500, 0.9, 0.0), (2.0, 5000, 1.0, 0.001), (3.0, 8999, 0.99, 0.0),
+                                     (5.0, 0, 0.97, 0.0), (0.01, 300, 0.9, 0.0), (1e9, 0, 0.5, 0.0), (1e-30, 40, 0.5, 0.1)])
+def test_filters_that_keep_many_tokens_and_extreme_temperatures(rows, vocab, t, k, p, m):
+    """Past the lists' sizes: the searches over the whole row take over."""
+
+    for masked in (False, True):
+        logits, u, bias, allowed = inputs(rows, vocab, torch.float32, k + vocab, masked=masked)
+        if masked:  # whole spans, as a grammar's classes: some CTAs' shares hold nothing
+            span = torch.arange(vocab) * 9 // vocab
+            allowed = allowed & (torch.rand(rows, 9, generator=torch.Generator().manual_seed(k)) < 0.4)[:, span]
+        check(logits, u, bias, allowed, t, k, p, m)
+    coarse, u, _, _ = inputs(rows, vocab, torch.float32, k, masked=False)
+    check(torch.round(coarse), u, None, None, t, k, p, m)  # a dozen values: thousands of ties at any threshold
+
+
+@gpu
 @pytest.mark.parametrize("vocab", [131071, 524288])
 def test_large_vocabularies(vocab):
     for i, (t, k, p, m) in enumerate(FILTERS[:5]):
