@@ -16,14 +16,13 @@
 // threshold, and the first few of the threshold's ties".  Most draws keep few
 // tokens, and those are found by a sieve: where k lanes hold a value of at least
 // L, so do k tokens, so the k-th largest of what each lane holds at most bounds
-// the k-th largest token from below, and little more than k tokens pass it.  Up
-// to 2048 of them are gathered and finished by one CTA.  Top-p alone tries the
-// same with the bound of 128 lanes: a decoder's nucleus is a few tokens.  Where
-// the sieve passes too many, or too little weight, the threshold is searched
-// among all: a histogram of counts (top-k) or weights (top-p) over 1024 bins
-// linear in M - x, then the tokens of the bin in which the sum crosses its
-// target, gathered and sorted; and when that bin holds too many (masses of equal
-// values), radix rounds over the images.
+// the k-th largest token from below, and little more than k tokens pass it.
+// Top-p alone starts from a histogram of the weights over 1024 bins linear in
+// M - x: the bin in which the sum crosses its share bounds what is kept.  Up to
+// 2048 tokens from the bound on are gathered and finished by one CTA.  Where
+// there are more, the threshold is searched among all: a histogram of counts or
+// weights, then the tokens of the crossing bin, gathered and sorted; and when
+// that bin holds too many (masses of equal values), radix rounds over the images.
 //
 // Weights are fixed-point integers, rint(exp(.) * 2^(61 - bits(vocab))), with
 // the exponential in 64 bits: which token is drawn depends on which side of a
@@ -60,7 +59,6 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 1024;  // of either histogram
 constexpr int kSampleBinBits = 10;
 constexpr int kSampleMaxSplits = 16;
-constexpr int kSampleNucleus = 128;   // lanes whose bound the sieve takes for top-p alone
 constexpr uint32_t kImgNegInf = 0x007fffffu;  // image of -inf: tokens at or below it are never drawn
 constexpr uint32_t kImgPosInf = 0xff800000u;
 
@@ -540,11 +538,10 @@ __device__ u64 cross_key(RowSampler<C>& row, int n, int bin, u64 above, u64 abov
 }
 
 // All filters and the draw on the n gathered tokens of sh.sorted, in index order (rank 0's CTA alone).  They
-// hold the k largest (COUNT), or are all there are above some value: then the prefix that reaches
-// `target` is kept, if they reach it; else the answer is false.  Leaves the drawn token's key in
-// sh.found[0].  The thresholds come from one histogram of the gathered tokens, counts and weights.
+// hold the k largest (COUNT), or all that the prefix which reaches `target` takes.  Leaves the drawn
+// token's key in sh.found[0].  The thresholds come from one histogram of the gathered tokens, counts and weights.
 template <bool COUNT, int C>
-__device__ __noinline__ bool finish(RowSampler<C> row, int n, uint32_t lowest, u64 target, const DrawArgs& d) {
+__device__ __noinline__ void finish(RowSampler<C> row, int n, uint32_t lowest, u64 target, const DrawArgs& d) {
   SampleShared<C>& sh = row.sh;
   constexpr int kEach = list_max(C) / kSampleThreads;
   // the histograms' memory is free here: counts, low and high words of the weights, places of a bin's tokens
@@ -588,7 +585,6 @@ __device__ __noinline__ bool finish(RowSampler<C> row, int n, uint32_t lowest, u
   }
   if (!COUNT || d.p < 1.f) {
     if (COUNT) target = share_of(d.p, total);
-    if (total < target) return false;
     if (run_w < target && run_w + v0 + v1 >= target) {
       const bool second = run_w + v0 < target;
       sh.part[0] = b0 + second;
@@ -615,13 +611,76 @@ __device__ __noinline__ bool finish(RowSampler<C> row, int n, uint32_t lowest, u
     begin += w[e];
   }
   __syncthreads();
+}
+
+// The CTA's tokens from image `lowest` on into sh.list, in index order; how many, or more than
+// list_max(C) where they do not fit.
+template <int C>
+__device__ unsigned collect(RowSampler<C>& row, uint32_t lowest) {
+  SampleShared<C>& sh = row.sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned count = 0;
+#pragma unroll 4
+  for (int i = row.w0 + lane; i < row.w1; i += 32) {
+    count += row.img[i] >= lowest;
+  }
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (lane == 0) sh.counts[warp] = count;
+  __syncthreads();
+  const unsigned c = lane < kSampleWarps ? sh.counts[lane] : 0u;
+  unsigned from = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0u);
+  const unsigned all = __reduce_add_sync(0xffffffffu, c);
+  if (all > (unsigned)list_max(C)) return list_max(C) + 1;
+  for (int i0 = row.w0; count && i0 < row.w1; i0 += 128) {
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = i0 + lane + 32 * e < row.w1 ? row.img[i0 + lane + 32 * e] : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned in = __ballot_sync(0xffffffffu, u[e] >= lowest);
+      if (in >> lane & 1)
+        sh.list[from + __popc(in & ((1u << lane) - 1))] =
+            ((u64)u[e] << 32) | (uint32_t)~(uint32_t)(row.first + i0 + lane + 32 * e);
+      from += __popc(in);
+    }
+  }
+  return all;  // (published by the exchange's barrier)
+}
+
+// Gather the tokens from image `lowest` on, if they fit, and have rank 0 apply the filters to them and
+// draw (finish's COUNT and target).  z: in this CTA's sum of exponentials, out the row's.
+template <bool COUNT, int C>
+__device__ bool try_finish(RowSampler<C>& row, const SampleArgs& a, int r, uint32_t lowest, u64 target, const DrawArgs& d,
+                           float& z) {
+  SampleShared<C>& sh = row.sh;
+  const unsigned mine = collect(row, lowest);
+  const u64(*box)[2] = row.exchange(mine, __float_as_uint(z));
+  unsigned total = 0, count[C];
+  z = 0.f;
+#pragma unroll
+  for (int p = 0; p < C; ++p) {
+    total += count[p] = (unsigned)box[p][0];
+    z += __uint_as_float((uint32_t)box[p][1]);
+  }
+  if (total > (unsigned)list_max(C)) return false;
+  if (row.rank == 0) {
+    gather(row, sh.list, count, total);
+    finish<COUNT, C>(row, (int)total, lowest, target, d);
+    if (threadIdx.x == 0) {
+      const u64 key = sh.found[0];
+      a.tokens[r] = (int64_t)~(uint32_t)key;
+      if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
+    }
+  }
+  row.barrier();  // rank 0 has read the peers' lists
   return true;
 }
 
 // Cuts `kept` to its first k tokens (COUNT) or to the shortest prefix that holds a share p of its
 // weight, from the histogram that fill_histogram left in sh.hist[(turn - 1) & 1] behind a barrier.
-template <bool COUNT, int C>
-__device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d) {
+// FINISH (weights, nothing cut yet): tries to finish the row on the way; true if it did.
+template <bool COUNT, bool FINISH, int C>
+__device__ bool shrink(RowSampler<C>& row, Kept& kept, const SampleArgs& a, int r, const DrawArgs& d, float& z) {
   SampleShared<C>& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const u64* hist = sh.hist[(row.turn - 1) & 1];
@@ -645,7 +704,7 @@ __device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d) {
   u64 all = 0;
   const u64 incl = block_scan(sh, v0 + v1, &all);
   const u64 target = COUNT ? (u64)d.k : share_of(d.p, all);
-  if (target > all) return;  // nothing to leave out (counts only)
+  if (target > all) return false;  // nothing to leave out (counts only)
   const u64 run = incl - v0 - v1;
   if (run < target && incl >= target) {
     const bool second = run + v0 < target;
@@ -655,8 +714,13 @@ __device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d) {
   __syncthreads();
   const int bin = (int)sh.found[0];
   const u64 above = sh.found[1];
-  // ---- the tokens of the crossing bin
   const uint32_t lowest = row.bin_floor(bin);
+  if (FINISH) {
+    if (try_finish<false>(row, a, r, lowest, target, d, z)) return true;
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+  }
+  // ---- the tokens of the crossing bin
   for (int i = row.w0 + lane; i < row.w1; i += 32) {
     const uint32_t u = row.img[i];
     if (u >= lowest && row.bin_of(u) == bin && kept.has(u, row.first + i)) {
@@ -673,7 +737,7 @@ __device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d) {
     const RadixResult res = shrink_radix<COUNT, C>(row, kept, target);
     kept = res.kept;
     row.turn = res.turn;
-    return;
+    return false;
   }
   const int padded = gather(row, sh.list, count, n);
   sort_descending(sh.sorted, padded);
@@ -698,6 +762,7 @@ __device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d) {
   __syncthreads();
   kept.lo = (uint32_t)(sh.found[0] >> 32);
   kept.last = (int)~(uint32_t)sh.found[0];
+  return false;
 }
 
 // Histogram of the row's kept tokens, of counts or weights, behind a barrier.
@@ -762,46 +827,6 @@ __device__ uint32_t sieve(RowSampler<C>& row, uint32_t lane_top, uint32_t bottom
   return max(value_image(edge - (fabsf(edge) + fabsf(row.best)) * 1e-6f), bottom);
 }
 
-// The CTA's tokens from image `lowest` on into sh.list, in index order; how many, or more than
-// list_max(C) where they do not fit.  WEIGH: `sum` receives the CTA's weight sum over all tokens.
-template <bool WEIGH, int C>
-__device__ unsigned collect(RowSampler<C>& row, uint32_t lowest, u64& sum) {
-  SampleShared<C>& sh = row.sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned count = 0;
-  u64 weight = 0;
-#pragma unroll 4
-  for (int i = row.w0 + lane; i < row.w1; i += 32) {
-    const uint32_t u = row.img[i];
-    count += u >= lowest;
-    if (WEIGH) weight += row.weight(u);
-  }
-  count = __reduce_add_sync(0xffffffffu, count);
-  if (lane == 0) sh.counts[warp] = count;
-  if (WEIGH)
-    sum = row.block_sum(weight);
-  else
-    __syncthreads();
-  const unsigned c = lane < kSampleWarps ? sh.counts[lane] : 0u;
-  unsigned from = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0u);
-  const unsigned all = __reduce_add_sync(0xffffffffu, c);
-  if (all > (unsigned)list_max(C)) return list_max(C) + 1;
-  for (int i0 = row.w0; count && i0 < row.w1; i0 += 128) {
-    uint32_t u[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = i0 + lane + 32 * e < row.w1 ? row.img[i0 + lane + 32 * e] : 0u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned in = __ballot_sync(0xffffffffu, u[e] >= lowest);
-      if (in >> lane & 1)
-        sh.list[from + __popc(in & ((1u << lane) - 1))] =
-            ((u64)u[e] << 32) | (uint32_t)~(uint32_t)(row.first + i0 + lane + 32 * e);
-      from += __popc(in);
-    }
-  }
-  return all;  // (published by the exchange's barrier)
-}
-
 template <int C>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char sample_smem[];
@@ -851,7 +876,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const bool greedy = !finite || !(t > 0.f);
   d.floor_w = m > 0.f ? (u64)ceil((double)fminf(m, 1.f) * (double)(1ull << a.scale_bits)) : 0ull;
   // this CTA's sum of exp(x - best) over the allowed tokens
-  bool summed = false;  // z is the row's
   float z = block_sum_f32(sh, finite && st.m != -INFINITY ? st.z * __expf(st.m - row.best) : 0.f);
 
   if (greedy) {
@@ -884,47 +908,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const bool by_count = d.k > 0 && d.k < a.vocab, by_share = d.p < 1.f;
   // tokens a.cut temperatures below the best weigh nothing
   row.per_unit = fminf((float)kSampleBins / fminf(a.cut * t, row.best - image_value(bottom)), 3e38f);
-  if (by_count || by_share) {
-    const uint32_t lowest = sieve(row, st.top, bottom, by_count ? d.k : kSampleNucleus);
-    u64 sum = 0;
-    const unsigned mine = by_count ? collect<false>(row, lowest, sum) : collect<true>(row, lowest, sum);
-    const u64(*box)[2] = row.exchange(sum, ((u64)mine << 32) | __float_as_uint(z));
-    unsigned total = 0, count[C];
-    sum = 0;
-    z = 0.f;
-#pragma unroll
-    for (int p = 0; p < C; ++p) {
-      sum += box[p][0];
-      total += count[p] = (unsigned)(box[p][1] >> 32);
-      z += __uint_as_float((uint32_t)box[p][1]);
-    }
-    summed = true;
-    if (total <= (unsigned)list_max(C)) {
-      bool found = false;
-      if (rank == 0) {
-        gather(row, sh.list, count, total);
-        found = by_count ? finish<true, C>(row, (int)total, lowest, 0, d)
-                         : finish<false, C>(row, (int)total, lowest, share_of(d.p, sum), d);
-        if (found && threadIdx.x == 0) {
-          const u64 key = sh.found[0];
-          a.tokens[r] = (int64_t)~(uint32_t)key;
-          if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
-        }
-      }
-      if (row.exchange(found, 0)[0][0]) return;  // (rank 0's answer; it has read the peers' lists)
-    }
-  }
   Kept kept;
   if (by_count) {
+    if (try_finish<true>(row, a, r, sieve(row, st.top, bottom, d.k), 0, d, z)) return;
     fill_histogram<true>(row, kept);
-    shrink<true>(row, kept, d);
+    shrink<true, false>(row, kept, a, r, d, z);
     if (kept.lo > kImgNegInf)
       row.per_unit = fminf((float)kSampleBins / (row.best - image_value(kept.lo)), 3e38f);
   }
   if (by_share) {
     fill_histogram<false>(row, kept);
-    shrink<false>(row, kept, d);
+    if (by_count)
+      shrink<false, false>(row, kept, a, r, d, z);
+    else if (shrink<false, true>(row, kept, a, r, d, z))
+      return;
   }
+  const bool summed = by_count || by_share;  // z is the row's
 
   // ---- the token: running sums in index order
   auto kept_weight = [&](int i, uint32_t u) -> u64 {
