@@ -361,8 +361,22 @@ __device__ __forceinline__ void store_out(const SharedAttnArgs& a, int r, int h,
                                           float top, bool first) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key at all: 0
   T* dst = static_cast<T*>(a.out) + r * a.out_row + h * a.out_head + d;
+  if (a.out_vector) {
+    if constexpr (N >= 8) {
 #pragma unroll
-  for (int e = 0; e < N; ++e) dst[e] = T(o[e] * inv);
+      for (int e = 0; e < N; e += 8)
+        *reinterpret_cast<uint4*>(dst + e) =
+            make_uint4(pack_pair(T(), o[e] * inv, o[e + 1] * inv), pack_pair(T(), o[e + 2] * inv, o[e + 3] * inv),
+                       pack_pair(T(), o[e + 4] * inv, o[e + 5] * inv), pack_pair(T(), o[e + 6] * inv, o[e + 7] * inv));
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e += 2)
+        *reinterpret_cast<uint32_t*>(dst + e) = pack_pair(T(), o[e] * inv, o[e + 1] * inv);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) dst[e] = T(o[e] * inv);
+  }
   if (a.lse && first) a.lse[(size_t)r * a.heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
@@ -1027,6 +1041,7 @@ cudaError_t launch_all(const SharedAttnArgs& a, cudaStream_t s) {
 size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
   const size_t pairs = (size_t)a.rows * a.heads;
   a.shared_splits = a.own_splits = 0;
+  a.out_vector = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_row % 8 == 0 && a.out_head % 8 == 0;
   if (a.shared_tokens > 0) {
     const int tiles = query_tiles(a), keys = (a.shared_tokens + KT - 1) / KT;
     a.pair = tiles > 1;

@@ -38,6 +38,7 @@ struct SharedAttnArgs {
   // set by plan_shared_attn
   int shared_splits, own_splits;  // parts of a (row, head)'s keys
   bool pair;                      // two query tiles a CTA
+  bool out_vector;                // out can be written 16 bytes at a time
   bool pdl;                       // the first launch may start while the kernel before it drains (it waits itself)
 };
 
