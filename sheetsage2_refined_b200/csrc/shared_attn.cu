@@ -53,8 +53,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kOwnThreads = 32;
 constexpr int kOwnWarps = kOwnThreads / 32;
 constexpr int kOwnStages = 2;
-constexpr int kOwnStage = 16384;  // bytes of a chunk, K then V
 constexpr int kOwnPiece = 16;     // tokens of a box of a row's last chunk
+constexpr int kOwnStage = 16384;  // bytes of a chunk, K then V (8 KB: rows of up to 200 tokens 3% faster, 1,500 10% slower)
 constexpr int kOwnSmem = kOwnWarps * kOwnStages * kOwnStage + 1024;  // + alignment slack
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -97,7 +97,24 @@ __global__ void __launch_bounds__(kOwnThreads)
   unsigned char* ring = base + warp * kOwnStages * kOwnStage;
   const int group = a.heads / a.kv_heads, sets = (group + kQueries - 1) / kQueries, splits = a.own_splits;
   const int per_row = a.kv_heads * sets * splits;
-  const int units = a.rows * per_row, stride = gridDim.x * kOwnWarps;  // (rows x heads <= 2^24, splits <= 32: below 2^31)
+  const int stride = gridDim.x * kOwnWarps;  // (rows x heads <= 2^24, splits <= 32: units stay below 2^31)
+  // Unit u is (row, place in the row); steps of `stride` need no division.
+  struct Unit {
+    int r, place;
+  };
+  const int step_r = stride / per_row, step_place = stride % per_row;
+  auto next = [&](Unit u) {
+    u.r += step_r;
+    u.place += step_place;
+    if (u.place >= per_row) {
+      u.place -= per_row;
+      ++u.r;
+    }
+    return u;
+  };
+  auto part_of = [&](Unit u) { return splits == 1 ? 0 : u.place % splits; };
+  auto set_of = [&](Unit u) { return sets == 1 ? 0 : u.place / splits % sets; };
+  auto kv_head_of = [&](Unit u) { return splits * sets == 1 ? u.place : u.place / (splits * sets); };
 
   if (lane == 0) {
     for (int i = 0; i < kOwnStages; ++i) mbar_init(&full[warp][i], 1);
@@ -107,41 +124,50 @@ __global__ void __launch_bounds__(kOwnThreads)
   __syncwarp();
 
   // Chunks [c0, c1) of unit u, given its row's length; a length past the page table counts as 0.
-  auto range = [&](int u, int n, int& c0, int& c1) {
+  auto range = [&](Unit u, int n, int& c0, int& c1) {
     const int chunks = ((n < 0 || n > a.pages_per_row * kPageTokens ? 0 : n) + kTokens - 1) / kTokens;
-    const int per = (chunks + splits - 1) / splits, part = u % splits;
-    c0 = min(chunks, part * per);
+    if (splits == 1) {
+      c0 = 0;
+      c1 = chunks;
+      return;
+    }
+    const int per = (chunks + splits - 1) / splits;
+    c0 = min(chunks, part_of(u) * per);
     c1 = min(chunks, c0 + per);
   };
-  auto length = [&](int u) { return u < units ? a.own_len[u / per_row] : 0; };
+  auto length = [&](Unit u) { return u.r < a.rows ? a.own_len[u.r] : 0; };
 
   // ---- the loader: walks the warp's units and their chunks up to kOwnStages chunks ahead.  A unit's
   // length is requested two units ahead and its first page numbers (32 chunks, one a lane) one unit
   // ahead, so that no unit starts with a wait for them.
-  int lu = blockIdx.x * kOwnWarps + warp, lc, lc1, base_c, n0, n1, n2, pages, pages1;
-  auto first_pages = [&](int u, int n) {
+  const int first = blockIdx.x * kOwnWarps + warp;
+  const Unit start{first / per_row, first % per_row};
+  Unit lu = start, lu1 = next(lu);  // the unit loaded and the one behind it
+  int lc, lc1, base_c, n0, n1, n2, pages, pages1;
+  auto first_pages = [&](Unit u, int n) {
     int c0, c1;
     range(u, n, c0, c1);
     const int c = c0 + lane;
-    return u < units && c < c1 ? a.page_table[(u / per_row) * a.page_stride + c * kTokens / kPageTokens] : 0;
+    return u.r < a.rows && c < c1 ? a.page_table[u.r * a.page_stride + c * kTokens / kPageTokens] : 0;
   };
   {
     n0 = length(lu);
-    n1 = length(lu + stride);
-    n2 = length(lu + 2 * stride);
+    n1 = length(lu1);
+    n2 = length(next(lu1));
     range(lu, n0, lc, lc1);
     base_c = lc;
     pages = first_pages(lu, n0);
-    pages1 = first_pages(lu + stride, n1);
+    pages1 = first_pages(lu1, n1);
   }
   int loaded = 0;         // chunks requested
   unsigned bad_stage = 0;  // stages whose page was broken (nothing was loaded)
   auto load_next = [&]() {  // one more chunk into stage loaded % kOwnStages, if there is one
     while (lc >= lc1) {
-      if (lu >= units) return;
-      lu += stride;
+      if (lu.r >= a.rows) return;
+      lu = lu1;
+      lu1 = next(lu1);
       range(lu, n1, lc, lc1);
-      if (lu >= units) {
+      if (lu.r >= a.rows) {
         lc = lc1 = 0;
         return;
       }
@@ -149,13 +175,13 @@ __global__ void __launch_bounds__(kOwnThreads)
       pages = pages1;
       n0 = n1;
       n1 = n2;
-      n2 = length(lu + 2 * stride);
-      pages1 = first_pages(lu + stride, n1);
+      n2 = length(next(lu1));
+      pages1 = first_pages(lu1, n1);
     }
     if (lc >= base_c + 32) {
       base_c = lc;
       const int c = lc + lane;
-      pages = c < lc1 ? a.page_table[(lu / per_row) * a.page_stride + c * kTokens / kPageTokens] : 0;
+      pages = c < lc1 ? a.page_table[lu.r * a.page_stride + c * kTokens / kPageTokens] : 0;
     }
     const int page = __shfl_sync(0xffffffffu, pages, lc - base_c), st = loaded % kOwnStages;
     const bool ok = page >= 0 && page < a.own_pages;
@@ -164,7 +190,7 @@ __global__ void __launch_bounds__(kOwnThreads)
       unsigned char* stage = ring + st * kOwnStage;
       uint64_t* bar = &full[warp][st];
       if (ok) {
-        const int g = lu / (sets * splits) % a.kv_heads;
+        const int g = kv_head_of(lu);
         const int token = (page * a.kv_heads + g) * kPageTokens + lc * kTokens % kPageTokens;
         const int live = n0 - lc * kTokens;
         if (live > kTokens - kOwnPiece) {
@@ -196,17 +222,17 @@ __global__ void __launch_bounds__(kOwnThreads)
   for (int i = 0; i < kOwnStages; ++i) load_next();
 
   // A unit's queries: the A operand of rows lane / 4 (and 8 more), 16 channels a step.
-  auto load_queries = [&](int u, uint32_t (&qa)[D / 16][4]) {
-    const int g = u / (sets * splits) % a.kv_heads, h0 = g * group + u / splits % sets * kQueries;
-    const int heads = min(kQueries, (g + 1) * group - h0);
-    const T* q = static_cast<const T*>(a.q) + (int64_t)(u / per_row) * a.q_row + (int64_t)h0 * a.q_head;
+  auto load_queries = [&](Unit u, uint32_t (&qa)[D / 16][4]) {
+    const int g = kv_head_of(u), h0 = g * group + set_of(u) * kQueries;
+    const int heads = u.r < a.rows ? min(kQueries, (g + 1) * group - h0) : 0;
+    const T* q = static_cast<const T*>(a.q) + u.r * a.q_row + h0 * a.q_head;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e)
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
         const int row = lane / 4 + (f & 1) * 8, at = e * 16 + (f >> 1) * 8 + (lane & 3) * 2;
         qa[e][f] = 0;
-        if ((f & 1) < kHalves && u < units && row < heads) {
+        if ((f & 1) < kHalves && row < heads) {
           const unsigned short* src = reinterpret_cast<const unsigned short*>(q + row * a.q_head + at);
           qa[e][f] = q_pairs ? *reinterpret_cast<const uint32_t*>(src) : src[0] | (uint32_t)src[1] << 16;
         }
@@ -214,16 +240,17 @@ __global__ void __launch_bounds__(kOwnThreads)
   };
   const float c = a.scale * kLog2e;
   uint32_t qa[D / 16][4], qn[D / 16][4];
-  int u = blockIdx.x * kOwnWarps + warp, n_unit = length(u);
+  Unit u = start;
+  int n_unit = length(u);
   load_queries(u, qa);
   int used = 0;  // chunks consumed
   bool timeout = false;
-  for (; u < units && !timeout; u += stride) {
+  for (; u.r < a.rows && !timeout; u = next(u)) {
     int c0, c1;
     const int n = n_unit;
     range(u, n, c0, c1);
-    n_unit = length(u + stride);
-    load_queries(u + stride, qn);  // in flight under this unit
+    n_unit = length(next(u));
+    load_queries(next(u), qn);  // in flight under this unit
     bool broken = n > a.pages_per_row * kPageTokens;
     if (broken && lane == 0 && a.error) atomicExch(a.error, kErrOwnLength);
     float o[D / 8][4], m[kHalves], l[kHalves];
@@ -319,7 +346,7 @@ __global__ void __launch_bounds__(kOwnThreads)
       load_next();
     }
     // ---- the unit's sums
-    const int g = u / (sets * splits) % a.kv_heads, h0 = g * group + u / splits % sets * kQueries;
+    const int g = kv_head_of(u), h0 = g * group + set_of(u) * kQueries;
     const int heads = min(kQueries, (g + 1) * group - h0);
 #pragma unroll
     for (int f = 0; f < kHalves; ++f) {
@@ -328,7 +355,7 @@ __global__ void __launch_bounds__(kOwnThreads)
       if (broken || timeout) l[f] = __uint_as_float(0x7fc00000u);  // a row with broken pages comes out as NaN
       const int row = lane / 4 + 8 * f;
       if (row >= heads) continue;
-      const size_t dst = ((size_t)(first_part + u % splits) * a.rows + u / per_row) * a.heads + h0 + row;
+      const size_t dst = ((size_t)(first_part + part_of(u)) * a.rows + u.r) * a.heads + h0 + row;
       if ((lane & 3) == 0) part_ml[dst] = make_float2(m[f], l[f]);
       if (m[f] == -INFINITY) continue;
 #pragma unroll
@@ -343,11 +370,11 @@ __global__ void __launch_bounds__(kOwnThreads)
   if (timeout) {  // mark what is left, let the copies in flight land before the CTA exits (bounded)
     if (lane == 0 && a.error) atomicExch(a.error, kErrSharedWait);
     for (int i = used; i < loaded; ++i) mbar_wait(&full[warp][i % kOwnStages], (i / kOwnStages) & 1);
-    for (; u < units; u += stride)
+    for (; u.r < a.rows; u = next(u))
       for (int row = lane; row < kQueries; row += 32) {
-        const int g = u / (sets * splits) % a.kv_heads, h0 = g * group + u / splits % sets * kQueries;
+        const int g = kv_head_of(u), h0 = g * group + set_of(u) * kQueries;
         if (h0 + row < (g + 1) * group)
-          part_ml[((size_t)(first_part + u % splits) * a.rows + u / per_row) * a.heads + h0 + row] =
+          part_ml[((size_t)(first_part + part_of(u)) * a.rows + u.r) * a.heads + h0 + row] =
               make_float2(-INFINITY, __uint_as_float(0x7fc00000u));
       }
   }
@@ -466,8 +493,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 // every 16-bit attention (half a step of each weight); l sums the unrounded
 // float32 values; O is float32 throughout.
 //
-// Warp 0 loads K and V tiles by TMA into a ring, warp 1 issues the MMAs, warps
-// 4-7 and 8-11 are the softmax warpgroups.  What bounds a large call is the chain
+// Warp 0 loads K and V tiles by TMA into a ring, warp 1 (at dim 128 warps 1 and 2,
+// one per stream) issues the MMAs, warps 4-7 and 8-11 are the softmax warpgroups.  What bounds a large call is the chain
 // of one stream, S -> weights -> O: a warp alone runs the exponentials of a tile at
 // half the rate of their unit, so a CTA is kept small enough for two on an SM:
 //
@@ -477,7 +504,10 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 //     order, so S complete also means the last product complete.
 //   dim 128: O alone fills half the tensor memory; one CTA an SM.  S is handed
 //     back as soon as the softmax has it in registers, P has columns of its own,
-//     and S of the next tile is computed under this tile's exponentials.
+//     and S of the next tile is computed under this tile's exponentials.  With an
+//     issuing warp per stream neither waits for the other's softmax (124 -> 102 us
+//     at 1,024 rows of 16 heads over 8,192 tokens; at dim 64, where S follows PV
+//     anyway, one warp is faster, 126 against 135 us over 16,384).
 //
 // Every mbarrier wait is bounded; on a timeout the CTA marks its rows NaN, drains
 // its copies and MMAs (bounded), frees its tensor memory and returns.
@@ -490,6 +520,7 @@ template <int D, bool PAIR>
 struct Tile {
   static constexpr bool kShareS = D == 64;            // P in S's columns, two CTAs an SM
   static constexpr int kPerSm = kShareS ? 2 : 1;
+  static constexpr int kIssuers = kShareS ? 1 : 2;    // warps that issue MMAs
   static constexpr int kCols = kShareS ? 256 : 512;   // tensor memory: S0 S1 O0 O1 (P0 P1)
   static constexpr uint32_t kAtS = 0, kAtO = 2 * KT, kAtP = kShareS ? kAtS : kAtO + 2 * D;
   static constexpr uint32_t kStepP = kShareS ? KT : KT / 2;
@@ -541,7 +572,7 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&empty[i], PAIR ? Shape::kIssuers : 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
@@ -549,7 +580,7 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
       mbar_init(&p_full[s], 4);
       mbar_init(&pv_done[s], 1);
     }
-    mbar_init(&done, 1);
+    mbar_init(&done, Shape::kIssuers);
     aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();  // this thread starts copies on them ahead of the block's barrier
@@ -648,17 +679,15 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
       // every copy has landed before the ring is reused or the CTA exits (bounded)
       for (int k = max(0, issued - kSlots); k < issued; ++k) mbar_wait(&full[k % kSlots], (k / kSlots) & 1);
     }
-  } else if (warp == 1) {
-    // ---- MMA issuer: the warp stays converged (what describes an MMA is then warp-uniform), one
-    // lane issues
+  } else if (warp <= Shape::kIssuers) {
+    // ---- MMA issuers: the warp stays converged (what describes an MMA is then warp-uniform), one lane
+    // issues
     constexpr uint32_t kFormat = std::is_same<T, bf16>::value ? 1u : 0u;
     constexpr uint32_t kIdescS = umma_idesc(kFormat, kTileRows, KT, false);
     constexpr uint32_t kIdescO = umma_idesc(kFormat, kTileRows, D, true);
-    // The issuer's own waits and commits are a tile's critical resource (some 100 cycles each), so there
-    // is one full and one empty barrier per key tile and nothing is waited for twice.
     bool ok = true;
     auto issue_s = [&](int s, int k, int nth) {  // S_s = Q K_k^T, the stream's nth
-      if (!PAIR || s == 0) ok = ok && mbar_wait_fast(&full[k % kSlots], (k / kSlots) & 1);
+      ok = ok && mbar_wait_fast(&full[k % kSlots], (k / kSlots) & 1);
       if (!kShareS && nth > 0) ok = ok && mbar_wait_fast(&s_empty[s], (nth - 1) & 1);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -690,21 +719,28 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
           umma_f16_ta(tmem + Shape::kAtO + s * D, tmem + Shape::kAtP + s * Shape::kStepP + e * 8,
                       db + (uint64_t)(e * (16 * 128 >> 4)), kIdescO, nth > 0 || e > 0);
         if (!kShareS) umma_commit(&pv_done[s]);
-        if (!PAIR || s == 1) umma_commit(&empty[k % kSlots]);
+        if (!PAIR || Shape::kIssuers == 2 || s == 1) umma_commit(&empty[k % kSlots]);
       }
       __syncwarp();
     };
-    // a stream's tile n: query tile or key tiles of its parity
-    const int lag = PAIR ? 1 : 2;
-    for (int s = 0; s < 2; ++s)
-      if ((PAIR ? 0 : s) < nt) issue_s(s, PAIR ? 0 : s, 0);
-    for (int k = 0; k < nt; ++k)
-      for (int s = PAIR ? 0 : k & 1; s <= (PAIR ? 1 : k & 1); ++s) {
-        const int n = PAIR ? k : k >> 1;
-        if (!kShareS && k + lag < nt) issue_s(s, k + lag, n + 1);  // S runs one tile ahead
+    const int step = PAIR ? 1 : 2;  // between a stream's key tiles
+    if (Shape::kIssuers == 2) {  // a warp per stream
+      const int s = warp - 1, k0 = PAIR ? 0 : s;
+      if (k0 < nt) issue_s(s, k0, 0);
+      for (int k = k0, n = 0; k < nt; k += step, ++n) {
+        if (k + step < nt) issue_s(s, k + step, n + 1);  // S runs one tile ahead
         issue_pv(s, k, n);
-        if (kShareS && k + lag < nt) issue_s(s, k + lag, n + 1);
       }
+    } else {
+      for (int s = 0; s < 2; ++s)
+        if ((PAIR ? 0 : s) < nt) issue_s(s, PAIR ? 0 : s, 0);
+      for (int k = 0; k < nt; ++k)
+        for (int s = PAIR ? 0 : k & 1; s <= (PAIR ? 1 : k & 1); ++s) {
+          const int n = PAIR ? k : k >> 1;
+          issue_pv(s, k, n);
+          if (k + step < nt) issue_s(s, k + step, n + 1);
+        }
+    }
     if (!ok && lane == 0) fail();
     if (elect_one()) umma_commit(&done);  // arrives once every MMA issued has completed
     __syncwarp();
@@ -1009,7 +1045,7 @@ cudaError_t launch_own(const SharedAttnArgs& a, float* o, float2* ml, cudaStream
   // a warp takes one unit of long rows (the hardware evens out their lengths; a persistent grid with
   // units dealt in turn was a quarter slower), or several of short ones, 16 chunks' room in all, as
   // long as that leaves six warps an SM
-  const long long room = std::max<long long>(1, (long long)a.pages_per_row * (a.dim / 64) / a.own_splits);
+  const long long room = std::max<long long>(1, (long long)a.pages_per_row * (kPageTokens / kTokens) / a.own_splits);
   const long long each = std::max<long long>(1, std::min<long long>(16 / room, units / (6 * 148))) * kOwnWarps;
   const dim3 grid((unsigned)((units + each - 1) / each));
   return launch(kernel, grid, kOwnThreads, kOwnSmem, s, pdl, map_k, map_v, map_k_piece, map_v_piece, a, q_pairs, o, ml,
