@@ -1831,6 +1831,9 @@ int32_t s2r_step_sampled(s2r_ctx* c, int32_t n_steps, const s2r_sampling* how, v
       (!how->top_p && !(how->top_p_all >= 0.f && how->top_p_all <= 1.f)) ||
       (!how->min_p && !(how->min_p_all >= 0.f && how->min_p_all <= 1.f)))
     return fail(S2R_EINVAL, "s2r_step_sampled: temperature >= 0, top_k >= 0, top_p and min_p in [0, 1] expected");
+  for (const void* p : {(const void*)how->uniforms, (const void*)how->temperature, (const void*)how->top_k,
+                        (const void*)how->top_p, (const void*)how->min_p, (const void*)how->logprobs})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return fail(S2R_EINVAL, "s2r_step_sampled: a pointer is not aligned to 4 bytes");
   CK(cudaSetDevice(c->device));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   for (int slot = 0; slot < c->B; ++slot) {

@@ -1087,6 +1087,11 @@ extern "C" int32_t s2r_sample(const s2r_sample_args* in, void* stream) {
   if (!in->top_p && !(in->top_p_all >= 0.f && in->top_p_all <= 1.f)) return bad("s2r_sample: top_p must be in [0, 1]");
   if (!in->min_p && !(in->min_p_all >= 0.f && in->min_p_all <= 1.f)) return bad("s2r_sample: min_p must be in [0, 1]");
   if (!in->top_k && in->top_k_all < 0) return bad("s2r_sample: top_k must be >= 0");
+  auto off = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+  if (off(in->logits, in->logits_dtype == S2R_F32 ? 4 : 2) || off(in->bias, 4) || off(in->uniforms, 4) ||
+      off(in->temperature, 4) || off(in->top_k, 4) || off(in->top_p, 4) || off(in->min_p, 4) || off(in->tokens, 8) ||
+      off(in->logprobs, 4))
+    return bad("s2r_sample: a pointer is not aligned to its type");
   s2r::SampleArgs a{};
   a.logits = in->logits;
   a.dtype = in->logits_dtype;

@@ -565,9 +565,9 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
   __shared__ int aborted;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int part = blockIdx.x, parts = gridDim.x, g = blockIdx.z;
+  const int parts = a.shared_splits, tile = (int)blockIdx.x / parts, part = (int)blockIdx.x - tile * parts, g = blockIdx.y;
   const int group = a.heads / a.kv_heads, queries = a.rows * group;
-  const int tile0 = blockIdx.y * (PAIR ? 2 : 1);  // first query tile
+  const int tile0 = tile * (PAIR ? 2 : 1);  // first query tile
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
@@ -1025,7 +1025,8 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml
   const cudaError_t e = allow_smem(kernel, smem, done);
   if (e != cudaSuccess) return e;
   const int tiles = PAIR ? (query_tiles(a) + 1) / 2 : query_tiles(a);
-  return launch(kernel, dim3(a.shared_splits, tiles, a.kv_heads), kTileThreads, smem, s, pdl, map_k, map_v, t);
+  // (parts and tiles on one axis: up to 65,536 tiles)
+  return launch(kernel, dim3((unsigned)tiles * a.shared_splits, a.kv_heads), kTileThreads, smem, s, pdl, map_k, map_v, t);
 }
 
 template <typename T, int D, bool WIDE>
@@ -1159,8 +1160,16 @@ int prepare(const s2r_shared_attention_args* in, s2r::SharedAttnArgs& a, size_t*
                              in->page_table_stride};
   for (int64_t s : strides)
     if (s < 0 || s > widest) return bad("strides must be between 0 and 2^38 elements");
-  if ((in->rows > 1 && in->out_row_stride < in->head_dim) || (in->heads > 1 && in->out_head_stride < in->head_dim))
+  // two (row, head) of out share no element if the longer stride steps over all the shorter one spans
+  const int64_t rows_apart = (in->heads - 1) * in->out_head_stride + in->head_dim;
+  const int64_t heads_apart = (in->rows - 1) * in->out_row_stride + in->head_dim;
+  if ((in->rows > 1 && in->out_row_stride < in->head_dim) || (in->heads > 1 && in->out_head_stride < in->head_dim) ||
+      (in->rows > 1 && in->heads > 1 && in->out_row_stride < rows_apart && in->out_head_stride < heads_apart))
     return bad("rows or heads of out overlap");
+  auto off = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+  if (off(in->q, 2) || off(in->out, 2) || off(in->lse, 4) || off(in->shared_len, 4) || off(in->page_table, 4) ||
+      off(in->own_len, 4) || off(in->error, 4))
+    return bad("a pointer is not aligned to its type");
   if (in->shared_tokens) {
     if (!in->shared_k || !in->shared_v) return bad("shared_k or shared_v is NULL");
     // K and V are fetched in 16-byte pieces

@@ -14,6 +14,10 @@
 * ``shard.decode_readings`` on it, end to end.
 """
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -245,3 +249,38 @@ def test_greedy_readings_are_alike():
     song = Song(memory_array(300, sc.C1_SHORT.width, 52), [SOS, OUT], frames=250, target=20)
     readings = decode_readings(eng, song, 3, temperature=0.0)
     assert len({tuple(r.tokens) for r in readings}) == 1 and readings[0].ended == "eos"
+
+
+CAPTURED_FIRST = """
+import torch
+from sheetsage2_refined_b200 import ops
+g = torch.Generator(device="cuda").manual_seed(1)
+def rand(*shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=dtype)
+q, k, v = rand(40, 8, 64), rand(300, 2, 64), rand(300, 2, 64)
+pool = rand(40, 2, 64, 64)
+own = dict(own_k=pool, own_v=pool, page_table=torch.arange(40, device="cuda", dtype=torch.int32).view(40, 1),
+           own_len=torch.arange(40, device="cuda", dtype=torch.int32))
+w, u = rand(512, 700, dtype=torch.float32), torch.rand(40, generator=g, device="cuda")
+def step():
+    out, lse = ops.shared_attention(q, k, v, **own)
+    logits = out.float().reshape(40, 512)[:, :, None].mul(w).sum(1)
+    return out, lse, *ops.sample(logits, u, top_k=20, top_p=0.9)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("equal")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Attention, then a draw from what it gives, captured before either kernel has been set up."""
+
+    run = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0 and "equal" in run.stdout, run.stderr[-2000:]

@@ -264,3 +264,33 @@ def test_calls_are_deterministic_overlap_and_replay():
         torch.cuda.synchronize()
         again, _ = ops.shared_attention(q, k, v, **own, shared_len=length)
         assert torch.equal(outs[0][0], again) and torch.equal(outs[1][0], again)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_k_and_v_in_different_layouts_and_out_in_place(dim):
+    """K as [heads, tokens, dim] and V as [tokens, heads, dim] or the other way round; out may be q itself."""
+
+    for k_major in (True, False):
+        q, k, v, own = make(20, 6, 3, dim, 333, [(41 * r) % 190 for r in range(20)], F16, seed=12)
+        if k_major:
+            v = v.contiguous()
+        else:
+            k = k.contiguous()
+        for pages in (own, {}):
+            want = exact(q, k, v, *[pages.get(x) for x in ("own_k", "own_v", "page_table", "own_len")], dim**-0.5)
+            mine = q.clone()
+            out, lse = ops.shared_attention(mine, k, v, **pages, out=mine)
+            assert_close(out, lse, want, F16)
+
+
+@gpu
+def test_the_most_rows_and_heads_of_a_call():
+    """2^24 (row, head) pairs over one kv head: 131,072 query tiles."""
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(32768, 512, 64, generator=g, device="cuda", dtype=BF16)
+    k, v = (torch.randn(70, 1, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+    out, lse = ops.shared_attention(q, k, v)
+    for rows in ([0, 1], [16383, 16384], [32766, 32767]):
+        assert_close(out[rows], lse[rows], exact(q[rows], k, v, None, None, None, None, 0.125), BF16)

@@ -22,7 +22,9 @@ def sample_args(**kw):
     (dict(logits_dtype=3), b"float32"), (dict(logits_stride=-1), b"stride"), (dict(allowed_stride=-8), b"stride"),
     (dict(temperature_all=-0.5), b"temperature"), (dict(temperature_all=float("nan")), b"temperature"),
     (dict(top_p_all=1.5), b"top_p"), (dict(top_p_all=float("nan")), b"top_p"), (dict(min_p_all=-0.1), b"min_p"),
-    (dict(top_k_all=-1), b"top_k"),
+    (dict(top_k_all=-1), b"top_k"), (dict(logits=18), b"aligned"), (dict(tokens=20), b"aligned"),
+    (dict(uniforms=17), b"aligned"), (dict(bias=18), b"aligned"), (dict(top_k=19), b"aligned"),
+    (dict(logprobs=22), b"aligned"),
 ])
 def test_sample_entry_point_refuses(change, word):
     lib = _lib.load()
@@ -64,6 +66,10 @@ OWN = dict(own_k=16, own_v=16, own_pages=4, pages_per_row=2, page_table=16, page
     (dict(scale=float("inf")), b"scale"), (dict(own_k=16), b"go together"), (dict(own_len=16), b"go together"),
     (dict(OWN, own_pages=0), b"own_pages"), (dict(OWN, pages_per_row=0), b"pages_per_row"),
     (dict(OWN, page_table_stride=1), b"page table"), (dict(OWN, own_pages=2**24), b"2^25"), (dict(OWN, own_v=40), b"aligned"),
+    (dict(q=17), b"aligned"), (dict(out=33), b"aligned"), (dict(lse=18), b"aligned"), (dict(shared_len=18), b"aligned"),
+    (dict(OWN, page_table=18), b"aligned"), (dict(OWN, own_len=18), b"aligned"), (dict(error=18), b"aligned"),
+    # rows one head apart, heads one row apart: (0, 1) and (1, 0) of out would be the same place
+    (dict(out_row_stride=64, out_head_stride=64), b"overlap"), (dict(out_row_stride=192, out_head_stride=64), b"overlap"),
 ])
 def test_shared_attention_entry_point_refuses(change, word):
     lib = _lib.load()
