@@ -1085,7 +1085,11 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     // the split with the fewest key tiles one after the other: waves of CTAs times the tiles of
     // each, plus about 6 tiles' time to start and end it
     const long long ctas = (long long)(a.pair ? (tiles + 1) / 2 : tiles) * a.kv_heads;
-    const long long slots = (long long)sms * (a.dim == 64 ? 2 : 1);
+    // Dim 64 runs two CTAs on an SM; a short shared part beside own pages takes one, which leaves the own
+    // part's warps room from the start (64 rows x 16 heads, own rows of 1,500: over 2,048 shared tokens
+    // 54 -> 50 us, 8,192 57.4 -> 56.3, but 16,384 65.6 -> 67.9)
+    const bool brief = a.own_k && ctas * keys <= 16ll * sms;
+    const long long slots = (long long)sms * (a.dim == 64 && !brief ? 2 : 1);
     long long best = -1;
     for (int sp = 1; sp <= keys && sp <= kMaxSharedSplits; ++sp) {
       const int per = (keys + sp - 1) / sp;
@@ -1098,11 +1102,14 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     }
   }
   if (a.own_k) {
-    // six warps an SM, two units for each
+    // Six warps an SM, two units for each, of four chunks or more (64 rows x 16 heads of dim 64, own rows of up
+    // to 400: one part of 7 pages 25 us, two 28); two pages do while most warps would stay idle (4 rows of
+    // 500: 2 pages a part 13.3 us, 4 pages 14.3).
     const int group = a.heads / a.kv_heads, queries = group > 8 ? 16 : 8;
     const long long pieces = (long long)a.rows * a.kv_heads * ((group + queries - 1) / queries);
+    const int chunks = a.pages_per_row * (a.dim / 64);
     int sp = 1;
-    while (sp < kMaxOwnSplits && pieces * sp < 12ll * sms && a.pages_per_row / (sp * 2) >= 2) sp *= 2;
+    while (sp < kMaxOwnSplits && pieces * sp < 12ll * sms && chunks / (sp * 2) >= (pieces * sp < 3ll * sms ? a.dim / 32 : 4)) sp *= 2;
     a.own_splits = sp;
   }
   const size_t parts = a.shared_splits + a.own_splits;
