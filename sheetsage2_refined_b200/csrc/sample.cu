@@ -663,16 +663,25 @@ __device__ bool try_finish(RowSampler<C>& row, const SampleArgs& a, int r, uint3
     z += __uint_as_float((uint32_t)box[p][1]);
   }
   if (total > (unsigned)list_max(C)) return false;
-  if (row.rank == 0) {
-    gather(row, sh.list, count, total);
-    finish<COUNT, C>(row, (int)total, lowest, target, d);
-    if (threadIdx.x == 0) {
-      const u64 key = sh.found[0];
-      a.tokens[r] = (int64_t)~(uint32_t)key;
-      if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
-    }
+  // into rank 0's memory, where they are in index order; the peers are then done
+  unsigned from = 0;
+#pragma unroll
+  for (int p = 0; p < C; ++p) from += p < row.rank ? count[p] : 0u;
+  u64* to = row.peer(sh.sorted, 0) + from;
+  for (unsigned i = threadIdx.x; i < mine; i += kSampleThreads) to[i] = sh.list[i];
+  if (C > 1) {
+    cg::this_cluster().barrier_arrive();
+    if (row.rank != 0) return true;
+    cg::this_cluster().barrier_wait();
+  } else {
+    __syncthreads();
   }
-  row.barrier();  // rank 0 has read the peers' lists
+  finish<COUNT, C>(row, (int)total, lowest, target, d);
+  if (threadIdx.x == 0) {
+    const u64 key = sh.found[0];
+    a.tokens[r] = (int64_t)~(uint32_t)key;
+    if (a.logprobs) a.logprobs[r] = (image_value((uint32_t)(key >> 32)) - row.best) - logf(z);
+  }
   return true;
 }
 
