@@ -669,13 +669,8 @@ __device__ bool try_finish(RowSampler<C>& row, const SampleArgs& a, int r, uint3
   for (int p = 0; p < C; ++p) from += p < row.rank ? count[p] : 0u;
   u64* to = row.peer(sh.sorted, 0) + from;
   for (unsigned i = threadIdx.x; i < mine; i += kSampleThreads) to[i] = sh.list[i];
-  if (C > 1) {
-    cg::this_cluster().barrier_arrive();
-    if (row.rank != 0) return true;
-    cg::this_cluster().barrier_wait();
-  } else {
-    __syncthreads();
-  }
+  row.barrier();
+  if (row.rank != 0) return true;
   finish<COUNT, C>(row, (int)total, lowest, target, d);
   if (threadIdx.x == 0) {
     const u64 key = sh.found[0];
