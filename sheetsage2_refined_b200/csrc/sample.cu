@@ -1005,8 +1005,8 @@ int sample_chunk(int vocab, int splits) {  // a multiple of 32 tokens a warp
   return (per + kSampleWarps * 32 - 1) / (kSampleWarps * 32) * (kSampleWarps * 32);
 }
 
-// CTAs per row: enough that two of them fit an SM (1,024 rows of 32,576 tokens: one CTA a row takes 181 us,
-// two 146 us, four 240 us, more of it in barriers), then more while the rows leave SMs idle and a
+// CTAs per row: enough that two of them fit an SM (1,024 rows of 32,576 tokens: one CTA a row takes 188 us,
+// two 152 us, four 228 us, more of it in barriers), then more while the rows leave SMs idle and a
 // share is worth splitting.
 int sample_splits(int rows, int vocab, int sms) {
   int c = 1;

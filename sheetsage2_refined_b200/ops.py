@@ -191,7 +191,7 @@ def shared_attention(q: torch.Tensor, shared_k: torch.Tensor, shared_v: torch.Te
         own_args = (own_k.data_ptr(), own_v.data_ptr(), pool[0], pages, page_table.data_ptr(),
                     page_table.stride(0) if rows > 1 else 0, _vector("own_len", own_len, rows, torch.int32, device))
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
     elif not isinstance(out, torch.Tensor) or out.dtype is not dtype or out.device != device or (
             out.shape != shape or out.stride(2) != 1):
         raise _bad("out", out, dtype, shape, device)
