@@ -44,6 +44,13 @@ __device__ __forceinline__ unsigned long long global_ns() {
 
 // Cluster barrier in two halves (release on arrive, acquire on wait), every
 // thread of every CTA of the cluster taking part.
+// 2^x on the special function unit (results below 2^-126 become 0).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // Arrive without ordering memory (execution only).

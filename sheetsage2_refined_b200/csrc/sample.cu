@@ -79,12 +79,11 @@ struct alignas(16) SampleShared {  // (the images behind it are stored four at a
   unsigned listed, counts[kSampleWarps];
 };
 
-// Order-preserving image of a float (select.cuh): -0 as +0, every NaN on top.
+// Order-preserving image of a float (select.cuh): -0 as +0, every NaN on top.  The addition makes +0 of
+// -0 and the canonical (positive) NaN of every NaN.
 __device__ __forceinline__ uint32_t value_image(float v) {
-  uint32_t u = __float_as_uint(v);
-  if (u == 0x80000000u) u = 0u;
-  if (v != v) u = 0x7fffffffu;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint(__fadd_rn(v, 0.f));
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float image_value(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
@@ -94,14 +93,17 @@ __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 
-// What a lane knows of its tokens after loading them: the largest and the lowest drawable image, and
-// z = sum exp(x - m) over the allowed with m the largest value (kept up as the sum of a running softmax).
+// What a lane knows of its tokens after loading them: the largest image, the lowest drawable one less
+// kImgNegInf + 1 (those that cannot be drawn wrap to the top), and z = sum exp(x - m) over the allowed with m
+// the largest value (kept up as the sum of a running softmax).
 struct LaneStats {
   uint32_t top = 0, bottom = 0xffffffffu;
   float m = -INFINITY, z = 0.f;
 };
 
-// This warp's images [w0, w1) of the allowed tokens (0: masked) into shared memory.  VEC: the row's
+__device__ __forceinline__ float exp_approx(float x) { return exp2_approx(x * 1.4426950408889634f); }
+
+// This warp's images [w0, w1) (masked tokens as -inf) into shared memory.  VEC: the row's
 // logits, mask and bias allow four tokens a load.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_images(const T* __restrict__ logits, const float* __restrict__ bias,
@@ -145,16 +147,16 @@ __device__ __forceinline__ void load_images(const T* __restrict__ logits, const 
         const float add = VEC ? (j == 0 ? b[q].x : j == 1 ? b[q].y : j == 2 ? b[q].z : b[q].w) : b1[q];
         const bool ok = ((mask[q] >> (8 * j)) & 0xffu) != 0;
         x[j] = bias ? __fadd_rn(to_float(raw[q][j]), add) : to_float(raw[q][j]);
-        u[j] = ok ? value_image(x[j]) : 0u;
-        st.top = u[j] > st.top ? u[j] : st.top;
-        if (u[j] > kImgNegInf) st.bottom = u[j] < st.bottom ? u[j] : st.bottom;
         x[j] = ok ? x[j] : -INFINITY;
+        u[j] = value_image(x[j]);
+        st.top = max(st.top, u[j]);
+        st.bottom = min(st.bottom, u[j] - (kImgNegInf + 1));
         m = fmaxf(m, x[j]);
       }
       if (m != -INFINITY) {
-        float z = st.z * __expf(st.m - m);
+        float z = st.z * exp_approx(st.m - m);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) z += __expf(x[j] - m);
+        for (int j = 0; j < kEach; ++j) z += exp_approx(x[j] - m);
         st.z = z;
         st.m = m;
       }
@@ -620,10 +622,13 @@ __device__ unsigned collect(RowSampler<C>& row, uint32_t lowest) {
   SampleShared<C>& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned count = 0;
+  const int whole = row.w0 + (row.w1 - row.w0) / 4 * 4;
 #pragma unroll 4
-  for (int i = row.w0 + lane; i < row.w1; i += 32) {
-    count += row.img[i] >= lowest;
+  for (int i = row.w0 + 4 * lane; i < whole; i += 128) {
+    const uint4 u = *reinterpret_cast<const uint4*>(row.img + i);
+    count += (unsigned)(u.x >= lowest) + (u.y >= lowest) + (u.z >= lowest) + (u.w >= lowest);
   }
+  if (whole + lane < row.w1) count += row.img[whole + lane] >= lowest;
   count = __reduce_add_sync(0xffffffffu, count);
   if (lane == 0) sh.counts[warp] = count;
   __syncthreads();
@@ -859,7 +864,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   d.uniform = a.uniforms[r];
   const float m = a.min_p ? a.min_p[r] : a.min_p_all;
   RowSampler<C> row{sh, img, first, rank, w0, w1};
-  uint32_t top = __reduce_max_sync(0xffffffffu, st.top), bottom = __reduce_min_sync(0xffffffffu, st.bottom);
+  uint32_t top = __reduce_max_sync(0xffffffffu, st.top);
+  uint32_t bottom = __reduce_min_sync(0xffffffffu, st.bottom);
   {
     if (lane == 0) sh.part[warp] = ((u64)top << 32) | bottom;
     __syncthreads();
@@ -872,6 +878,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
       top = max(top, (uint32_t)(box[p][0] >> 32));
       bottom = min(bottom, (uint32_t)box[p][0]);
     }
+    bottom += kImgNegInf + 1;
   }
   const bool finite = top > kImgNegInf && top < kImgPosInf;
   row.best = finite ? image_value(top) : 0.f;
@@ -880,7 +887,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   const bool greedy = !finite || !(t > 0.f);
   d.floor_w = m > 0.f ? (u64)ceil((double)fminf(m, 1.f) * (double)(1ull << a.scale_bits)) : 0ull;
   // this CTA's sum of exp(x - best) over the allowed tokens
-  float z = block_sum_f32(sh, finite && st.m != -INFINITY ? st.z * __expf(st.m - row.best) : 0.f);
+  float z = block_sum_f32(sh, finite && st.m != -INFINITY ? st.z * exp_approx(st.m - row.best) : 0.f);
 
   if (greedy) {
     uint32_t lowest = 0xffffffffu;
@@ -1005,7 +1012,7 @@ int sample_chunk(int vocab, int splits) {  // a multiple of 32 tokens a warp
   return (per + kSampleWarps * 32 - 1) / (kSampleWarps * 32) * (kSampleWarps * 32);
 }
 
-// CTAs per row: enough that two of them fit an SM (1,024 rows of 32,576 tokens: one CTA a row takes 188 us,
+// CTAs per row: enough that two of them fit an SM (1,024 rows of 32,576 tokens: one CTA a row took 188 us,
 // two 152 us, four 228 us, more of it in barriers), then more while the rows leave SMs idle and a
 // share is worth splitting.
 int sample_splits(int rows, int vocab, int sms) {

@@ -247,3 +247,22 @@ def test_streams_overlapping_calls_and_graph_replay():
     torch.cuda.synchronize()
     again, _ = expect(logits, uu.cpu(), bias, allowed, 0.9, 70, 0.9, 0.0)
     assert torch.equal(tokens.cpu(), again)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_nans_of_either_sign_and_masked_ones(dtype):
+    x = torch.zeros(5, 700, dtype=dtype)
+    ints = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    wide = {torch.float32: 0xFFC00001 - 2**32, torch.bfloat16: 0xFFC1 - 2**16, torch.float16: 0xFE01 - 2**16}[dtype]
+    ints[0, 300] = wide  # a negative NaN with a payload
+    ints[1, 300], x[1, 650] = wide, math.nan
+    x[2, 12], ints[2, 600] = math.nan, wide
+    ints[3, 300] = wide
+    x[4], x[4, ::3] = -0.0, 0.0
+    allowed = torch.ones(5, 700, dtype=torch.bool)
+    allowed[3, 300] = False
+    tokens, lp = ops.sample(x.cuda(), torch.full((5,), 0.5, device="cuda"), allowed=allowed.cuda())
+    # rows 3 and 4: equal weights, the middle one of 699 and of 700 tokens
+    assert tokens.tolist() == [300, 300, 12, 350, 350]
+    assert lp[:3].isnan().all() and (lp[3:].cpu() + torch.tensor([699.0, 700.0]).log()).abs().max() < 1e-5
