@@ -407,7 +407,7 @@ typedef struct s2r_shared_attention_args {
   const int32_t* page_table; /* [rows, pages_per_row]; entries past a row's length are not read */
   int64_t page_table_stride; /* between rows; 0: every row the same pages */
   const int32_t* own_len;    /* [rows] tokens of each row, 0 .. pages_per_row * S2R_PAGE_TOKENS (below 0 counts as 0) */
-  void* out;                 /* [rows, heads, head_dim] */
+  void* out;                 /* [rows, heads, head_dim]; may be q with the same strides, else apart from every input */
   int64_t out_row_stride, out_head_stride;
   float* lse;                /* [rows, heads] contiguous, or NULL */
   void* workspace;           /* s2r_shared_attention_workspace bytes, 16-byte aligned */

@@ -46,7 +46,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // two cost no start of their own (a CTA per row and head reached 3.3 TB/s on
 // such rows).  Memory bounds this part (a key is read for heads / kv_heads
 // queries), so what counts is bytes in flight, 192 KB an SM, and there is no
-// barrier beyond the warp.  The products are mma.sync m16n8k16, rows = the
+// barrier beyond the warp (5.6 TB/s on rows of up to 2,500 tokens, 8 heads of
+// dim 128; 4.9 TB/s on rows of up to 200, 16 heads of dim 64).  The products are mma.sync m16n8k16, rows = the
 // group's queries (8, or 16 with WIDE): a 128-row tcgen05 tile would hold at
 // most 16 live rows and its round trip through tensor memory would sit in the
 // chain of every chunk.
@@ -494,9 +495,12 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 // float32 values; O is float32 throughout.
 //
 // Warp 0 loads K and V tiles by TMA into a ring, warp 1 (at dim 128 warps 1 and 2,
-// one per stream) issues the MMAs, warps 4-7 and 8-11 are the softmax warpgroups.  What bounds a large call is the chain
-// of one stream, S -> weights -> O: a warp alone runs the exponentials of a tile at
-// half the rate of their unit, so a CTA is kept small enough for two on an SM:
+// one per stream) issues the MMAs, warps 4-7 and 8-11 are the softmax warpgroups.
+// What bounds a large call is the chain of one stream, S -> weights -> O (about
+// half of a tile's time passes in its barriers and the tensor memory's round
+// trips; the exponentials' unit is busy 54% of the time at dim 64), so as many
+// streams as fit run on an SM (1,024 rows of 16 heads over 16,384 tokens: 126 us,
+// 546 TFLOP/s):
 //
 //   dim 64: P lies in S's columns, 256 columns and 98 KB a CTA, two CTAs an SM,
 //     four streams.  The next S of a stream follows the product that reads P;

@@ -149,7 +149,7 @@ def shared_attention(q: torch.Tensor, shared_k: torch.Tensor, shared_v: torch.Te
     pages]`` and ``own_len`` ``[rows]`` are int32.  ``scale`` defaults to
     ``dim ** -0.5``.
 
-    Returns ``(out, lse)``: ``out`` like ``q``, ``lse`` ``[rows, heads]``
+    Returns ``(out, lse)``: ``out`` like ``q`` (it may be ``q`` itself), ``lse`` ``[rows, heads]``
     float32, the log of the sum of exponentials of the scaled scores.  A row
     without keys gives 0 and ``-inf``; a row whose pages are broken gives NaN
     and sets ``error`` (an int32 tensor of one value) if given.
