@@ -1089,11 +1089,13 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     // the split with the fewest key tiles one after the other: waves of CTAs times the tiles of
     // each, plus about 6 tiles' time to start and end it
     const long long ctas = (long long)(a.pair ? (tiles + 1) / 2 : tiles) * a.kv_heads;
-    // Dim 64 runs two CTAs on an SM; a short shared part beside own pages takes one, which leaves the own
-    // part's warps room from the start (64 rows x 16 heads, own rows of 1,500: over 2,048 shared tokens
-    // 54 -> 50 us, 8,192 57.4 -> 56.3, but 16,384 65.6 -> 67.9)
+    // Dim 64 runs two CTAs on an SM; a short shared part beside own pages takes one, or at dim 128, whose CTA
+    // fills an SM, half of the SMs: the own part's warps have room from the start.  (Dim 64, 64 rows x 16 heads,
+    // own rows of up to 1,500: over 2,048 shared tokens 54 -> 50 us, 8,192 57.4 -> 56.3, but 16,384 65.6 -> 67.9.
+    // Dim 128, 100 rows x 32/8 heads, own rows of up to 2,500, over 1,111 tokens 123 -> 114 us, 4,000 125 -> 120,
+    // 32 rows 61 -> 52, own rows of up to 300 43 -> 40.)
     const bool brief = a.own_k && ctas * keys <= 16ll * sms;
-    const long long slots = (long long)sms * (a.dim == 64 && !brief ? 2 : 1);
+    const long long slots = a.dim == 64 ? (brief ? sms : 2ll * sms) : (brief ? std::max(1, sms / 2) : sms);
     long long best = -1;
     for (int sp = 1; sp <= keys && sp <= kMaxSharedSplits; ++sp) {
       const int per = (keys + sp - 1) / sp;

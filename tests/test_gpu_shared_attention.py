@@ -294,3 +294,25 @@ def test_the_most_rows_and_heads_of_a_call():
     out, lse = ops.shared_attention(q, k, v)
     for rows in ([0, 1], [16383, 16384], [32766, 32767]):
         assert_close(out[rows], lse[rows], exact(q[rows], k, v, None, None, None, None, 0.125), BF16)
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+def test_broadcast_queries_one_page_table_for_all_and_repeated_pages(dim, dtype):
+    q, k, v, own = make(6, 4, 2, dim, 200, [256] * 6, dtype, seed=21, junk=False)
+    table = own["page_table"][0].clone()
+    table[2] = table[0]  # the same page twice in a row
+    own["page_table"] = table.expand(6, -1)
+    own["own_len"] = torch.tensor([256, 200, 64, 1, 0, 129], dtype=torch.int32, device="cuda")
+    check(q[:1].expand(6, -1, -1), k, v, own, dtype)
+    check(q[:, :1].expand(-1, 4, -1), k, v, own, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dim,heads,kvh", [(64, 16, 16), (128, 32, 8)])
+def test_short_and_long_shared_parts_beside_own_pages(dim, heads, kvh):
+    """Either side of the size up to which the shared part leaves the own part room on the SMs."""
+
+    for shared in (1111, 20000 if dim == 64 else 24000):
+        q, k, v, own = make(24, heads, kvh, dim, shared, [(97 * r) % 500 for r in range(24)], BF16, seed=22)
+        check(q, k, v, own, BF16)
