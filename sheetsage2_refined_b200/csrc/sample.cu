@@ -693,13 +693,12 @@ __device__ bool try_finish(RowSampler<C>& row, const SampleArgs& a, int r, uint3
 }
 
 // Cuts `kept` to its first k tokens (COUNT) or to the shortest prefix that holds a share p of its
-// weight, from the histogram that fill_histogram left in sh.hist[(turn - 1) & 1] behind a barrier.
-// FINISH (weights, nothing cut yet): tries to finish the row on the way; true if it did.
-template <bool COUNT, bool FINISH, int C>
-__device__ bool shrink(RowSampler<C>& row, Kept& kept, const SampleArgs& a, int r, const DrawArgs& d, float& z) {
+// weight, from the histogram that fill_histogram left in sh.hist[buffer] behind a barrier.
+template <bool COUNT, int C>
+__device__ void shrink(RowSampler<C>& row, Kept& kept, const DrawArgs& d, int buffer) {
   SampleShared<C>& sh = row.sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const u64* hist = sh.hist[(row.turn - 1) & 1];
+  const u64* hist = sh.hist[buffer];
   constexpr int kPer = kSampleBins / kSampleThreads;  // bin 0 holds the largest values
   static_assert(kPer == 2, "two bins a thread");
   const int b0 = (int)threadIdx.x * kPer;
@@ -720,7 +719,7 @@ __device__ bool shrink(RowSampler<C>& row, Kept& kept, const SampleArgs& a, int 
   u64 all = 0;
   const u64 incl = block_scan(sh, v0 + v1, &all);
   const u64 target = COUNT ? (u64)d.k : share_of(d.p, all);
-  if (target > all) return false;  // nothing to leave out (counts only)
+  if (target > all) return;  // nothing to leave out (counts only)
   const u64 run = incl - v0 - v1;
   if (run < target && incl >= target) {
     const bool second = run + v0 < target;
@@ -731,11 +730,6 @@ __device__ bool shrink(RowSampler<C>& row, Kept& kept, const SampleArgs& a, int 
   const int bin = (int)sh.found[0];
   const u64 above = sh.found[1];
   const uint32_t lowest = row.bin_floor(bin);
-  if (FINISH) {
-    if (try_finish<false>(row, a, r, lowest, target, d, z)) return true;
-    if (threadIdx.x == 0) sh.listed = 0;
-    __syncthreads();
-  }
   // ---- the tokens of the crossing bin
   for (int i = row.w0 + lane; i < row.w1; i += 32) {
     const uint32_t u = row.img[i];
@@ -753,7 +747,7 @@ __device__ bool shrink(RowSampler<C>& row, Kept& kept, const SampleArgs& a, int 
     const RadixResult res = shrink_radix<COUNT, C>(row, kept, target);
     kept = res.kept;
     row.turn = res.turn;
-    return false;
+    return;
   }
   const int padded = gather(row, sh.list, count, n);
   sort_descending(sh.sorted, padded);
@@ -778,7 +772,6 @@ __device__ bool shrink(RowSampler<C>& row, Kept& kept, const SampleArgs& a, int 
   __syncthreads();
   kept.lo = (uint32_t)(sh.found[0] >> 32);
   kept.last = (int)~(uint32_t)sh.found[0];
-  return false;
 }
 
 // Histogram of the row's kept tokens, of counts or weights, behind a barrier.
@@ -809,6 +802,26 @@ __device__ void fill_histogram(RowSampler<C>& row, const Kept& kept) {
   }
   ++row.turn;
   row.barrier();
+}
+
+// Top-p alone, on the same histogram: the bin in which the sum crosses its share bounds what is kept, and the
+// tokens from it on are finished, if they fit; true if they did.  z: in this CTA's sum of exponentials, out
+// the row's.
+template <int C>
+__device__ bool nucleus(RowSampler<C>& row, const SampleArgs& a, int r, const DrawArgs& d, float& z) {
+  SampleShared<C>& sh = row.sh;
+  const u64* hist = sh.hist[(row.turn - 1) & 1];
+  u64 v0 = 0, v1 = 0, all = 0;
+#pragma unroll
+  for (int p = 0; p < C; ++p) {
+    const ulonglong2 x = reinterpret_cast<const ulonglong2*>(row.peer(hist, p))[threadIdx.x];
+    v0 += x.x;
+    v1 += x.y;
+  }
+  const u64 incl = block_scan(sh, v0 + v1, &all), run = incl - v0 - v1, target = share_of(d.p, all);
+  if (run < target && incl >= target) sh.found[0] = 2 * threadIdx.x + (run + v0 < target);
+  __syncthreads();
+  return try_finish<false>(row, a, r, row.bin_floor((int)sh.found[0]), target, d, z);
 }
 
 // A bound below the row's k-th largest value from what each lane holds at most: where k lanes reach a
@@ -930,16 +943,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
   if (by_count) {
     if (try_finish<true>(row, a, r, sieve(row, st.top, bottom, d.k), 0, d, z)) return;
     fill_histogram<true>(row, kept);
-    shrink<true, false>(row, kept, a, r, d, z);
+    shrink<true>(row, kept, d, (row.turn - 1) & 1);
     if (kept.lo > kImgNegInf)
       row.per_unit = fminf((float)kSampleBins / (row.best - image_value(kept.lo)), 3e38f);
   }
   if (by_share) {
     fill_histogram<false>(row, kept);
-    if (by_count)
-      shrink<false, false>(row, kept, a, r, d, z);
-    else if (shrink<false, true>(row, kept, a, r, d, z))
-      return;
+    const int buffer = (row.turn - 1) & 1;
+    if (!by_count && nucleus(row, a, r, d, z)) return;
+    shrink<false>(row, kept, d, buffer);
   }
   const bool summed = by_count || by_share;  // z is the row's
 
