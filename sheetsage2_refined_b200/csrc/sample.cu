@@ -40,9 +40,9 @@
 // What bounds it: a few rows, the chain of exchanges (one row of 32,576 tokens,
 // top-k 50 and top-p: 12 us, of it 2 loading; 16 rows of 2,048: 5.3 us); many
 // rows, instruction issue and the barriers, not memory (1,024 rows of 32,576
-// float32 logits with mask, bias, top-k 200 and top-p: 143 us, 1.2 TB/s, half
+// float32 logits with mask, bias, top-k 200 and top-p: 136 us, 1.2 TB/s, half
 // of the issue slots; without the top-k sieve, so with every token's weight in
-// 64 bits, 249 us).
+// 64 bits, 245 us).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Share
 // What bounds a large call is the chain of one stream, S -> weights -> O (about
 // half of a tile's time passes in its barriers and the tensor memory's round
 // trips; the exponentials' unit is busy 54% of the time at dim 64), so as many
-// streams as fit run on an SM (1,024 rows of 16 heads over 16,384 tokens: 126 us,
-// 546 TFLOP/s):
+// streams as fit run on an SM (1,024 rows of 16 heads over 16,384 tokens: 120 us,
+// 575 TFLOP/s):
 //
 //   dim 64: P lies in S's columns, 256 columns and 98 KB a CTA, two CTAs an SM,
 //     four streams.  The next S of a stream follows the product that reads P;
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
   __shared__ int aborted;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int parts = a.shared_splits, tile = (int)blockIdx.x / parts, part = (int)blockIdx.x - tile * parts, g = blockIdx.y;
+  const int tile = blockIdx.x, g = blockIdx.y, part = blockIdx.z;  // (the parts' short last ones start last)
   const int group = a.heads / a.kv_heads, queries = a.rows * group;
   const int tile0 = tile * (PAIR ? 2 : 1);  // first query tile
 
@@ -601,7 +601,9 @@ __global__ void __launch_bounds__(kTileThreads, Tile<D, PAIR>::kPerSm)
   }
   pdl_wait();  // the queries come from the kernel before
   const int tokens = a.shared_len ? min(max(*a.shared_len, 0), a.shared_tokens) : a.shared_tokens;
-  const int tiles = (tokens + KT - 1) / KT, per = (tiles + parts - 1) / parts;
+  // every part `per` of the live tiles, in the proportion planned for all of them, the last what is left
+  const int tiles = (tokens + KT - 1) / KT, planned = (a.shared_tokens + KT - 1) / KT;
+  const int per = tiles == planned ? a.part_tiles : (int)(((long long)tiles * a.part_tiles + planned - 1) / planned);
   const int t0 = min(tiles, part * per), nt = min(tiles, t0 + per) - t0;
 
   auto fail = [&]() {
@@ -1028,9 +1030,7 @@ cudaError_t launch_tiles(const SharedAttnArgs& a, float* part_o, float2* part_ml
   static std::atomic<bool> done[64];
   const cudaError_t e = allow_smem(kernel, smem, done);
   if (e != cudaSuccess) return e;
-  const int tiles = PAIR ? (query_tiles(a) + 1) / 2 : query_tiles(a);
-  // (parts and tiles on one axis: up to 65,536 tiles)
-  return launch(kernel, dim3((unsigned)tiles * a.shared_splits, a.kv_heads), kTileThreads, smem, s, pdl, map_k, map_v, t);
+  return launch(kernel, dim3(a.query_blocks, a.kv_heads, a.shared_splits), kTileThreads, smem, s, pdl, map_k, map_v, t);
 }
 
 template <typename T, int D, bool WIDE>
@@ -1088,7 +1088,8 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     a.pair = tiles > 1;
     // the split with the fewest key tiles one after the other: waves of CTAs times the tiles of
     // each, plus about 6 tiles' time to start and end it
-    const long long ctas = (long long)(a.pair ? (tiles + 1) / 2 : tiles) * a.kv_heads;
+    a.query_blocks = a.pair ? (tiles + 1) / 2 : tiles;
+    const long long ctas = (long long)a.query_blocks * a.kv_heads;
     // Dim 64 runs two CTAs on an SM; a short shared part beside own pages takes one, or at dim 128, whose CTA
     // fills an SM, half of the SMs: the own part's warps have room from the start.  (Dim 64, 64 rows x 16 heads,
     // own rows of up to 1,500: over 2,048 shared tokens 54 -> 50 us, 8,192 57.4 -> 56.3, but 16,384 65.6 -> 67.9.
@@ -1098,12 +1099,30 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
     const long long slots = a.dim == 64 ? (brief ? sms : 2ll * sms) : (brief ? std::max(1, sms / 2) : sms);
     long long best = -1;
     for (int sp = 1; sp <= keys && sp <= kMaxSharedSplits; ++sp) {
-      const int per = (keys + sp - 1) / sp;
+      int per = (keys + sp - 1) / sp;
       if ((keys + per - 1) / per != sp) continue;  // the same tiles in fewer parts
-      const long long cost = (ctas * sp + slots - 1) / slots * (per + 6);
+      long long cost = (ctas * sp + slots - 1) / slots * (per + 6);
+      const long long room = slots - ctas * (sp - 1);
+      if (a.dim == 64 && per >= 48 && sp > 1 && room > 0 && room < ctas) {
+        // all but the last parts fill most of one wave: shorter last parts, `rounds` of them one after the
+        // other in what room is left, so that both end together (dim 64, 1,024 rows x 16 heads over 16,384
+        // tokens 126 -> 120 us, at dim 128, where a CTA starts on an SM by
+        // itself, 103 -> 116)
+        const long long rounds = (ctas + room - 1) / room;
+        const long long last = (keys + 6ll * (sp - 1) * (1 - rounds)) / (rounds * (sp - 1) + 1);
+        if (last > 0) {
+          const int most = (int)((keys - last + sp - 2) / (sp - 1));
+          const long long rest = keys - (long long)most * (sp - 1), even = std::max(most + 6ll, rounds * (rest + 6));
+          if (rest > 0 && rest <= most && even < cost) {
+            cost = even;
+            per = most;
+          }
+        }
+      }
       if (best < 0 || cost < best) {
         best = cost;
         a.shared_splits = sp;
+        a.part_tiles = per;
       }
     }
   }

@@ -37,6 +37,8 @@ struct SharedAttnArgs {
   int* error;  // null, or set to kErrOwn* when a row's pages are broken
   // set by plan_shared_attn
   int shared_splits, own_splits;  // parts of a (row, head)'s keys
+  int part_tiles;                 // key tiles of a shared part (the last has what is left)
+  int query_blocks;               // CTAs that a part's queries take
   bool pair;                      // two query tiles a CTA
   bool out_vector;                // out can be written 16 bytes at a time
   bool pdl;                       // the first launch may start while the kernel before it drains (it waits itself)

@@ -316,3 +316,16 @@ def test_short_and_long_shared_parts_beside_own_pages(dim, heads, kvh):
     for shared in (1111, 20000 if dim == 64 else 24000):
         q, k, v, own = make(24, heads, kvh, dim, shared, [(97 * r) % 500 for r in range(24)], BF16, seed=22)
         check(q, k, v, own, BF16)
+
+
+@gpu
+@pytest.mark.parametrize("live", [None, 16000, 5000, 40])
+def test_parts_of_unequal_length(live):
+    """Few query tiles over a long shared part: the last part of each is shorter, for every live length."""
+
+    q, k, v, _ = make(1000, 16, 16, 64, 16001, None, BF16, seed=23)
+    length = None if live is None else torch.tensor([live], dtype=torch.int32, device="cuda")
+    out, lse = ops.shared_attention(q, k, v, shared_len=length)
+    rows = [0, 127, 128, 511, 999]
+    seen = 16001 if live is None else live
+    assert_close(out[rows], lse[rows], exact(q[rows], k[:seen], v[:seen], None, None, None, None, 0.125), BF16)
