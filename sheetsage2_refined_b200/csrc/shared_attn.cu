@@ -1106,8 +1106,7 @@ size_t plan_shared_attn(SharedAttnArgs& a, int sms) {
       if (a.dim == 64 && per >= 48 && sp > 1 && room > 0 && room < ctas) {
         // all but the last parts fill most of one wave: shorter last parts, `rounds` of them one after the
         // other in what room is left, so that both end together (dim 64, 1,024 rows x 16 heads over 16,384
-        // tokens 126 -> 120 us, at dim 128, where a CTA starts on an SM by
-        // itself, 103 -> 116)
+        // tokens 126 -> 120 us; dim 128, where a CTA starts on an SM by itself, over 8,192 103 -> 116)
         const long long rounds = (ctas + room - 1) / room;
         const long long last = (keys + 6ll * (sp - 1) * (1 - rounds)) / (rounds * (sp - 1) + 1);
         if (last > 0) {
